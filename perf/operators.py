@@ -1,0 +1,339 @@
+"""The measured cases of three operators over embeddings, and their plain forms.
+
+    store    a store of embeddings held in 4 or 8 bits: rows are quantised as they are written into slots, and rows are
+             read back by index (the candidate memory of a training run, a corpus that grows)
+    scores   inner products of a few queries with every row of a 4-bit store, group scales applied in the product
+    distill  the loss that draws a retriever's softmax over its candidates towards a teacher's top list, with the
+             gradients of queries, candidates and temperature
+
+How the store holds a row of `dim` values, padded with zeros to whole pieces of 128:
+
+    fp4   groups of 32, 64 or 128 consecutive values; scale = max(bf16(max|x| / 6), 2^-120); a value is held as the nearest of
+          0, 0.5, 1, 1.5, 2, 3, 4, 6 times the scale (codes 0..7; ties to the even code; the sign is bit 3).  Within a piece
+          value k = 32 m + 8 c + j (m, c < 4, j < 8) is the nibble 32 c + 8 m + j, low nibble of a byte first.
+    i8    one scale per row: max|x| / 127 (1 for a row of zeros); code = rint(x / scale), |code| <= 127
+
+`run` computes the plain forms where `own` is false and calls the package where it is true; both take the same state.
+"""
+import math
+
+import torch
+
+own = False
+
+LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+# ---- the cases ---------------------------------------------------------------------------------------------------------
+
+def listed():
+    return [
+        # one document replaced and one read: what a call costs
+        {"name": "store one i8", "op": "store", "form": "i8", "group": 0, "dim": 896, "rows": 25_000, "writes": 1, "reads": 1,
+         "dtype": "f32", "out": "f32"},
+        # a training step: the step's candidates enter the memory, a draw of old ones comes back as negatives
+        {"name": "store step fp4", "op": "store", "form": "fp4", "group": 128, "dim": 4096, "rows": 65_536, "writes": 256,
+         "reads": 1024, "dtype": "f32", "out": "bf16"},
+        # a width that fills no whole piece, small groups, odd counts
+        {"name": "store ragged fp4", "op": "store", "form": "fp4", "group": 32, "dim": 900, "rows": 10_007, "writes": 1001,
+         "reads": 3001, "dtype": "bf16", "out": "f32"},
+        # a corpus loaded in one go and half of it read back
+        {"name": "store bulk i8", "op": "store", "form": "i8", "group": 0, "dim": 3584, "rows": 131_072, "writes": 131_072,
+         "reads": 65_536, "dtype": "f32", "out": "bf16"},
+        # one query over a caption set of an evaluation
+        {"name": "scores one small", "op": "scores", "dim": 3584, "rows": 5_000, "group": 64, "queries": 1, "dtype": "bf16"},
+        # one query over the share of a 3.3 M row corpus that one of eight GPUs holds
+        {"name": "scores one shard", "op": "scores", "dim": 4096, "rows": 412_500, "group": 128, "queries": 1, "dtype": "f32"},
+        # a small batch of queries, odd sizes throughout
+        {"name": "scores some", "op": "scores", "dim": 1000, "rows": 100_003, "group": 32, "queries": 13, "dtype": "f32"},
+        # a small retriever on one GPU
+        {"name": "distill small", "op": "distill", "batch": 32, "cands": 256, "memory": 0, "dim": 896, "list": 10,
+         "dtype": "f32", "grad": True},
+        # the training step of the contrastive loss, with a teacher's list of 64
+        {"name": "distill step", "op": "distill", "batch": 128, "cands": 1024, "memory": 0, "dim": 4096, "list": 64,
+         "dtype": "f32", "grad": True},
+        # the loss alone, as an evaluation asks for it
+        {"name": "distill eval bf16", "op": "distill", "batch": 1000, "cands": 5000, "memory": 0, "dim": 3584, "list": 10,
+         "dtype": "bf16", "grad": False},
+        # half-precision embeddings, their step's candidates and a memory of older ones
+        {"name": "distill memory bf16", "op": "distill", "batch": 512, "cands": 2048, "memory": 14_336, "dim": 3584, "list": 100,
+         "dtype": "bf16", "grad": True},
+        # the largest: a memory of 31 k candidates in fp32
+        {"name": "distill memory f32", "op": "distill", "batch": 256, "cands": 1024, "memory": 31_744, "dim": 4096, "list": 64,
+         "dtype": "f32", "grad": True},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(("store", "scores", "distill"))
+    dim = _log(rng, 64, 4096)
+    if rng.random() < 0.7:                                   # most encoders' widths are multiples of 8, some are odd
+        dim = dim // 8 * 8
+    dtype = rng.choice(("f32", "bf16"))
+    if op == "store":
+        form = rng.choice(("fp4", "i8"))
+        rows = _log(rng, 100, 131_072)
+        return {"op": op, "form": form, "group": rng.choice((32, 64, 128)) if form == "fp4" else 0, "dim": dim, "rows": rows,
+                "writes": _log(rng, 1, rows), "reads": _log(rng, 1, 65_536), "dtype": dtype, "out": rng.choice(("f32", "bf16"))}
+    if op == "scores":
+        return {"op": op, "dim": dim, "rows": _log(rng, 100, 412_500), "group": rng.choice((32, 64, 128)),
+                "queries": _log(rng, 1, 16), "dtype": dtype}
+    batch, cands, grad = _log(rng, 1, 512), _log(rng, 16, 4096), rng.random() < 0.75
+    room = (256 * 32_768 - batch * cands * 2) // batch        # no dearer than the largest listed case
+    memory = max(0, min(rng.choice((0, _log(rng, 100, 31_744))), room))
+    return {"op": op, "batch": batch, "cands": cands, "memory": memory, "dim": dim,
+            "list": min(_log(rng, 1, 128), cands), "dtype": dtype, "grad": grad}
+
+
+_SIZE = {"f32": 4, "bf16": 2}
+
+
+def _padded(dim):
+    return (dim + 127) // 128 * 128
+
+
+def work(case):
+    d = case["dim"]
+    if case["op"] == "store":
+        held = _padded(d) // 2 + _padded(d) // case["group"] * 2 if case["form"] == "fp4" else _padded(d) + 4
+        n, r = case["writes"], case["reads"]
+        return {"bytes": n * (d * _SIZE[case["dtype"]] + held + 8) + r * (held + d * _SIZE[case["out"]] + 8), "flops": n * d * 3 + r * d}
+    if case["op"] == "scores":
+        n, q = case["rows"], case["queries"]
+        return {"bytes": n * (_padded(d) // 2 + _padded(d) // case["group"] * 2) + q * d * _SIZE[case["dtype"]] + q * n * 4,
+                "flops": 2 * q * n * d}
+    b, c, m, s = case["batch"], case["cands"], case["memory"], _SIZE[case["dtype"]]
+    bytes_, flops = (b + c + m) * d * s + b * case["list"] * 12, 2 * b * (c + m) * d
+    if case["grad"]:
+        bytes_, flops = bytes_ + (b + c) * d * s, 2 * flops + 2 * b * c * d
+    return {"bytes": bytes_, "flops": flops}
+
+
+# ---- inputs ------------------------------------------------------------------------------------------------------------
+
+_TYPE = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def _unit(gen, n, d):
+    """Rows of length one whose coordinates differ in spread, as an encoder's do."""
+    x = torch.randn(n, d, device="cuda", generator=gen)
+    x *= torch.exp(0.5 * torch.randn(d, device="cuda", generator=gen))
+    return x / (x * x).sum(1, keepdim=True).sqrt()
+
+
+def _inputs(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    t = _TYPE[case["dtype"]]
+    if case["op"] == "store":
+        n, w, r = case["rows"], case["writes"], case["reads"]
+        first = int(torch.randint(n, (1,), generator=torch.Generator().manual_seed(seed)))
+        slots = (first + torch.arange(w, device="cuda")) % n                     # the next slots of a ring
+        index = torch.randint(n, (r,), device="cuda", generator=gen)
+        if r >= 8:
+            index[:: 2] = slots[torch.randint(w, (len(index[:: 2]),), device="cuda", generator=gen)]
+            index[5] = -1                                                        # no entry: a row of zeros
+        old = _unit(gen, min(n, 4096), case["dim"])
+        return {"old": old, "x": _unit(gen, w, case["dim"]).to(t), "slots": slots, "index": index}
+    if case["op"] == "scores":
+        return {"x": _unit(gen, case["rows"], case["dim"]), "q": _unit(gen, case["queries"], case["dim"]).to(t)}
+    b, c, m, d, k = case["batch"], case["cands"], case["memory"], case["dim"], case["list"]
+    q = _unit(gen, b, d)
+    p = _unit(gen, c, d)
+    n = min(b, c)
+    p[:n] = q[:n] + 0.8 * p[:n]
+    p = p / (p * p).sum(1, keepdim=True).sqrt()
+    index = torch.argsort(torch.rand(b, c + m, device="cuda", generator=gen), 1)[:, :k].contiguous()   # distinct columns
+    score = (torch.rand(b, k, device="cuda", generator=gen) * 0.6).sort(1, descending=True)[0].contiguous()
+    if b >= 8:                                                                    # a short list, and one with nothing in it
+        index[3, k // 2 + 1:], score[3, k // 2 + 1:] = -1, -math.inf
+        index[5], score[5] = -1, -math.inf
+    mem = _unit(gen, m, d).to(t) if m else None
+    return {"q": q.to(t), "p": p.to(t), "memory": mem, "index": index, "score": score, "tau": 0.07, "teacher_tau": 0.05}
+
+
+def prepare(case, seed):
+    s = _inputs(case, seed)
+    if case["op"] == "store":
+        n, old = case["rows"], s.pop("old")
+        data, scale = _fp4_pack(old, case["group"]) if case["form"] == "fp4" else _i8_pack(old)
+        at = torch.arange(n, device="cuda") % len(old)                            # what the slots hold before the call
+        return s | {"op": "store", "form": case["form"], "group": case["group"], "dim": case["dim"],
+                    "data": data[at].contiguous(), "scale": scale[at].contiguous(), "out": _TYPE[case["out"]]}
+    if case["op"] == "scores":
+        data, scale = _fp4_pack(s["x"], case["group"])
+        return {"op": "scores", "q": s["q"], "data": data, "scale": scale, "dim": case["dim"]}
+    s["temp"] = torch.tensor(s.pop("tau"), device="cuda", requires_grad=case["grad"])
+    s["q"].requires_grad_(case["grad"])
+    s["p"].requires_grad_(case["grad"])
+    return s | {"op": "distill", "grad": case["grad"]}
+
+
+# ---- the plain forms -----------------------------------------------------------------------------------------------------
+
+def _pad(x, to):
+    return x if x.shape[1] == to else torch.cat((x, x.new_zeros(x.shape[0], to - x.shape[1])), 1)
+
+
+def _fp4_pack(x, group):
+    """(packed codes uint8 [n, padded / 2], scales bf16 [n, padded / group]) of x [n, dim]."""
+    n, width = x.shape[0], _padded(x.shape[1])
+    g = _pad(x.float(), width).view(n, width // group, group)
+    a = g.abs()
+    scale = (a.amax(2).double() / 6).float().to(torch.bfloat16).float().clamp(min=2.0 ** -120)
+    s = scale[:, :, None]
+    # midpoints between neighbouring levels; a tie goes to the even code: up from 1 / 3 / 5 (>=), down to 0 / 2 / 4 / 6 (>)
+    code = ((a > 0.25 * s).to(torch.uint8) + (a >= 0.75 * s).to(torch.uint8) + (a > 1.25 * s).to(torch.uint8)
+            + (a >= 1.75 * s).to(torch.uint8) + (a > 2.5 * s).to(torch.uint8) + (a >= 3.5 * s).to(torch.uint8)
+            + (a > 5.0 * s).to(torch.uint8))
+    code = code + (g < 0).to(torch.uint8) * 8
+    code = code.view(n, width // 128, 4, 4, 8).transpose(2, 3).reshape(n, width // 2, 2)
+    return code[:, :, 0] + code[:, :, 1] * 16, scale.to(torch.bfloat16)
+
+
+def _fp4_unpack(data, scale, dim):
+    n, width = data.shape[0], data.shape[1] * 2
+    code = torch.stack((data & 15, data >> 4), 2).view(n, width // 128, 4, 4, 8).transpose(2, 3).reshape(n, width)
+    level = torch.tensor(LEVELS, device=data.device)[(code & 7).int()]
+    level = torch.where(code > 7, -level, level).view(n, scale.shape[1], -1)
+    return (level * scale.float()[:, :, None]).view(n, width)[:, :dim]
+
+
+def _i8_pack(x):
+    x = x.float()
+    top = x.abs().amax(1)
+    scale = torch.where(top > 0, (top.double() / 127).float(), 1.0)
+    code = (x.double() / scale.double()[:, None]).float().round().clamp(-127, 127).to(torch.int8)
+    return _pad(code, _padded(x.shape[1])), scale
+
+
+def _plain_store(s):
+    data, scale = _fp4_pack(s["x"], s["group"]) if s["form"] == "fp4" else _i8_pack(s["x"])
+    s["data"][s["slots"]] = data
+    s["scale"][s["slots"]] = scale
+    at = s["index"].clamp(min=0)
+    if s["form"] == "fp4":
+        x = _fp4_unpack(s["data"][at], s["scale"][at], s["dim"])
+    else:
+        x = s["data"][at][:, : s["dim"]].float() * s["scale"][at][:, None]
+    return torch.where((s["index"] >= 0)[:, None], x, 0.0).to(s["out"])
+
+
+def _plain_scores(s):
+    return s["q"].float() @ _fp4_unpack(s["data"], s["scale"], s["dim"]).t()
+
+
+def _plain_distill(s):
+    cand = s["p"].float() if s["memory"] is None else torch.cat((s["p"].float(), s["memory"].float()), 0)
+    z = s["q"].float() @ cand.t() / s["temp"]
+    top, best = z.max(1)
+    lse = top + (z - top[:, None]).exp().sum(1).log()
+    there = (s["index"] >= 0) & (s["score"] > -math.inf)
+    some = there.any(1)
+    score = torch.where(there, s["score"].float() / s["teacher_tau"], -math.inf)
+    first = torch.where(some, score.max(1)[0], 0.0)
+    e = (score - first[:, None]).exp()
+    t = e / e.sum(1, keepdim=True).clamp(min=1e-30)
+    log_t = torch.where(t > 0, t, 1.0).log()
+    picked = z.gather(1, s["index"].clamp(min=0))
+    row = torch.where(some, (t * (log_t - picked + lse[:, None])).sum(1), 0.0)
+    rows = some.sum().clamp(min=1)
+    loss = row.sum() / rows
+    teacher = s["index"].gather(1, score.max(1)[1][:, None])[:, 0]
+    agree = ((best == teacher) & some).sum() / rows
+    return loss, agree
+
+
+def run(s):
+    if own:
+        return _own(s)
+    if s["op"] == "store":
+        return _plain_store(s)
+    if s["op"] == "scores":
+        return _plain_scores(s)
+    if not s["grad"]:
+        with torch.no_grad():
+            return _plain_distill(s)
+    loss, agree = _plain_distill(s)
+    return (loss.detach(), agree) + torch.autograd.grad(loss, (s["q"], s["p"], s["temp"]))
+
+
+# ---- the package's operators ---------------------------------------------------------------------------------------------
+
+def _own(s):
+    from vllm_amd import kernels
+    from vllm_amd.loss import compute_distillation_loss
+    if s["op"] == "store":
+        kernels.store_write(s["x"], s["slots"], s["data"], s["scale"])
+        return kernels.store_read(s["index"], s["data"], s["scale"], s["dim"], dtype=s["out"])
+    if s["op"] == "scores":
+        return kernels.store_scores(s["q"], s["data"], s["scale"])
+    if not s["grad"]:
+        with torch.no_grad():
+            return compute_distillation_loss(s["q"], s["p"], s["temp"], s["index"], s["score"],
+                                             teacher_temperature=s["teacher_tau"], memory=s["memory"])
+    loss, agree = compute_distillation_loss(s["q"], s["p"], s["temp"], s["index"], s["score"],
+                                            teacher_temperature=s["teacher_tau"], memory=s["memory"])
+    return (loss.detach(), agree) + torch.autograd.grad(loss, (s["q"], s["p"], s["temp"]))
+
+
+# ---- the definitions in 64 bits --------------------------------------------------------------------------------------------
+
+def _held(x, form, group):
+    """The values that the store holds for the rows of x, in 64 bits."""
+    x = x.double()
+    n, d = x.shape
+    if form == "i8":
+        top = x.abs().max(1, keepdim=True)[0]
+        scale = (top / 127).float().double()
+        scale[top == 0] = 1.0
+        return torch.clamp((x / scale).float().double().round(), -127, 127) * scale
+    full = torch.zeros(n, _padded(d), dtype=torch.float64, device=x.device)
+    full[:, :d] = x
+    full = full.reshape(n, -1, group)
+    scale = (full.abs().max(2, keepdim=True)[0] / 6).float().bfloat16().double()
+    scale = torch.maximum(scale, torch.full_like(scale, 2.0 ** -120))
+    y = full.abs() / scale
+    # the spacing of the levels is 1/2 below 2, 1 up to 4 and 2 up to 6; rounding to an even multiple is the even code
+    step = torch.where(y < 2, 0.5, torch.where(y < 4, 1.0, 2.0)).double()
+    y = ((y / step).round() * step).clamp(max=6.0)
+    return (torch.sign(full) * y * scale).reshape(n, -1)[:, :d]
+
+
+def exact(case, seed):
+    s = _inputs(case, seed)
+    if case["op"] == "store":
+        n = case["rows"]
+        old = _held(s["old"], case["form"], case["group"])
+        new = _held(s["x"], case["form"], case["group"])
+        writer = torch.full((n,), -1, dtype=torch.int64, device="cuda")
+        writer[s["slots"]] = torch.arange(len(s["slots"]), device="cuda")
+        at = s["index"]
+        by = writer[at.clamp(min=0)]
+        rows = torch.where((by >= 0)[:, None], new[by.clamp(min=0)], old[at.clamp(min=0) % len(old)])
+        return rows * (at >= 0)[:, None]
+    if case["op"] == "scores":
+        return torch.matmul(s["q"].double(), _held(s["x"], "fp4", case["group"]).t())
+    q, p = s["q"].double(), s["p"].double()
+    c = p if s["memory"] is None else torch.cat((p, s["memory"].double()))
+    tau = float(torch.tensor(s["tau"], dtype=torch.float32))
+    dots = q @ c.t()
+    z = dots / tau
+    logp = torch.log_softmax(z, 1)
+    live = (s["index"] >= 0) & torch.isfinite(s["score"])
+    want = torch.softmax(torch.where(live, s["score"].double() / s["teacher_tau"], -1e300), 1) * live
+    some = live.any(1)
+    count = max(1, int(some.sum()))
+    target = torch.zeros_like(z).scatter_add_(1, s["index"].clamp(min=0), want)
+    entropy = torch.where(want > 0, want * torch.log(torch.where(want > 0, want, 1.0)), 0.0).sum()
+    loss = (entropy - (target * logp).sum()) / count
+    best = torch.where(live, s["score"].double(), -math.inf).argmax(1)
+    chosen = s["index"][torch.arange(len(best), device="cuda"), best]
+    agree = ((z.argmax(1) == chosen) & some).double().sum() / count
+    if not case["grad"]:
+        return loss, agree
+    g = (torch.exp(logp) - target) * some[:, None] / count
+    return (loss, agree, g @ c / tau, (g.t() @ q / tau)[: len(p)], -(g * dots).sum() / tau ** 2)
