@@ -265,12 +265,12 @@ def run(s):
 
 def _own(s):
     from vllm_amd import kernels
-    from vllm_amd.loss import compute_distillation_loss
     if s["op"] == "store":
         kernels.store_write(s["x"], s["slots"], s["data"], s["scale"])
         return kernels.store_read(s["index"], s["data"], s["scale"], s["dim"], dtype=s["out"])
     if s["op"] == "scores":
         return kernels.store_scores(s["q"], s["data"], s["scale"])
+    from vllm_amd.loss import compute_distillation_loss
     if not s["grad"]:
         with torch.no_grad():
             return compute_distillation_loss(s["q"], s["p"], s["temp"], s["index"], s["score"],
