@@ -239,6 +239,34 @@ int abc_mean_pool_bwd_f32(const float* dx, const int64_t* ids, int64_t pad_id, c
                           float* dhidden, void* stream);
 
 /*
+ * A store of embeddings held in 4 or 8 bits (no counterpart in the reference, whose corpora are fp32 tensors that never change):
+ * rows are quantised as they are written into slots of a resident matrix and read back by index.  dim in [1, 8192]; a row is held
+ * padded with zeros to width = dim rounded up to 128.
+ *   group = 0          i8: data [capacity, width] i8, scale [capacity] f32, abc_quantize_i8's rule (abc_topk_i8 takes data and scale)
+ *   group = 32|64|128  fp4: data [capacity, width / 2] u8, scale [capacity, width / group] bf16.  Per group of consecutive values
+ *                      scale = max(bf16(max|x| / 6), 2^-120) and codes 0..7 for the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times the
+ *                      scale (ties to the even code), sign in bit 3.  Value k = 32 m + 8 c + j (m, c < 4, j < 8) of a piece of 128 is
+ *                      nibble 32 c + 8 m + j of the piece's 64 bytes, low nibble first.
+ *   A row (i8) or group (fp4) with an infinity or a NaN gets scale NaN and codes 0.
+ * data must be 16-byte aligned, fp4 scales to 256 / group bytes (any row of a store is).  x and out may have any alignment of their element and any row stride
+ * (ldx, ldo: elements, >= dim).  x_dtype / out_dtype / q_dtype: ABC_DT_F32 or ABC_DT_BF16.
+ *
+ * abc_store_write: row i of x goes to slot slots[i], or to (first + i) % capacity where slots is null (n <= capacity then).  A slot
+ *   outside [0, capacity) drops its row; of rows that name one slot the last is kept.
+ *   workspace >= abc_store_write_workspace_bytes(n, capacity) where slots is given (0 up to 1024 rows).
+ * abc_store_read: out[i, :] = the values held by row index[i] (first + i where index is null); index < 0 gives zeros, index >=
+ *   capacity NaN.  fp32 products code * scale, rounded once to bf16 where out is bf16.
+ * abc_store_scores (fp4): out[i, n] = q[i, :] . (values of row n), n < rows; fp32 sums, fp32 queries at full precision.
+ */
+size_t abc_store_write_workspace_bytes(int64_t n, int64_t capacity);
+int abc_store_write(int x_dtype, const void* x, int64_t ldx, const int64_t* slots, int64_t first, int64_t n, int dim, void* data,
+                    void* scale, int64_t capacity, int group, void* workspace, size_t workspace_bytes, void* stream);
+int abc_store_read(const int64_t* index, int64_t first, int64_t n, const void* data, const void* scale, int64_t capacity, int dim,
+                   int group, int out_dtype, void* out, int64_t ldo, void* stream);
+int abc_store_scores(int q_dtype, const void* q, int64_t ldq, int64_t nq, const void* data, const void* scale, int64_t rows, int dim,
+                     int group, float* out, int64_t ldo, void* stream);
+
+/*
  * negatives.json text, host code (no GPU, no stream).  Replaces the serialisation half of
  * pretrain/create_negative_index.py:40-43 (json.dump(negative_dict, f) over {int idx: [100 ints]}): the bytes json.dump
  * writes for rows first_row .. first_row + n_rows - 1 -- `"17": [3, 5, 8]` entries joined by ", ", keys as strings, no

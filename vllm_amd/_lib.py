@@ -47,6 +47,10 @@ SIGNATURES = {
     "abc_embed_head_bwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "abc_mean_pool_bwd_bf16": (_int, [_vp, _vp, _i64, _vp, _int, _int, _int, _vp, _vp]),
     "abc_mean_pool_bwd_f32": (_int, [_vp, _vp, _i64, _vp, _int, _int, _int, _vp, _vp]),
+    "abc_store_write_workspace_bytes": (_sz, [_i64, _i64]),
+    "abc_store_write": (_int, [_int, _vp, _i64, _vp, _i64, _i64, _int, _vp, _vp, _i64, _int, _vp, _sz, _vp]),
+    "abc_store_read": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _int, _int, _int, _vp, _i64, _vp]),
+    "abc_store_scores": (_int, [_int, _vp, _i64, _i64, _vp, _vp, _i64, _int, _int, _vp, _i64, _vp]),
     "abc_infonce_bwd": (_int, [_vp, _vp, _vp, _vp, _f32, _vp, _int, _int, _int, _int, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 

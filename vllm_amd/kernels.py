@@ -224,6 +224,133 @@ def cast_bf16(x: torch.Tensor) -> torch.Tensor:
     return out
 
 
+# ---- rows held in 4 or 8 bits -------------------------------------------------------------------------------------------
+def _store_form(data: torch.Tensor, scale: torch.Tensor) -> Tuple[int, int]:
+    """(group, width) of a store's pair of tensors: int8 rows with one fp32 scale each (group 0), or packed 4-bit rows (uint8)
+    with bf16 scales for groups of 32 / 64 / 128 values."""
+    _need_gpu(data, scale)
+    if data.dim() != 2 or not data.is_contiguous() or not scale.is_contiguous() or data.device != scale.device:
+        raise _lib.AbcError("store: data and scale must be contiguous matrices on one device")
+    if data.dtype == torch.int8:
+        if scale.dtype != torch.float32 or tuple(scale.shape) != (data.shape[0],) or data.shape[1] % 128 or data.shape[1] == 0:
+            raise _lib.AbcError(f"store: int8 rows {tuple(data.shape)} need a width of whole 128s and fp32 scales [rows], "
+                                f"got {scale.dtype} {tuple(scale.shape)}")
+        return 0, data.shape[1]
+    if data.dtype != torch.uint8 or scale.dtype != torch.bfloat16 or scale.dim() != 2 or scale.shape[0] != data.shape[0]:
+        raise _lib.AbcError(f"store: {data.dtype} rows with {scale.dtype} scales: int8 + fp32 or uint8 + bf16 [rows, groups]")
+    width = data.shape[1] * 2
+    group = width // scale.shape[1] if scale.shape[1] else 0
+    if width == 0 or width % 128 or group not in (32, 64, 128) or group * scale.shape[1] != width:
+        raise _lib.AbcError(f"store: 4-bit rows of {width} values with {scale.shape[1]} scales: groups of 32, 64 or 128 and a "
+                            "width of whole 128s")
+    return group, width
+
+
+def _store_dim(dim: int, width: int) -> int:
+    if not width - 128 < dim <= width:
+        raise _lib.AbcError(f"store: {dim} values a row do not belong in rows of {width}")
+    return int(dim)
+
+
+def _index64(index: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor:
+    if index.dtype not in (torch.int64, torch.int32):
+        raise _lib.AbcError(f"{what} must be int64 or int32, got {index.dtype}")
+    if index.device != like.device:
+        raise _lib.AbcError(f"{what} on {index.device}, the store on {like.device}")
+    return index.to(torch.int64).contiguous()
+
+
+def _rows_of(x: torch.Tensor) -> torch.Tensor:
+    """x with unit stride along its rows (the kernels take any row stride from the width up)."""
+    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+
+
+def store_write(x: torch.Tensor, slots: Optional[torch.Tensor], data: torch.Tensor, scale: torch.Tensor, first: int = 0) -> None:
+    """Quantise the rows of x [n, dim] (f32 / bf16) into the given slots of a store, in place; slots None: the n slots from
+    `first` on, past the last one on from 0.  A slot outside the store drops its row (-1 = padding), and of rows that name the same slot
+    the last one stays."""
+    group, width = _store_form(data, scale)
+    _need_gpu(x, slots)
+    if x.dim() != 2 or x.dtype not in (torch.float32, torch.bfloat16) or x.device != data.device:
+        raise _lib.AbcError(f"store_write: expected f32 / bf16 rows [n, dim] on {data.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    dim, n, capacity = _store_dim(x.shape[1], width), x.shape[0], data.shape[0]
+    if slots is not None:
+        slots = _index64(slots, data, "slots")
+        if slots.shape != (n,):
+            raise _lib.AbcError(f"store_write: {n} rows but slots {tuple(slots.shape)}")
+    elif n and (n > capacity or not 0 <= first < capacity):
+        raise _lib.AbcError(f"store_write: {n} rows from slot {first} do not fit a store of {capacity}")
+    if n == 0:
+        return
+    x = _rows_of(x.detach())
+    lib = _lib.load()
+    need = lib.abc_store_write_workspace_bytes(n, capacity) if slots is not None else 0
+    with _on(data):
+        # scratch of its own, not the per-stream cache: a captured graph keeps it for itself
+        ws = torch.empty(need, dtype=torch.uint8, device=data.device) if need else None
+        rc = lib.abc_store_write(_DT[x.dtype], x.data_ptr(), x.stride(0) if n > 1 else dim, _ptr(slots), int(first), n, dim,
+                                 data.data_ptr(), scale.data_ptr(), capacity, group, _ptr(ws), need, _stream(data))
+    _lib.check(rc, "abc_store_write")
+
+
+def store_read(index: Optional[torch.Tensor], data: torch.Tensor, scale: torch.Tensor, dim: int, dtype: torch.dtype = torch.float32,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The values that rows `index` (any shape; None: every row) of a store hold, f32 or bf16 [*index.shape, dim].  A negative
+    index reads as a row of zeros (the -1 of a top-k list), an index past the store as a row of NaN.  `out`: a tensor of that shape to
+    write into, its last dimension contiguous and its rows evenly spaced (a slice of a larger buffer)."""
+    group, width = _store_form(data, scale)
+    dim = _store_dim(dim, width)
+    if out is not None:
+        dtype = out.dtype
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise _lib.AbcError(f"store_read: rows are read as f32 or bf16, not {dtype}")
+    shape = (data.shape[0],) if index is None else tuple(index.shape)
+    if index is not None:
+        _need_gpu(index)
+        index = _index64(index, data, "index").reshape(-1)
+    n = data.shape[0] if index is None else index.numel()
+    if out is None:
+        out = torch.empty(shape + (dim,), dtype=dtype, device=data.device)
+    elif tuple(out.shape) != shape + (dim,) or out.device != data.device:
+        raise _lib.AbcError(f"store_read: out is {tuple(out.shape)} on {out.device}, expected {shape + (dim,)} on {data.device}")
+    elif out.requires_grad:
+        raise _lib.AbcError("store_read: out must not require a gradient (what is read back is constant)")
+    if n == 0:
+        return out
+    try:
+        rows = out.view(-1, dim)
+    except RuntimeError:
+        raise _lib.AbcError("store_read: the rows of out are not evenly spaced") from None
+    if rows.stride(1) != 1 and dim > 1 or (n > 1 and rows.stride(0) < dim):
+        raise _lib.AbcError("store_read: the last dimension of out must be contiguous and its rows must not overlap")
+    lib = _lib.load()
+    with _on(data):
+        rc = lib.abc_store_read(_ptr(index), 0, n, data.data_ptr(), scale.data_ptr(), data.shape[0], dim, group, _DT[dtype],
+                                rows.data_ptr(), rows.stride(0) if n > 1 else dim, _stream(data))
+    _lib.check(rc, "abc_store_read")
+    return out
+
+
+def store_scores(q: torch.Tensor, data: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """f32 [nq, rows]: inner products of the queries q [nq, dim] (f32 / bf16) with every row of a 4-bit store.  For a few queries,
+    where the stream over the store is the cost; a large set of them belongs in topk."""
+    group, width = _store_form(data, scale)
+    _need_gpu(q)
+    if group == 0:
+        raise _lib.AbcError("store_scores: the 4-bit form only (an int8 store is searched by topk)")
+    if q.dim() != 2 or q.dtype not in (torch.float32, torch.bfloat16) or q.device != data.device:
+        raise _lib.AbcError(f"store_scores: expected f32 / bf16 queries [nq, dim] on {data.device}, got {q.dtype} {tuple(q.shape)} on {q.device}")
+    dim, nq, rows = _store_dim(q.shape[1], width), q.shape[0], data.shape[0]
+    q = _rows_of(q.detach())
+    out = torch.empty((nq, rows), dtype=torch.float32, device=q.device)
+    lib = _lib.load()
+    with _on(q):
+        rc = lib.abc_store_scores(_DT[q.dtype], q.data_ptr(), q.stride(0) if nq > 1 else dim, nq, data.data_ptr(), scale.data_ptr(),
+                                  rows, dim, group, out.data_ptr(), rows, _stream(q))
+    _lib.check(rc, "abc_store_scores")
+    return out
+
+
 def debug_set(name: str, value: int) -> None:
     """Diagnostics hook of the library (tests, timing scripts): "flags", "plan_qb"."""
     _lib.check(_lib.load().abc_debug_set(name.encode(), int(value)), "abc_debug_set")

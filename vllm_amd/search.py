@@ -73,6 +73,88 @@ class Embeddings:
         return out
 
 
+class EmbeddingStore:
+    """Embeddings held in 4 or 8 bits that change while they are in use: rows are quantised as they are written into slots, and
+    read back by index -- a corpus that grows, the candidates of earlier training steps kept as negatives.
+
+    form "fp4": 4-bit codes (e2m1) with a bf16 scale for every `group` (32, 64 or 128) values, 0.52 bytes a value at 128; `scores` runs a
+    few queries over it.  form "i8": the int8 rows of Embeddings(x, "i8"), one fp32 scale each; `embeddings` hands them to topk.
+
+    Calls on one store run in the order of the stream they are made on; a store used on two streams is the caller's to order, like
+    any tensor.  Slots that nothing was written to hold zeros.  No counterpart in the reference (its corpora are saved fp32 tensors)."""
+
+    def __init__(self, capacity: int, dim: int, form: str = "fp4", group: int = 128, device=None):
+        if form not in ("fp4", "i8"):
+            raise AbcError(f"form must be fp4 or i8, not {form}")
+        if form == "fp4" and group not in (32, 64, 128):
+            raise AbcError(f"group must be 32, 64 or 128, not {group}")
+        if not 0 < int(capacity) < 1 << 31 or not 1 <= int(dim) <= 8192:
+            raise AbcError(f"a store of {capacity} rows of {dim} values: 1 to 2^31 - 1 rows of 1 to 8192 values")
+        dev = _device(device)
+        width = (int(dim) + 127) // 128 * 128
+        self.capacity, self.dim, self.form, self._next = int(capacity), int(dim), form, 0
+        if form == "fp4":
+            self.data = torch.zeros((self.capacity, width // 2), dtype=torch.uint8, device=dev)
+            self.scale = torch.zeros((self.capacity, width // group), dtype=torch.bfloat16, device=dev)
+        else:
+            self.data = torch.zeros((self.capacity, width), dtype=torch.int8, device=dev)
+            self.scale = torch.ones((self.capacity,), dtype=torch.float32, device=dev)
+
+    def write(self, x: torch.Tensor, slots: torch.Tensor) -> None:
+        """Row i of x [n, dim] (f32 / bf16) replaces what slot slots[i] holds; a slot outside the store drops its row, and of rows
+        that name the same slot the last one stays."""
+        if slots is None:
+            raise AbcError("write needs slots; append takes the next ones")
+        self._width(x)
+        kernels.store_write(x, slots, self.data, self.scale)
+
+    def append(self, x: torch.Tensor) -> int:
+        """Write x into the next slots, past the last one on from slot 0, over the oldest rows; returns the first slot taken.
+        The position is the host's: a captured graph would write the same slots at every replay, so capture is refused (use write)."""
+        self._width(x)
+        n = x.shape[0]
+        if n > self.capacity:
+            raise AbcError(f"{n} rows do not fit a store of {self.capacity}")
+        if torch.cuda.is_current_stream_capturing():
+            raise AbcError("append cannot be captured into a graph: its position is kept on the host; use write with slots")
+        first = self._next
+        kernels.store_write(x, None, self.data, self.scale, first)
+        self._next = (first + n) % self.capacity
+        return first
+
+    def read(self, index: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float32,
+             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The values of rows `index` (any shape; None: all), [*index.shape, dim] f32 / bf16.  Negative: zeros (the -1 of a top-k
+        list); past the store: NaN.  `out`: a tensor to write into."""
+        return kernels.store_read(index, self.data, self.scale, self.dim, dtype, out)
+
+    def rows(self, lo: int, hi: int) -> "EmbeddingStore":
+        """Slots [lo, hi) as a store of their own, sharing this one's memory."""
+        if not 0 <= lo < hi <= self.capacity:
+            raise AbcError(f"rows [{lo}, {hi}) of a store of {self.capacity}")
+        out = object.__new__(EmbeddingStore)
+        out.capacity, out.dim, out.form, out._next = hi - lo, self.dim, self.form, 0
+        out.data, out.scale = self.data[lo:hi], self.scale[lo:hi]
+        return out
+
+    def scores(self, q: torch.Tensor) -> torch.Tensor:
+        """f32 [nq, capacity]: inner products of a few queries q [nq, dim] (f32 / bf16) with every row (fp4 form)."""
+        self._width(q)
+        return kernels.store_scores(q, self.data, self.scale)
+
+    def embeddings(self) -> Embeddings:
+        """The int8 rows as a corpus for topk / mine_negatives, sharing this store's memory (i8 form)."""
+        if self.form != "i8":
+            raise AbcError("topk contracts int8 rows: the fp4 form is searched by scores")
+        emb = object.__new__(Embeddings)
+        emb.compute, emb.data, emb.scale = "i8", self.data, self.scale
+        return emb
+
+    def _width(self, x: torch.Tensor) -> None:
+        if x.dim() != 2 or x.shape[1] != self.dim:
+            raise AbcError(f"expected rows of {self.dim} values, got {tuple(x.shape)}")
+
+
 def topk(q: Embeddings, c: Embeddings, k: int, upper_bound=None, idx_offset: int = 0, rank_ref=None,
          rank_self_offset=None):
     """Exact top-k of q @ c.T (values, indices[, rank counts]) on the GPU."""
