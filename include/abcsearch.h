@@ -191,6 +191,30 @@ int abc_infonce_bwd(const float* q, const float* p, const float* lse, const floa
                     void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Distillation from a teacher's top list (no counterpart in the reference; stands beside the InfoNCE loss): queries q [B,d], the
+ * step's candidates p [C,d] and M further candidates memory [M,d] that are constants (null where M = 0), all f32 or all bf16
+ * (dtype); candidate j >= C is row j - C of memory, T = C + M.
+ *   z = (q @ cand^T) / temp;  teacher_idx [B,k] i64 / teacher_score [B,k] f32: the teacher's list of each query, as abc_topk_*
+ *   returns it (an index < 0 or a score of -inf is no entry; an index >= T makes the row NaN; an index may come twice)
+ *   t_b = softmax over row b's entries of score / teacher_temp;  row_b = sum_i t_bi (log t_bi - z_b,idx) + logsumexp_j z_bj
+ *   out_loss [1] f32: mean of row_b over the rows that have an entry (0 where none has)
+ *   out_agree [1] f32: share of those rows whose best candidate (argmax z) is the best entry of the list
+ *   B in [1, 65535], d % 8 == 0, d <= 65536, k in [1, 1024].
+ * abc_distill_bwd: `fwd_ws` is the workspace abc_distill_fwd was given for the same arguments, unchanged since (it is only read:
+ *   the backward may run more than once).  dq [B,d], dp [C,d] in dtype, d_temp [1] f32, each nullable (not computed), overwritten;
+ *   grad_out is a device scalar.  Rows without an entry receive no gradient.
+ * Both workspaces may hold anything before; nothing is kept in the library between calls; results do not vary from run to run.
+ */
+size_t abc_distill_workspace_bytes(int dtype, int64_t B, int64_t C, int64_t M, int d, int k);
+int abc_distill_fwd(int dtype, const void* q, const void* p, const void* memory, const float* temp, const int64_t* teacher_idx,
+                    const float* teacher_score, float teacher_temp, int64_t B, int64_t C, int64_t M, int d, int k, float* out_loss,
+                    float* out_agree, void* workspace, size_t workspace_bytes, void* stream);
+size_t abc_distill_bwd_workspace_bytes(int dtype, int64_t B, int64_t C, int64_t M, int d, int k);
+int abc_distill_bwd(int dtype, const void* q, const void* p, const void* memory, const float* temp, const int64_t* teacher_idx,
+                    const float* grad_out, int64_t B, int64_t C, int64_t M, int d, int k, void* dq, void* dp, float* d_temp,
+                    const void* fwd_ws, size_t fwd_ws_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Embedding epilogue: the step that produces the vectors the search and the loss consume.
  *
  * Mean pool.  Replaces get_mean_token_embed, model/abc_util.py:33-41:

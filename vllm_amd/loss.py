@@ -3,6 +3,7 @@
     Temperature               model/modeling_abc.py:36-43
     compute_contrastive_loss  model/abc_util.py:43-56
     compute_gathered_loss     model/abc_util.py:5-31
+    compute_distillation_loss (no counterpart in the reference: a teacher's top list instead of the one positive)
 
 The logits / logsumexp / label-smoothed cross entropy / argmax and their backward run in
 libabcsearch.so (abc_infonce_fwd / abc_infonce_bwd, exact fp32 on the matrix cores); the candidate
@@ -12,6 +13,7 @@ from __future__ import annotations
 
 import torch
 import torch.distributed as dist
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .kernels import _on, _stream
@@ -139,7 +141,11 @@ def _loss_and_acc(q_embeds, p_embeds, temperature, label_smoothing, local_rows, 
         temp = temp.to(q_embeds.device)
     if p_local is None:
         p_local = p_embeds if local_rows == p_embeds.shape[0] else p_embeds[:local_rows]
+    held = None
+    if torch.is_grad_enabled() and q_embeds.is_cuda and torch.cuda.is_current_stream_capturing():
+        held = _captured_leaves((q_embeds, p_embeds, temp), refuse=False)
     loss, accuracy = _InfoNCE.apply(q_embeds, p_embeds.detach(), p_local, temp, float(label_smoothing))
+    del held
     return loss, accuracy
 
 
@@ -148,6 +154,146 @@ def compute_contrastive_loss(q_embeds, p_embeds, temperature, label_smoothing=0.
     accuracy.  Same call and return as model/abc_util.py:43-56; differentiable w.r.t. q_embeds,
     p_embeds and temperature.temp."""
     return _loss_and_acc(q_embeds, p_embeds, temperature, label_smoothing, p_embeds.size(0))
+
+
+def _captured_leaves(leaves, refuse: bool) -> list:
+    """Under graph capture: mark the gradient nodes of these leaves as the capturing stream's, and (refuse) raise where a leaf's node was
+    there before.  A leaf has one gradient node while any autograd graph of it lives, bound to the stream that graph was built on; a
+    captured backward that reaches a node of an eager graph makes the eager stream wait inside the capture, which ends the process when the
+    capture ends.  Whether a node was there before: one that only this function holds is gone when it lets go, with its mark.
+    Returns the marked nodes: hold them until the call's own graph does."""
+    held = []
+    for x in leaves:
+        if not (torch.is_tensor(x) and x.requires_grad and x.is_leaf):
+            continue
+        stream = torch.cuda.current_stream(x.device).cuda_stream
+        node = torch.autograd.graph.get_gradient_edge(x).node
+        mine = node.metadata.get("abc_capture") == stream
+        node.metadata["abc_probe"] = True
+        del node
+        node = torch.autograd.graph.get_gradient_edge(x).node
+        if node.metadata.pop("abc_probe", False) and not mine:
+            if refuse:
+                raise _lib.AbcError(
+                    "capture: an autograd graph of a leaf (queries, candidates or temperature) is alive from before; its gradient belongs to "
+                    "another stream and capturing this backward would end the process.  Drop earlier losses and outputs of these leaves "
+                    "before the capture (inside one capture: call this loss first, or hand it x * 1)")
+            continue
+        node.metadata["abc_capture"] = stream
+        held.append(node)
+    return held
+
+
+class _Distill(torch.autograd.Function):
+    """loss, agreement = distillation from a teacher's list.  `memory` and the list are constants."""
+
+    @staticmethod
+    def forward(ctx, q, p, temp, memory, index, score, teacher_temp: float):
+        lib = _lib.load()
+        B, d = q.shape
+        C, M, k = p.shape[0], 0 if memory is None else memory.shape[0], index.shape[1]
+        dtype = _lib.DT_BF16 if q.dtype is torch.bfloat16 else _lib.DT_F32
+        need = lib.abc_distill_workspace_bytes(dtype, B, C, M, d, k)
+        if need == 0:
+            _lib.check(-1, "abc_distill_workspace_bytes")
+        dev = q.device
+        t = temp if (temp.dtype is torch.float32 and temp.device == dev) else temp.detach().to(device=dev, dtype=torch.float32)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        agree = torch.empty((), dtype=torch.float32, device=dev)
+        with _on(q):
+            # scratch of its own (the caching allocator's, in stream order): two losses alive, or two captured graphs, share nothing
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            rc = lib.abc_distill_fwd(dtype, q.data_ptr(), p.data_ptr(), None if M == 0 else memory.data_ptr(), t.data_ptr(),
+                                     index.data_ptr(), score.data_ptr(), teacher_temp, B, C, M, d, k, loss.data_ptr(), agree.data_ptr(),
+                                     ws.data_ptr(), need, _stream(q))
+        _lib.check(rc, "abc_distill_fwd")
+        ctx.save_for_backward(q, p, t, memory, index)
+        ctx.ws = ws
+        ctx.meta = (dtype, B, C, M, d, k, temp.dtype, tuple(temp.shape))
+        ctx.mark_non_differentiable(agree)
+        return loss, agree
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss, _grad_agree):
+        q, p, t, memory, index = ctx.saved_tensors
+        dtype, B, C, M, d, k, tdtype, tshape = ctx.meta
+        lib = _lib.load()
+        need_q, need_p, need_t = ctx.needs_input_grad[:3]
+        go = _f32c(grad_loss)
+        dev = q.device
+        dq = torch.empty((B, d), dtype=q.dtype, device=dev) if need_q else None
+        dp = torch.empty((C, d), dtype=p.dtype, device=dev) if need_p else None
+        dt = torch.empty(tshape, dtype=torch.float32, device=dev) if need_t else None
+        need = lib.abc_distill_bwd_workspace_bytes(dtype, B, C, M, d, k)
+        with _on(q):
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            rc = lib.abc_distill_bwd(dtype, q.data_ptr(), p.data_ptr(), None if M == 0 else memory.data_ptr(), t.data_ptr(), index.data_ptr(),
+                                     go.data_ptr(), B, C, M, d, k, None if dq is None else dq.data_ptr(),
+                                     None if dp is None else dp.data_ptr(), None if dt is None else dt.data_ptr(), ctx.ws.data_ptr(),
+                                     ctx.ws.numel(), ws.data_ptr(), need, _stream(q))
+        _lib.check(rc, "abc_distill_bwd")
+        if dt is not None and tdtype is not torch.float32:
+            dt = dt.to(tdtype)
+        return dq, dp, dt, None, None, None, None
+
+
+def compute_distillation_loss(q_embeds, p_embeds, temperature, teacher_index, teacher_scores, teacher_temperature=1.0, memory=None):
+    """Draw the softmax of each query over its candidates towards a teacher's top list: the mean over the queries of
+    KL(teacher's list || softmax(temperature(q @ candidates.T))).
+
+    The candidates are the rows of p_embeds [C, D] and after them the rows of `memory` [M, D], constants that receive no
+    gradient (read back from a search.EmbeddingStore, or the other ranks' rows c_global[n:] of gathered_candidates).
+    teacher_index [B, k] numbers them (0 .. C + M - 1), teacher_scores [B, k] are the teacher's scores of them, as topk returns them:
+    an index below 0 or a score of -inf is no entry, a column may come twice (its shares add up).  The teacher's shares are
+    softmax(teacher_scores / teacher_temperature) over a row's entries, which carry no gradient.  A row without an entry counts
+    nowhere and gets a gradient of zero; an index past the candidates makes the loss NaN.
+
+    q_embeds [B, D], p_embeds and memory all bf16 run on bf16 products with fp32 sums and return bf16 gradients; any other mix is
+    computed in fp32.  Returns (loss, agreement): agreement is the share of the rows with an entry whose best candidate is the
+    list's best entry.  Differentiable (once) w.r.t. q_embeds, p_embeds and temperature.temp.  Under graph capture take gradients
+    with torch.autograd.grad, as for every captured backward.  No counterpart in the reference."""
+    temp = _temp_param(temperature)
+    embeds = (q_embeds, p_embeds) if memory is None else (q_embeds, p_embeds, memory)
+    if not all(t.is_cuda for t in embeds + (teacher_index, teacher_scores)):
+        raise _lib.AbcError("the distillation kernels run on the GPU only (no CPU fallback)")
+    if any(t.device != q_embeds.device for t in embeds + (teacher_index, teacher_scores)):
+        raise _lib.AbcError("distillation: queries, candidates, memory and the teacher's list must be on one device")
+    if any(t.dim() != 2 or t.shape[1] != q_embeds.shape[1] for t in embeds):
+        raise _lib.AbcError(f"distillation: expected rows of one width, got {[tuple(t.shape) for t in embeds]}")
+    if not all(t.is_floating_point() for t in embeds + (teacher_scores,)):
+        raise _lib.AbcError("distillation: embeddings and teacher_scores must be floating point")
+    if teacher_index.dtype not in (torch.int64, torch.int32) or teacher_index.dim() != 2 or \
+            teacher_index.shape != teacher_scores.shape or teacher_index.shape[0] != q_embeds.shape[0]:
+        raise _lib.AbcError(f"distillation: expected teacher_index (int64 / int32) and teacher_scores [{q_embeds.shape[0]}, k], got "
+                            f"{teacher_index.dtype} {tuple(teacher_index.shape)} and {tuple(teacher_scores.shape)}")
+    if temp.numel() != 1:
+        raise _lib.AbcError("distillation: the temperature is one number")
+    if not float(teacher_temperature) > 0.0:
+        raise _lib.AbcError("distillation: teacher_temperature must be positive")
+    held = None
+    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
+        held = _captured_leaves((q_embeds, p_embeds, temp), refuse=True)
+    if temp.device != q_embeds.device:
+        temp = temp.to(q_embeds.device)
+    if not all(t.dtype is torch.bfloat16 for t in embeds):
+        q_embeds, p_embeds = q_embeds.float(), p_embeds.float()
+        memory = None if memory is None else memory.float()
+    extra = -q_embeds.shape[1] % 8
+    if extra:                                                               # zero columns change no product
+        q_embeds, p_embeds = (torch.nn.functional.pad(t, (0, extra)) for t in (q_embeds, p_embeds))
+        memory = None if memory is None else torch.nn.functional.pad(memory, (0, extra))
+    memory = None if memory is None or memory.shape[0] == 0 else _aligned(memory.detach())
+    out = _Distill.apply(_aligned(q_embeds), _aligned(p_embeds), temp, memory, teacher_index.to(torch.int64).contiguous(),
+                         _f32c(teacher_scores.detach()), float(teacher_temperature))
+    del held
+    return out
+
+
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """x contiguous, on a 16-byte boundary (a slice of a larger tensor may start anywhere)."""
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
 def _all_gather_rows(x: torch.Tensor) -> torch.Tensor:
