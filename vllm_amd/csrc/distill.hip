@@ -177,15 +177,16 @@ struct GemmArgs {
     unsigned* clear;                 // set to zero by the first workgroup (the arrival counter of the next launch), or null
 };
 
-// out[m][n] = sum_k A(m, k) B(n, k): tiles of TM x TN, four waves as 2 x 2, 32x32x16 bf16 MFMAs over every pair of planes whose
-// indices add up to less than KEEP.  One LDS stage; the next stage's values are on their way in registers while the current
-// one is multiplied, and two or more workgroups a CU fill each other's waits.
+// out[m][n] = sum_k A(m, k) B(n, k): tiles of TM x TN, four waves as 2 x 2, 16x16x32 bf16 MFMAs over every pair of planes whose
+// indices add up to less than KEEP.  An MFMA rounds its accumulator once (to nearest), so the products of the lower parts have an
+// accumulator of their own: the sum of the leading ones is rounded K / 32 times, not 6 K / 32.  One LDS stage; the next stage's values
+// are on their way in registers while the current one is multiplied, and two workgroups a CU fill each other's waits.
 template <class LA, class LB, int PA, int PB, int KEEP, int TM, int TN, int NKB, bool OUT_BF16>
 __global__ __launch_bounds__(256, 2) void distill_gemm_kernel(const GemmArgs g) {
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
     char* la = smem_raw;
     char* lb = smem_raw + PA * NKB * TM * 64;
-    constexpr int WM = TM / 64, WN = TN / 64;                   // 32 x 32 blocks a wave holds along m and n
+    constexpr int WM = TM / 32, WN = TN / 32, TWO = KEEP > 1;   // 16 x 16 blocks a wave holds along m and n
     if (g.clear && blockIdx.x == 0 && threadIdx.x == 0) *g.clear = 0u;
     // an XCD (every eighth id) takes a run of neighbouring tiles, those of one n tile and split next to each other, so that the larger
     // operand's values are fetched once into its L2
@@ -196,19 +197,20 @@ __global__ __launch_bounds__(256, 2) void distill_gemm_kernel(const GemmArgs g) 
     const int tm = inner % g.nm, sp = inner / g.nm;
     const int64_t k0 = sp * g.kstep, k1 = min(g.k, k0 + g.kstep);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int l31 = lane & 31, h = lane >> 5;
+    const int l15 = lane & 15, h = lane >> 4;
     const int wm = wave & 1, wn = wave >> 1;
     LA A;
     LB B;
     A.init(g.a, (int64_t)tm * TM, threadIdx.x);
     B.init(g.b, (int64_t)tn * TN, threadIdx.x);
-    v16f acc[WM][WN];
+    v4f acc[WM][WN], low[TWO ? WM : 1][TWO ? WN : 1];
 #pragma unroll
     for (int i = 0; i < WM; ++i)
 #pragma unroll
-        for (int j = 0; j < WN; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+        for (int j = 0; j < WN; ++j) {
+            acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+            if constexpr (TWO) low[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+        }
     A.load(g.a, k0, k1);
     B.load(g.b, k0, k1);
     for (int64_t k = k0; k < k1; k += NKB * 32) {
@@ -220,26 +222,28 @@ __global__ __launch_bounds__(256, 2) void distill_gemm_kernel(const GemmArgs g) 
             B.load(g.b, k + NKB * 32, k1);
         }
 #pragma unroll
-        for (int kk = 0; kk < NKB * 2; ++kk) {
-            v8bf fa[WM][PA], fb[WN][PB];
-#pragma unroll
-            for (int i = 0; i < WM; ++i)
-#pragma unroll
-                for (int p = 0; p < PA; ++p) fa[i][p] = *(const v8bf*)(la + lds_at<TM, NKB>(p, (wm * WM + i) * 32 + l31, kk * 2 + h));
+        for (int kb = 0; kb < NKB; ++kb) {
+            v8bf fb[WN][PB];
 #pragma unroll
             for (int j = 0; j < WN; ++j)
 #pragma unroll
-                for (int p = 0; p < PB; ++p) fb[j][p] = *(const v8bf*)(lb + lds_at<TN, NKB>(p, (wn * WN + j) * 32 + l31, kk * 2 + h));
+                for (int p = 0; p < PB; ++p) fb[j][p] = *(const v8bf*)(lb + lds_at<TN, NKB>(p, (wn * WN + j) * 16 + l15, kb * 4 + h));
 #pragma unroll
-            for (int pa = 0; pa < PA; ++pa)
+            for (int i = 0; i < WM; ++i) {
+                v8bf fa[PA];
 #pragma unroll
-                for (int pb = 0; pb < PB; ++pb)
-                    if (pa + pb < KEEP)
+                for (int p = 0; p < PA; ++p) fa[p] = *(const v8bf*)(la + lds_at<TM, NKB>(p, (wm * WM + i) * 16 + l15, kb * 4 + h));
 #pragma unroll
-                        for (int i = 0; i < WM; ++i)
+                for (int pa = 0; pa < PA; ++pa)
 #pragma unroll
-                            for (int j = 0; j < WN; ++j)
-                                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i][pa], fb[j][pb], acc[i][j], 0, 0, 0);
+                    for (int pb = 0; pb < PB; ++pb)
+                        if (pa + pb < KEEP)
+#pragma unroll
+                            for (int j = 0; j < WN; ++j) {
+                                v4f& c = pa + pb == 0 ? acc[i][j] : low[TWO ? i : 0][TWO ? j : 0];
+                                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[pa], fb[j][pb], c, 0, 0, 0);
+                            }
+            }
         }
         __syncthreads();
     }
@@ -247,10 +251,11 @@ __global__ __launch_bounds__(256, 2) void distill_gemm_kernel(const GemmArgs g) 
     for (int i = 0; i < WM; ++i)
 #pragma unroll
         for (int j = 0; j < WN; ++j) {
-            const int64_t n = (int64_t)tn * TN + (wn * WN + j) * 32 + l31;
+            const int64_t n = (int64_t)tn * TN + (wn * WN + j) * 16 + l15;
+            if constexpr (TWO) acc[i][j] += low[i][j];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t m = (int64_t)tm * TM + (wm * WM + i) * 32 + (r & 3) + 8 * (r >> 2) + 4 * h;
+            for (int r = 0; r < 4; ++r) {
+                const int64_t m = (int64_t)tm * TM + (wm * WM + i) * 16 + 4 * h + r;
                 if (m < g.a.rows && n < g.b.rows) {
                     if constexpr (OUT_BF16) ((uint16_t*)g.out)[m * g.ldo + n] = (uint16_t)f32_to_bf16_bits(acc[i][j][r]);
                     else ((float*)g.out)[sp * g.slab + m * g.ldo + n] = acc[i][j][r];
