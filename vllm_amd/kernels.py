@@ -225,25 +225,45 @@ def cast_bf16(x: torch.Tensor) -> torch.Tensor:
 
 
 # ---- rows held in 4 or 8 bits -------------------------------------------------------------------------------------------
-def _store_form(data: torch.Tensor, scale: torch.Tensor) -> Tuple[int, int]:
-    """(group, width) of a store's pair of tensors: int8 rows with one fp32 scale each (group 0), or packed 4-bit rows (uint8)
+# One row is a few microseconds of GPU work, so what the host does around a call counts: attributes are read once, the device is made
+# current only where it is not, and the stream is asked for by its raw handle (13 -> 7 us a call).
+def _launch(fn, what: str, device: torch.device, *args) -> None:
+    """fn(*args, current stream of `device`) with `device` current; raises the library's error."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, what)
+
+
+_ROW_DT = {torch.bfloat16: _lib.DT_BF16, torch.float32: _lib.DT_F32}
+
+
+def _store_form(data: torch.Tensor, scale: torch.Tensor) -> Tuple[int, int, int]:
+    """(group, width, rows) of a store's pair of tensors: int8 rows with one fp32 scale each (group 0), or packed 4-bit rows (uint8)
     with bf16 scales for groups of 32 / 64 / 128 values."""
-    _need_gpu(data, scale)
+    if not (data.is_cuda and scale.is_cuda):
+        _need_gpu(data, scale)
     if data.dim() != 2 or not data.is_contiguous() or not scale.is_contiguous() or data.device != scale.device:
         raise _lib.AbcError("store: data and scale must be contiguous matrices on one device")
-    if data.dtype == torch.int8:
-        if scale.dtype != torch.float32 or tuple(scale.shape) != (data.shape[0],) or data.shape[1] % 128 or data.shape[1] == 0:
+    rows, width = data.shape
+    if data.dtype is torch.int8:
+        if scale.dtype is not torch.float32 or tuple(scale.shape) != (rows,) or width % 128 or width == 0:
             raise _lib.AbcError(f"store: int8 rows {tuple(data.shape)} need a width of whole 128s and fp32 scales [rows], "
                                 f"got {scale.dtype} {tuple(scale.shape)}")
-        return 0, data.shape[1]
-    if data.dtype != torch.uint8 or scale.dtype != torch.bfloat16 or scale.dim() != 2 or scale.shape[0] != data.shape[0]:
+        return 0, width, rows
+    if data.dtype is not torch.uint8 or scale.dtype is not torch.bfloat16 or scale.dim() != 2 or scale.shape[0] != rows:
         raise _lib.AbcError(f"store: {data.dtype} rows with {scale.dtype} scales: int8 + fp32 or uint8 + bf16 [rows, groups]")
-    width = data.shape[1] * 2
-    group = width // scale.shape[1] if scale.shape[1] else 0
-    if width == 0 or width % 128 or group not in (32, 64, 128) or group * scale.shape[1] != width:
-        raise _lib.AbcError(f"store: 4-bit rows of {width} values with {scale.shape[1]} scales: groups of 32, 64 or 128 and a "
+    width *= 2
+    groups = scale.shape[1]
+    group = width // groups if groups else 0
+    if width == 0 or width % 128 or group not in (32, 64, 128) or group * groups != width:
+        raise _lib.AbcError(f"store: 4-bit rows of {width} values with {groups} scales: groups of 32, 64 or 128 and a "
                             "width of whole 128s")
-    return group, width
+    return group, width, rows
 
 
 def _store_dim(dim: int, width: int) -> int:
@@ -253,44 +273,54 @@ def _store_dim(dim: int, width: int) -> int:
 
 
 def _index64(index: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor:
-    if index.dtype not in (torch.int64, torch.int32):
-        raise _lib.AbcError(f"{what} must be int64 or int32, got {index.dtype}")
     if index.device != like.device:
+        _need_gpu(index)
         raise _lib.AbcError(f"{what} on {index.device}, the store on {like.device}")
-    return index.to(torch.int64).contiguous()
+    if index.dtype is torch.int64:
+        return index.contiguous()
+    if index.dtype is torch.int32:
+        return index.to(torch.int64).contiguous()
+    raise _lib.AbcError(f"{what} must be int64 or int32, got {index.dtype}")
 
 
-def _rows_of(x: torch.Tensor) -> torch.Tensor:
-    """x with unit stride along its rows (the kernels take any row stride from the width up)."""
-    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+def _store_rows(x: torch.Tensor, like: torch.Tensor, width: int, what: str) -> Tuple[torch.Tensor, int, int, int, int]:
+    """(x with unit stride along its rows, rows, values a row, row stride, dtype code) of rows [n, dim] for or against a store."""
+    dt = _ROW_DT.get(x.dtype)
+    if dt is None or x.dim() != 2 or x.device != like.device:
+        _need_gpu(x)
+        raise _lib.AbcError(f"{what}: expected f32 / bf16 rows [n, dim] on {like.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    n, dim = x.shape
+    _store_dim(dim, width)
+    ld = x.stride(0)
+    if x.stride(1) != 1 or ld < dim:
+        x = x.contiguous()
+        ld = dim
+    return x, n, dim, ld, dt
 
 
 def store_write(x: torch.Tensor, slots: Optional[torch.Tensor], data: torch.Tensor, scale: torch.Tensor, first: int = 0) -> None:
     """Quantise the rows of x [n, dim] (f32 / bf16) into the given slots of a store, in place; slots None: the n slots from
     `first` on, past the last one on from 0.  A slot outside the store drops its row (-1 = padding), and of rows that name the same slot
     the last one stays."""
-    group, width = _store_form(data, scale)
-    _need_gpu(x, slots)
-    if x.dim() != 2 or x.dtype not in (torch.float32, torch.bfloat16) or x.device != data.device:
-        raise _lib.AbcError(f"store_write: expected f32 / bf16 rows [n, dim] on {data.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    dim, n, capacity = _store_dim(x.shape[1], width), x.shape[0], data.shape[0]
+    group, width, capacity = _store_form(data, scale)
+    x, n, dim, ld, dt = _store_rows(x, data, width, "store_write")
+    lib = _lib.load()
+    at = ws = None
+    need = 0
     if slots is not None:
         slots = _index64(slots, data, "slots")
-        if slots.shape != (n,):
+        if slots.dim() != 1 or slots.shape[0] != n:
             raise _lib.AbcError(f"store_write: {n} rows but slots {tuple(slots.shape)}")
+        at = slots.data_ptr()
+        need = lib.abc_store_write_workspace_bytes(n, capacity)
+        if need:
+            # scratch of its own, not the per-stream cache: a captured graph keeps it for itself
+            ws = torch.empty(need, dtype=torch.uint8, device=data.device)
     elif n and (n > capacity or not 0 <= first < capacity):
         raise _lib.AbcError(f"store_write: {n} rows from slot {first} do not fit a store of {capacity}")
-    if n == 0:
-        return
-    x = _rows_of(x.detach())
-    lib = _lib.load()
-    need = lib.abc_store_write_workspace_bytes(n, capacity) if slots is not None else 0
-    with _on(data):
-        # scratch of its own, not the per-stream cache: a captured graph keeps it for itself
-        ws = torch.empty(need, dtype=torch.uint8, device=data.device) if need else None
-        rc = lib.abc_store_write(_DT[x.dtype], x.data_ptr(), x.stride(0) if n > 1 else dim, _ptr(slots), int(first), n, dim,
-                                 data.data_ptr(), scale.data_ptr(), capacity, group, _ptr(ws), need, _stream(data))
-    _lib.check(rc, "abc_store_write")
+    if n:
+        _launch(lib.abc_store_write, "abc_store_write", data.device, dt, x.data_ptr(), ld, at, int(first), n, dim, data.data_ptr(),
+                scale.data_ptr(), capacity, group, None if ws is None else ws.data_ptr(), need)
 
 
 def store_read(index: Optional[torch.Tensor], data: torch.Tensor, scale: torch.Tensor, dim: int, dtype: torch.dtype = torch.float32,
@@ -298,56 +328,57 @@ def store_read(index: Optional[torch.Tensor], data: torch.Tensor, scale: torch.T
     """The values that rows `index` (any shape; None: every row) of a store hold, f32 or bf16 [*index.shape, dim].  A negative
     index reads as a row of zeros (the -1 of a top-k list), an index past the store as a row of NaN.  `out`: a tensor of that shape to
     write into, its last dimension contiguous and its rows evenly spaced (a slice of a larger buffer)."""
-    group, width = _store_form(data, scale)
+    group, width, capacity = _store_form(data, scale)
     dim = _store_dim(dim, width)
-    if out is not None:
-        dtype = out.dtype
-    if dtype not in (torch.float32, torch.bfloat16):
-        raise _lib.AbcError(f"store_read: rows are read as f32 or bf16, not {dtype}")
-    shape = (data.shape[0],) if index is None else tuple(index.shape)
-    if index is not None:
-        _need_gpu(index)
-        index = _index64(index, data, "index").reshape(-1)
-    n = data.shape[0] if index is None else index.numel()
+    at = None
+    if index is None:
+        shape, n = (capacity, dim), capacity
+    else:
+        index = _index64(index, data, "index")
+        shape, n, at = (*index.shape, dim), index.numel(), index.data_ptr()
     if out is None:
-        out = torch.empty(shape + (dim,), dtype=dtype, device=data.device)
-    elif tuple(out.shape) != shape + (dim,) or out.device != data.device:
-        raise _lib.AbcError(f"store_read: out is {tuple(out.shape)} on {out.device}, expected {shape + (dim,)} on {data.device}")
-    elif out.requires_grad:
+        dt = _ROW_DT.get(dtype)
+        if dt is None:
+            raise _lib.AbcError(f"store_read: rows are read as f32 or bf16, not {dtype}")
+        out = torch.empty(shape, dtype=dtype, device=data.device)
+        to, ld = out.data_ptr(), dim
+    else:
+        to, ld, dt = _store_out(out, shape, n, data)
+    if n:
+        _launch(_lib.load().abc_store_read, "abc_store_read", data.device, at, 0, n, data.data_ptr(), scale.data_ptr(), capacity, dim, group,
+                dt, to, ld)
+    return out
+
+
+def _store_out(out: torch.Tensor, shape: tuple, n: int, data: torch.Tensor) -> Tuple[int, int, int]:
+    """(address, row stride, dtype code) of a caller's tensor that rows are read into."""
+    dt, dim = _ROW_DT.get(out.dtype), shape[-1]
+    if dt is None or tuple(out.shape) != shape or out.device != data.device:
+        raise _lib.AbcError(f"store_read: out is {out.dtype} {tuple(out.shape)} on {out.device}, expected f32 / bf16 {shape} on {data.device}")
+    if out.requires_grad:
         raise _lib.AbcError("store_read: out must not require a gradient (what is read back is constant)")
     if n == 0:
-        return out
+        return 0, dim, dt
     try:
         rows = out.view(-1, dim)
     except RuntimeError:
         raise _lib.AbcError("store_read: the rows of out are not evenly spaced") from None
-    if rows.stride(1) != 1 and dim > 1 or (n > 1 and rows.stride(0) < dim):
+    if (dim > 1 and rows.stride(1) != 1) or (n > 1 and rows.stride(0) < dim):
         raise _lib.AbcError("store_read: the last dimension of out must be contiguous and its rows must not overlap")
-    lib = _lib.load()
-    with _on(data):
-        rc = lib.abc_store_read(_ptr(index), 0, n, data.data_ptr(), scale.data_ptr(), data.shape[0], dim, group, _DT[dtype],
-                                rows.data_ptr(), rows.stride(0) if n > 1 else dim, _stream(data))
-    _lib.check(rc, "abc_store_read")
-    return out
+    return rows.data_ptr(), rows.stride(0) if n > 1 else dim, dt
 
 
 def store_scores(q: torch.Tensor, data: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     """f32 [nq, rows]: inner products of the queries q [nq, dim] (f32 / bf16) with every row of a 4-bit store.  For a few queries,
     where the stream over the store is the cost; a large set of them belongs in topk."""
-    group, width = _store_form(data, scale)
-    _need_gpu(q)
+    group, width, rows = _store_form(data, scale)
     if group == 0:
         raise _lib.AbcError("store_scores: the 4-bit form only (an int8 store is searched by topk)")
-    if q.dim() != 2 or q.dtype not in (torch.float32, torch.bfloat16) or q.device != data.device:
-        raise _lib.AbcError(f"store_scores: expected f32 / bf16 queries [nq, dim] on {data.device}, got {q.dtype} {tuple(q.shape)} on {q.device}")
-    dim, nq, rows = _store_dim(q.shape[1], width), q.shape[0], data.shape[0]
-    q = _rows_of(q.detach())
+    q, nq, dim, ld, dt = _store_rows(q, data, width, "store_scores")
     out = torch.empty((nq, rows), dtype=torch.float32, device=q.device)
-    lib = _lib.load()
-    with _on(q):
-        rc = lib.abc_store_scores(_DT[q.dtype], q.data_ptr(), q.stride(0) if nq > 1 else dim, nq, data.data_ptr(), scale.data_ptr(),
-                                  rows, dim, group, out.data_ptr(), rows, _stream(q))
-    _lib.check(rc, "abc_store_scores")
+    if nq and rows:
+        _launch(_lib.load().abc_store_scores, "abc_store_scores", data.device, dt, q.data_ptr(), ld, nq, data.data_ptr(), scale.data_ptr(),
+                rows, dim, group, out.data_ptr(), rows)
     return out
 
 

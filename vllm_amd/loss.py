@@ -16,7 +16,7 @@ import torch.distributed as dist
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kernels import _on, _stream
+from .kernels import _launch, _on, _stream
 
 
 class Temperature(torch.nn.Module):
@@ -191,51 +191,53 @@ class _Distill(torch.autograd.Function):
     def forward(ctx, q, p, temp, memory, index, score, teacher_temp: float):
         lib = _lib.load()
         B, d = q.shape
-        C, M, k = p.shape[0], 0 if memory is None else memory.shape[0], index.shape[1]
+        C, k = p.shape[0], index.shape[1]
+        M, mem = (0, None) if memory is None else (memory.shape[0], memory.data_ptr())
         dtype = _lib.DT_BF16 if q.dtype is torch.bfloat16 else _lib.DT_F32
         need = lib.abc_distill_workspace_bytes(dtype, B, C, M, d, k)
         if need == 0:
             _lib.check(-1, "abc_distill_workspace_bytes")
         dev = q.device
-        t = temp if (temp.dtype is torch.float32 and temp.device == dev) else temp.detach().to(device=dev, dtype=torch.float32)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        agree = torch.empty((), dtype=torch.float32, device=dev)
-        with _on(q):
-            # scratch of its own (the caching allocator's, in stream order): two losses alive, or two captured graphs, share nothing
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            rc = lib.abc_distill_fwd(dtype, q.data_ptr(), p.data_ptr(), None if M == 0 else memory.data_ptr(), t.data_ptr(),
-                                     index.data_ptr(), score.data_ptr(), teacher_temp, B, C, M, d, k, loss.data_ptr(), agree.data_ptr(),
-                                     ws.data_ptr(), need, _stream(q))
-        _lib.check(rc, "abc_distill_fwd")
-        ctx.save_for_backward(q, p, t, memory, index)
-        ctx.ws = ws
-        ctx.meta = (dtype, B, C, M, d, k, temp.dtype, tuple(temp.shape))
+        t = temp if temp.dtype is torch.float32 else temp.detach().to(torch.float32)
+        loss, agree = torch.empty((), dtype=torch.float32, device=dev), torch.empty((), dtype=torch.float32, device=dev)
+        # scratch of its own (the caching allocator's, in stream order): two losses alive, or two captured graphs, share nothing
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _launch(lib.abc_distill_fwd, "abc_distill_fwd", dev, dtype, q.data_ptr(), p.data_ptr(), mem, t.data_ptr(), index.data_ptr(),
+                score.data_ptr(), teacher_temp, B, C, M, d, k, loss.data_ptr(), agree.data_ptr(), ws.data_ptr(), need)
+        if any(ctx.needs_input_grad):
+            ctx.save_for_backward(q, p, t, memory, index)
+            ctx.ws = ws
+            ctx.meta = (dtype, B, C, M, d, k, need, temp.dtype, temp.shape)
         ctx.mark_non_differentiable(agree)
         return loss, agree
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_loss, _grad_agree):
-        q, p, t, memory, index = ctx.saved_tensors
-        dtype, B, C, M, d, k, tdtype, tshape = ctx.meta
-        lib = _lib.load()
-        need_q, need_p, need_t = ctx.needs_input_grad[:3]
-        go = _f32c(grad_loss)
-        dev = q.device
-        dq = torch.empty((B, d), dtype=q.dtype, device=dev) if need_q else None
-        dp = torch.empty((C, d), dtype=p.dtype, device=dev) if need_p else None
-        dt = torch.empty(tshape, dtype=torch.float32, device=dev) if need_t else None
-        need = lib.abc_distill_bwd_workspace_bytes(dtype, B, C, M, d, k)
-        with _on(q):
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            rc = lib.abc_distill_bwd(dtype, q.data_ptr(), p.data_ptr(), None if M == 0 else memory.data_ptr(), t.data_ptr(), index.data_ptr(),
-                                     go.data_ptr(), B, C, M, d, k, None if dq is None else dq.data_ptr(),
-                                     None if dp is None else dp.data_ptr(), None if dt is None else dt.data_ptr(), ctx.ws.data_ptr(),
-                                     ctx.ws.numel(), ws.data_ptr(), need, _stream(q))
-        _lib.check(rc, "abc_distill_bwd")
-        if dt is not None and tdtype is not torch.float32:
-            dt = dt.to(tdtype)
-        return dq, dp, dt, None, None, None, None
+        # once_differentiable costs some 10 us of bookkeeping; only a backward that is itself recorded needs it
+        return _distill_bwd_once(ctx, grad_loss, _grad_agree) if torch.is_grad_enabled() else _distill_bwd(ctx, grad_loss, _grad_agree)
+
+
+def _distill_bwd(ctx, grad_loss, _grad_agree):
+    q, p, t, memory, index = ctx.saved_tensors
+    dtype, B, C, M, d, k, fwd_need, tdtype, tshape = ctx.meta
+    lib = _lib.load()
+    need_q, need_p, need_t = ctx.needs_input_grad[:3]
+    go = _f32c(grad_loss)
+    dev = q.device
+    dq = torch.empty_like(q) if need_q else None
+    dp = torch.empty_like(p) if need_p else None
+    dt = torch.empty(tshape, dtype=torch.float32, device=dev) if need_t else None
+    need = lib.abc_distill_bwd_workspace_bytes(dtype, B, C, M, d, k)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _launch(lib.abc_distill_bwd, "abc_distill_bwd", dev, dtype, q.data_ptr(), p.data_ptr(), None if memory is None else memory.data_ptr(),
+            t.data_ptr(), index.data_ptr(), go.data_ptr(), B, C, M, d, k, None if dq is None else dq.data_ptr(),
+            None if dp is None else dp.data_ptr(), None if dt is None else dt.data_ptr(), ctx.ws.data_ptr(), fwd_need, ws.data_ptr(), need)
+    if dt is not None and tdtype is not torch.float32:
+        dt = dt.to(tdtype)
+    return dq, dp, dt, None, None, None, None
+
+
+_distill_bwd_once = once_differentiable(_distill_bwd)
 
 
 def compute_distillation_loss(q_embeds, p_embeds, temperature, teacher_index, teacher_scores, teacher_temperature=1.0, memory=None):
@@ -254,38 +256,43 @@ def compute_distillation_loss(q_embeds, p_embeds, temperature, teacher_index, te
     list's best entry.  Differentiable (once) w.r.t. q_embeds, p_embeds and temperature.temp.  Under graph capture take gradients
     with torch.autograd.grad, as for every captured backward.  No counterpart in the reference."""
     temp = _temp_param(temperature)
+    dev, width = q_embeds.device, q_embeds.shape[-1]
     embeds = (q_embeds, p_embeds) if memory is None else (q_embeds, p_embeds, memory)
-    if not all(t.is_cuda for t in embeds + (teacher_index, teacher_scores)):
-        raise _lib.AbcError("the distillation kernels run on the GPU only (no CPU fallback)")
-    if any(t.device != q_embeds.device for t in embeds + (teacher_index, teacher_scores)):
-        raise _lib.AbcError("distillation: queries, candidates, memory and the teacher's list must be on one device")
-    if any(t.dim() != 2 or t.shape[1] != q_embeds.shape[1] for t in embeds):
-        raise _lib.AbcError(f"distillation: expected rows of one width, got {[tuple(t.shape) for t in embeds]}")
-    if not all(t.is_floating_point() for t in embeds + (teacher_scores,)):
-        raise _lib.AbcError("distillation: embeddings and teacher_scores must be floating point")
-    if teacher_index.dtype not in (torch.int64, torch.int32) or teacher_index.dim() != 2 or \
-            teacher_index.shape != teacher_scores.shape or teacher_index.shape[0] != q_embeds.shape[0]:
-        raise _lib.AbcError(f"distillation: expected teacher_index (int64 / int32) and teacher_scores [{q_embeds.shape[0]}, k], got "
-                            f"{teacher_index.dtype} {tuple(teacher_index.shape)} and {tuple(teacher_scores.shape)}")
+    same = True                                                             # all bf16 or all fp32, as they come
+    for t in embeds:
+        if t.dim() != 2 or t.shape[1] != width or t.device != dev or not t.is_floating_point():
+            raise _lib.AbcError(f"distillation: expected floating-point rows of one width on one device, got "
+                                f"{[(t.dtype, tuple(t.shape), str(t.device)) for t in embeds]}")
+        same = same and t.dtype is q_embeds.dtype
+    if not (q_embeds.is_cuda and teacher_index.device == dev and teacher_scores.device == dev):
+        raise _lib.AbcError("distillation runs on the GPU only (no CPU fallback), with the teacher's list on the embeddings' device")
+    if teacher_index.dim() != 2 or teacher_index.shape != teacher_scores.shape or teacher_index.shape[0] != q_embeds.shape[0] or \
+            teacher_index.dtype not in (torch.int64, torch.int32) or not teacher_scores.is_floating_point():
+        raise _lib.AbcError(f"distillation: expected teacher_index (int64 / int32) and teacher_scores (floating point) "
+                            f"[{q_embeds.shape[0]}, k], got {teacher_index.dtype} {tuple(teacher_index.shape)} and "
+                            f"{teacher_scores.dtype} {tuple(teacher_scores.shape)}")
     if temp.numel() != 1:
         raise _lib.AbcError("distillation: the temperature is one number")
-    if not float(teacher_temperature) > 0.0:
+    teacher_temperature = float(teacher_temperature)
+    if not teacher_temperature > 0.0:
         raise _lib.AbcError("distillation: teacher_temperature must be positive")
     held = None
     if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
         held = _captured_leaves((q_embeds, p_embeds, temp), refuse=True)
-    if temp.device != q_embeds.device:
-        temp = temp.to(q_embeds.device)
-    if not all(t.dtype is torch.bfloat16 for t in embeds):
+    if temp.device != dev:
+        temp = temp.to(dev)
+    if not (same and (q_embeds.dtype is torch.bfloat16 or q_embeds.dtype is torch.float32)):
         q_embeds, p_embeds = q_embeds.float(), p_embeds.float()
         memory = None if memory is None else memory.float()
-    extra = -q_embeds.shape[1] % 8
-    if extra:                                                               # zero columns change no product
-        q_embeds, p_embeds = (torch.nn.functional.pad(t, (0, extra)) for t in (q_embeds, p_embeds))
-        memory = None if memory is None else torch.nn.functional.pad(memory, (0, extra))
-    memory = None if memory is None or memory.shape[0] == 0 else _aligned(memory.detach())
-    out = _Distill.apply(_aligned(q_embeds), _aligned(p_embeds), temp, memory, teacher_index.to(torch.int64).contiguous(),
-                         _f32c(teacher_scores.detach()), float(teacher_temperature))
+    if width % 8:                                                           # zero columns change no product
+        q_embeds, p_embeds = (torch.nn.functional.pad(t, (0, -width % 8)) for t in (q_embeds, p_embeds))
+        memory = None if memory is None else torch.nn.functional.pad(memory, (0, -width % 8))
+    if memory is not None:
+        memory = None if memory.shape[0] == 0 else _aligned(memory.detach())
+    if teacher_index.dtype is not torch.int64:
+        teacher_index = teacher_index.to(torch.int64)
+    out = _Distill.apply(_aligned(q_embeds), _aligned(p_embeds), temp, memory, teacher_index.contiguous(), _f32c(teacher_scores.detach()),
+                         teacher_temperature)
     del held
     return out
 
