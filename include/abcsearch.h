@@ -210,9 +210,9 @@ int abc_distill_fwd(int dtype, const void* q, const void* p, const void* memory,
                     const float* teacher_score, float teacher_temp, int64_t B, int64_t C, int64_t M, int d, int k, float* out_loss,
                     float* out_agree, void* workspace, size_t workspace_bytes, void* stream);
 size_t abc_distill_bwd_workspace_bytes(int dtype, int64_t B, int64_t C, int64_t M, int d, int k);
-int abc_distill_bwd(int dtype, const void* q, const void* p, const void* memory, const float* temp, const int64_t* teacher_idx,
-                    const float* grad_out, int64_t B, int64_t C, int64_t M, int d, int k, void* dq, void* dp, float* d_temp,
-                    const void* fwd_ws, size_t fwd_ws_bytes, void* workspace, size_t workspace_bytes, void* stream);
+int abc_distill_bwd(int dtype, const void* q, const void* p, const void* memory, const float* temp, const float* grad_out, int64_t B,
+                    int64_t C, int64_t M, int d, int k, void* dq, void* dp, float* d_temp, const void* fwd_ws, size_t fwd_ws_bytes,
+                    void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Embedding epilogue: the step that produces the vectors the search and the loss consume.

@@ -44,13 +44,18 @@ def distill_ref(q, cand, temp, index, score, teacher_temp, n_local, grad_out=1.0
 
 def distill_bounds(r, q, cand, temp, score, teacher_temp, n_local, k, bf16, grad_out=1.0):
     """How far fp32 arithmetic can be from `r`: u = 2^-24 is half a step of fp32; a sum of n terms in any order is off by at most n u times the
-    sum of the terms' magnitudes; what the three-part products leave out is below 2^-21 of a product (mid lo + lo mid + lo lo with
-    |mid| <= 2^-7, |lo| <= 2^-15 of the value); expf and logf are off by at most 4 steps (8 u)."""
+    sum of the terms' magnitudes; what the products of bf16 parts leave out is below 2^-21 of a product (mid lo + lo mid + lo lo with
+    |mid| <= 2^-7, |lo| <= 2^-15 of the value), what the products of fp16 parts leave out below 2^-22 (each value is off by 2^-24 of it and
+    by 2^-36, lo lo is 2^-22 of a product); exp and log are off by at most 4 steps (8 u).  `cand` rows of magnitude 2^-10 and more carry
+    the 2^-36 as 2^-26 of the row's largest value: `floor` below."""
     u, lost = 2.0 ** -24, 0.0 if bf16 else 2.0 ** -21
+    floor = 0.0 if bf16 else 2.0 ** -26
     q, c = q.double().abs(), cand.double().abs()
     B, D = q.shape
     T = c.shape[0]
-    dz = ((D + 16) * u + lost) * (q @ c.t()) / temp + 2 * u * r["z"].abs()
+    qm, cm = q.amax(1, keepdim=True), c.amax(1, keepdim=True)
+    dz = (((D + 16) * u + lost) * (q @ c.t()) + floor * (qm @ c.sum(1, keepdim=True).t() + q.sum(1, keepdim=True) @ cm.t())) / temp \
+        + 3 * u * r["z"].abs()
     worst = dz.max(1)[0]
     l_err = worst + (T + 20) * u + 8 * u * r["lse"].abs()
     live = torch.isfinite(score)
@@ -66,6 +71,11 @@ def distill_bounds(r, q, cand, temp, score, teacher_temp, n_local, k, bf16, grad
     cut = 2.0 ** -15 if bf16 else lost                            # g in two parts: hi 8 bits, mid 8 bits
     dq = (dg @ c + ((T + 16) * u + cut) * (ga @ c)) / temp
     dp = (dg.t() @ q + ((B + 16) * u + cut) * (ga.t() @ q))[:n_local] / temp
+    if not bf16:
+        # fp16 parts: a gradient of the logits is carried to 2^-50 of 1, a candidate or query to 2^-26 of its row's largest value
+        w = r["some"][:, None] * scale
+        dq = dq + ((2.0 ** -50) * w * c.sum(0, keepdim=True) + floor * (ga @ cm)) / temp
+        dp = dp + ((2.0 ** -50) * (w * q).sum(0, keepdim=True) + floor * (ga.t() @ qm)[:n_local]) / temp
     if bf16:
         dq, dp = dq * 1.01 + 2.0 ** -8 * r["dq"].abs(), dp * 1.01 + 2.0 ** -8 * r["dp"].abs()
     dt = ((dg * r["z"].abs() + ga * dz).sum() + (B * T + 16) * u * (ga * r["z"].abs()).sum()) / temp

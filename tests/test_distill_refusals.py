@@ -17,8 +17,8 @@ def fwd(dtype=F32, q=OK, p=OK, memory=None, temp=OK, idx=OK, score=OK, tt=1.0, B
     return lib().abc_distill_fwd(dtype, q, p, memory, temp, idx, score, tt, B, C, M, d, k, loss, agree, ws, ws_bytes, None)
 
 
-def bwd(dtype=F32, q=OK, p=OK, memory=None, temp=OK, idx=OK, go=OK, B=4, C=8, M=0, d=16, k=3, dq=OK, dp=OK, dt=OK, fws=OK, fws_bytes=0, ws=OK, ws_bytes=0):
-    return lib().abc_distill_bwd(dtype, q, p, memory, temp, idx, go, B, C, M, d, k, dq, dp, dt, fws, fws_bytes, ws, ws_bytes, None)
+def bwd(dtype=F32, q=OK, p=OK, memory=None, temp=OK, go=OK, B=4, C=8, M=0, d=16, k=3, dq=OK, dp=OK, dt=OK, fws=OK, fws_bytes=0, ws=OK, ws_bytes=0):
+    return lib().abc_distill_bwd(dtype, q, p, memory, temp, go, B, C, M, d, k, dq, dp, dt, fws, fws_bytes, ws, ws_bytes, None)
 
 
 SIZES = [dict(dtype=I8), dict(dtype=7), dict(B=0), dict(B=65536), dict(C=0), dict(M=-1), dict(M=1 << 31), dict(d=0), dict(d=12), dict(d=65544),

@@ -76,6 +76,52 @@ SHAPES = [(1, 1, 0, 8, 1), (1, 3, 0, 16, 2), (2, 5, 7, 24, 3), (33, 100, 0, 72, 
           (200, 300, 5000, 256, 1024), (257, 513, 100, 328, 17), (40, 2000, 30, 1024, 33), (6, 5, 0, 2056, 2)]
 
 
+# fp32 products of 8 GFLOP and more go by fp16 parts
+LARGE = [(256, 1000, 15_400, 1024, 40), (520, 2100, 0, 4096, 9)]
+
+
+@pytest.mark.parametrize("shape", LARGE)
+def test_large_fp32(shape):
+    check(*shape, seed=sum(shape))
+
+
+@pytest.mark.parametrize("what", ["large query", "tiny queries", "large candidate", "tiny memory row", "infinite candidate", "zero rows"])
+def test_large_fp32_where_fp16_parts_do_not_hold(what):
+    """The largest magnitude of a row outside [2^-10, 65000]: the six products take over, for all rows."""
+    B, C, M, D, k = 256, 1000, 15_400, 1024, 5
+    q, p, m, index, score = problem(B, C, M, D, k, 21)
+    temp = 0.07
+    if what == "large query":
+        q[7] *= 3e6
+        p, m, temp = p * 1e-3, m * 1e-3, 5.0
+    elif what == "tiny queries":
+        q *= 1e-4
+        temp = 1e-5
+    elif what == "large candidate":
+        p[999] *= 1e7
+        q *= 1e-2
+        temp = 1e3
+    elif what == "tiny memory row":
+        m[15_399] *= 1e-6
+    elif what == "infinite candidate":
+        p[3, 9] = INF
+    else:
+        q[9], p[17], m[0] = 0.0, 0.0, 0.0                           # held by the fp16 parts
+    leaves = [x.to(DEV).requires_grad_(True) for x in (q, p, torch.tensor(temp))]
+    loss, _ = call(leaves[0], leaves[1], m.to(DEV), leaves[2], index.to(DEV), score.to(DEV), 0.05)
+    dq, dp, dt = torch.autograd.grad(loss, leaves)
+    if what == "infinite candidate":
+        assert bool(torch.isnan(loss.detach())) and bool(torch.isnan(dq[0]).all())
+        return
+    cand = torch.cat((p, m))
+    t32 = float(torch.tensor(temp))
+    r = distill_ref(q, cand, t32, index, score, 0.05, C)
+    lim = distill_bounds(r, q, cand, t32, score, 0.05, C, k, False)
+    assert abs(float(loss.detach()) - float(r["loss"])) <= lim["loss"]
+    for got, name in ((dq, "dq"), (dp, "dp"), (dt, "dtemp")):
+        assert bool(((got.cpu().double() - r[name]).abs() <= lim[name]).all()), name
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("shape", SHAPES)
 def test_against_the_closed_form(shape, dtype):
@@ -223,10 +269,16 @@ def test_two_losses_alive_backward_twice_and_leaves_untouched():
     y, z = x.detach().clone().requires_grad_(True), x.detach().clone().requires_grad_(True)
     loss, _ = call(y, z, None, 0.07, index, score, 1.0)
     assert torch.equal(g, sum(torch.autograd.grad(loss, (y, z))))
-    with pytest.raises(RuntimeError):                               # the saved list was changed in place
-        idx = index.clone()
-        loss, _ = call(y, z, None, 0.07, idx, score, 1.0)
-        idx.zero_()
+    # the list is done with after the forward; the candidates are not, and autograd says so where they were changed
+    want = torch.autograd.grad(call(y, z, None, 0.07, index, score, 1.0)[0], (y, z))
+    idx = index.clone()
+    loss, _ = call(y, z, None, 0.07, idx, score, 1.0)
+    idx.zero_()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (y, z)), want))
+    loss, _ = call(y, z, None, 0.07, index, score, 1.0)
+    with torch.no_grad():
+        z.mul_(2)
+    with pytest.raises(RuntimeError, match="modified"):
         torch.autograd.grad(loss, (y, z))
 
 

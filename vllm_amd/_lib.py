@@ -54,7 +54,7 @@ SIGNATURES = {
     "abc_distill_workspace_bytes": (_sz, [_int, _i64, _i64, _i64, _int, _int]),
     "abc_distill_fwd": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _sz, _vp]),
     "abc_distill_bwd_workspace_bytes": (_sz, [_int, _i64, _i64, _i64, _int, _int]),
-    "abc_distill_bwd": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp]),
+    "abc_distill_bwd": (_int, [_int, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp]),
     "abc_infonce_bwd": (_int, [_vp, _vp, _vp, _vp, _f32, _vp, _int, _int, _int, _int, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 

@@ -6,11 +6,20 @@
 //   loss = mean of row_b over the rows that have an entry; a row without one counts nowhere and receives no gradient
 //   g_bj = (softmax(z)_bj - sum_{i: idx(b,i) = j} t_bi) grad_out / rows;  dq = g/temp c, dc = (g/temp)^T q, dtemp = -sum g z / temp
 //
-// Three products (s, dq, dc) over B x T x d are the work.  fp32 embeddings are multiplied at fp32 accuracy on the bf16 matrix cores:
-// x = hi + mid + lo, three bf16 values that carry 24 bits (hi cut, the rest rounded), and the six products of the parts down to
-// 2^-16 relative (hi hi, hi mid, mid hi, hi lo, lo hi, mid mid) in fp32 accumulators; what is left out is below 2^-22 of a
-// product, random in sign.  Six bf16 MFMAs cost 6/16 of the fp32 MFMA's time for the same product.  bf16 embeddings take
-// one product for s; their gradients take two (g in hi + mid, 2^-16 relative, below the 2^-9 of the result's own rounding).
+// Three products (s, dq, dc) over B x T x d are the work, on the 16-bit matrix cores (v_mfma_f32_16x16x32):
+//
+//   fp32, small   x = hi + mid + lo, three bf16 values that carry 24 bits (hi cut, the rest rounded), and the six products of the
+//                 parts down to 2^-16 relative (hi hi, hi mid, mid hi, hi lo, lo hi, mid mid): what is left out is below 2^-21 of a
+//                 product, random in sign.  Any fp32 value.
+//   fp32, large   x = hi + 2^-11 lo, two fp16 values of 11 bits each, and three products: half the matrix work for an error of
+//                 2^-23 of a product.  Holds for rows whose largest magnitude is in [2^-10, 65000] (a value is carried to 2^-36, 2^-26 of
+//                 that, at worst) or zero; unit rows are.  Whether all are is found out while they are read for s; where not, flag is set, and
+//                 the same launches once more, which return at once otherwise, take the six products.
+//   bf16          one product for s; the gradients take two (g in hi + mid, 2^-16 relative, below the 2^-8 of the result's own
+//                 rounding).
+//
+// An MFMA rounds its accumulator once (to nearest), so the products of the lower parts have an accumulator of their own: the sum of
+// the leading ones is rounded K / 32 times, not 6 K / 32.
 #include "common.h"
 #include <type_traits>
 #include "../../include/abcsearch.h"
@@ -21,11 +30,23 @@ int abc_fail_ws(size_t need, size_t have);
 
 typedef __attribute__((ext_vector_type(8))) __bf16 v8bf;
 typedef __attribute__((ext_vector_type(2))) __bf16 v2bf;
+typedef __attribute__((ext_vector_type(8))) _Float16 v8h;
+typedef __attribute__((ext_vector_type(2))) _Float16 v2h;
 typedef __attribute__((ext_vector_type(2))) float v2f;
 typedef __attribute__((ext_vector_type(4))) unsigned int v4u;
 
 #define DISTILL_MAX_K 1024
-#define DISTILL_SEG 4096            // columns of a row that one workgroup turns into gradients
+#define DISTILL_SEG 2048            // columns of a row that one workgroup of the row and gradient kernels takes
+#define G_SCALE 32768.0f            // fp16 gradients are held times 2^15 (softmax - target lies in [-1, 1])
+#define H_LOW 65000.0f
+#define H_MIN 0x1p-10f
+
+// exp(x) for x <= 0 (and whatever is not a number): 2^n 2^f with n = rint(x log2 e), f to 2^-25
+__device__ __forceinline__ float exp_neg(float x) {
+    const float n = rintf(x * 1.44269504f);
+    const float f = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269502f, -n));      // log2 e in two parts
+    return x < -150.f ? 0.f : ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
+}
 
 // ---- operands -----------------------------------------------------------------------------------------------------------
 // One side of a product: `rows` x K values.  K-contiguous (KC): value (r, k) at row r; K-strided (KS): at row k, column r.
@@ -36,134 +57,168 @@ struct Side {
     int64_t n0;                      // storage rows in p0
     int64_t ld;                      // elements between storage rows
     int64_t rows;                    // rows of the product on this side
+    int64_t plane;                   // bytes from one part of the values to the next, where they lie split
 };
 
-template <bool BF16>
+// how the values become the 16-bit parts that are multiplied
+enum { RAW, SPLIT_B3, SPLIT_H2 };    // as they lie; fp32 -> three bf16; fp32 -> two fp16
+constexpr int bytes_of(int num) { return num == RAW ? 2 : 4; }
+
+template <int ES>
 __device__ __forceinline__ const char* storage_row(const Side& s, int64_t i) {
     const char* base = i < s.n0 ? (const char*)s.p0 : (const char*)s.p1;
-    return base + (i < s.n0 ? i : i - s.n0) * s.ld * (BF16 ? 2 : 4);
+    return base + (i < s.n0 ? i : i - s.n0) * s.ld * ES;
 }
 
-// two fp32 values into their bf16 parts, packed (first value low)
-template <int PLANES>
-__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[PLANES]) {
+// two fp32 values into their parts, packed (first value low)
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[3]) {
     const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
     w[0] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
     float ra = a - __uint_as_float(ua & 0xFFFF0000u), rb = b - __uint_as_float(ub & 0xFFFF0000u);
-#pragma unroll
-    for (int p = 1; p < PLANES; ++p) {
-        const v2bf h = __builtin_convertvector(v2f{ra, rb}, v2bf);
-        w[p] = __builtin_bit_cast(uint32_t, h);
-        if (p + 1 < PLANES) {
-            ra -= __uint_as_float(w[p] << 16);
-            rb -= __uint_as_float(w[p] & 0xFFFF0000u);
-        }
-    }
+    w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{ra, rb}, v2bf));
+    ra -= __uint_as_float(w[1] << 16);
+    rb -= __uint_as_float(w[1] & 0xFFFF0000u);
+    w[2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{ra, rb}, v2bf));
+}
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[2]) {
+    const v2h h = __builtin_convertvector(v2f{a, b}, v2h);
+    w[0] = __builtin_bit_cast(uint32_t, h);
+    const float ra = fmaf((float)h[0], -2048.f, a * 2048.f), rb = fmaf((float)h[1], -2048.f, b * 2048.f);
+    w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{ra, rb}, v2h));
 }
 
-// A tile side in LDS: [plane][k block of 32][row][32 k] bf16, 64 bytes a row, its four 16-byte chunks permuted by (row / 2) % 4 so
-// that neither the fragments' reads (8 neighbouring rows, one chunk) nor the writes meet in a bank.
+// A tile side in LDS: [part][k block of 32][row][32 k], 64 bytes a row, its four 16-byte chunks permuted with the row so
+// that neither the fragments' reads (8 neighbouring rows, one chunk) nor the writes of turned columns (every second row) meet in a bank.
 template <int R, int NKB>
-__device__ __forceinline__ int lds_at(int plane, int row, int chunk) {
-    return (((plane * NKB + (chunk >> 2)) * R + row) << 6) + (((chunk & 3) ^ ((row >> 1) & 3)) << 4);
+__device__ __forceinline__ int lds_at(int part, int row, int chunk) {
+    return (((part * NKB + (chunk >> 2)) * R + row) << 6) + (((chunk & 3) ^ ((row >> 1) & 3) ^ ((row >> 3) & 3)) << 4);
 }
 
-// KC: a thread holds chunks of 8 values along k of one row.  K is a multiple of 8.
-template <bool BF16, int PLANES, int R, int NKB>
+// KC: a thread holds chunks of 8 values along k of one row, DEPTH stages of them.  Storage goes on to a multiple of 8 values with zeros.
+// RANGE: keeps the largest magnitude of what it reads.
+template <int NUM, int PARTS, int R, int NKB, int DEPTH, bool RANGE = false>
 struct LoadKC {
-    static constexpr int CH = NKB * 4, N = R * CH / 256;
+    static constexpr int ES = bytes_of(NUM), CH = NKB * 4, N = R * CH / 256, Q = NUM == RAW ? PARTS : 2;
     const char* at[N];
-    v4u w[N][BF16 ? 1 : 2];
+    v4u w[DEPTH][N][Q];
+    float top[RANGE ? N : 1];
     int row0, chunk;
     __device__ __forceinline__ void init(const Side& s, int64_t r0, int tid) {
         chunk = tid % CH;
         row0 = tid / CH;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            int64_t r = r0 + row0 + i * (256 / CH);
-            at[i] = r < s.rows ? storage_row<BF16>(s, r) : nullptr;
+            const int64_t r = r0 + row0 + i * (256 / CH);
+            at[i] = r < s.rows ? storage_row<ES>(s, r) : nullptr;
+            if constexpr (RANGE) top[i] = 0.f;
         }
     }
-    __device__ __forceinline__ void load(const Side&, int64_t k0, int64_t k1) {
+    __device__ __forceinline__ void load(int d, const Side& s, int64_t k0, int64_t k1) {
         const int64_t k = k0 + chunk * 8;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (at[i] && k < k1) {
-                const v4u* src = (const v4u*)(at[i] + k * (BF16 ? 2 : 4));
-                w[i][0] = src[0];
-                if constexpr (!BF16) w[i][1] = src[1];
-            } else {
-                w[i][0] = v4u{0, 0, 0, 0};
-                if constexpr (!BF16) w[i][1] = v4u{0, 0, 0, 0};
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int p = 0; p < Q; ++p) {
+                if (at[i] && k < k1) w[d][i][p] = *(const v4u*)(at[i] + (NUM == RAW ? p * s.plane : p * 16) + k * ES);
+                else w[d][i][p] = v4u{0, 0, 0, 0};
             }
-        }
     }
-    __device__ __forceinline__ void store(char* lds) {
+    __device__ __forceinline__ void store(int d, char* lds) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int row = row0 + i * (256 / CH);
-            if constexpr (BF16) {
-                *(v4u*)(lds + lds_at<R, NKB>(0, row, chunk)) = w[i][0];
+            if constexpr (NUM == RAW) {
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) *(v4u*)(lds + lds_at<R, NKB>(p, row, chunk)) = w[d][i][p];
             } else {
-                uint32_t o[4][PLANES];
+                uint32_t o[4][PARTS];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    split_pair<PLANES>(__uint_as_float(w[i][j >> 1][(2 * j) & 3]), __uint_as_float(w[i][j >> 1][(2 * j + 1) & 3]), o[j]);
+                for (int j = 0; j < 4; ++j) {
+                    const float a = __uint_as_float(w[d][i][j >> 1][(2 * j) & 3]), b = __uint_as_float(w[d][i][j >> 1][(2 * j + 1) & 3]);
+                    split_pair(a, b, o[j]);
+                    if constexpr (RANGE) top[i] = fmaxf(fmaxf(fabsf(a), fabsf(b)), top[i]);
+                }
 #pragma unroll
-                for (int p = 0; p < PLANES; ++p)
+                for (int p = 0; p < PARTS; ++p)
                     *(v4u*)(lds + lds_at<R, NKB>(p, row, chunk)) = v4u{o[0][p], o[1][p], o[2][p], o[3][p]};
             }
         }
     }
+    // whether a row that this thread has a part in does not fit the fp16 parts
+    __device__ __forceinline__ bool outside() {
+        bool bad = false;
+        if constexpr (RANGE)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                float v = top[i];
+#pragma unroll
+                for (int m = 1; m < CH; m <<= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
+                bad |= v > 0.f && !(v >= H_MIN && v <= H_LOW);
+            }
+        return bad;
+    }
 };
 
-// KS: a thread holds 8 storage rows (k) of two neighbouring columns and turns them round in its registers.  `rows` is a multiple of
-// 2 or storage goes on past it.
-template <bool BF16, int PLANES, int R, int NKB>
+// KS: a thread holds 8 storage rows (k) of two neighbouring columns (one, where a narrow fp32 tile has too few) and turns them round
+// in its registers.  `rows` is even or storage goes on past it.
+template <int NUM, int PARTS, int R, int NKB, int DEPTH>
 struct LoadKS {
-    static constexpr int CG = R / 2, TASKS = CG * NKB * 4, N = TASKS < 256 ? 1 : TASKS / 256;
-    typedef typename std::conditional<BF16, uint32_t, v2f>::type pair_t;
-    pair_t w[N][8];
+    static constexpr int ES = bytes_of(NUM), COLS = NUM != RAW && R * NKB * 2 < 256 ? 1 : 2, CG = R / COLS, N = CG * NKB * 4 / 256;
+    static constexpr int Q = NUM == RAW ? PARTS : 1;
+    static_assert(N >= 1, "a tile too narrow for 256 threads");
+    typedef typename std::conditional<NUM == RAW, uint32_t, typename std::conditional<COLS == 2, v2f, float>::type>::type piece_t;
+    piece_t w[DEPTH][N][Q][8];
     int64_t col;
     int cg, chunk0;
     bool ok;
     __device__ __forceinline__ void init(const Side& s, int64_t r0, int tid) {
         cg = tid % CG;
-        chunk0 = tid / CG;
-        col = r0 + cg * 2;
-        ok = col < s.rows && (TASKS >= 256 || chunk0 < NKB * 4);
+        chunk0 = CG >= 64 ? __builtin_amdgcn_readfirstlane(tid / CG) : tid / CG;   // a wave's storage rows are scalar then
+        col = r0 + cg * COLS;
+        ok = col < s.rows;
     }
-    __device__ __forceinline__ void load(const Side& s, int64_t k0, int64_t k1) {
+    __device__ __forceinline__ void load(int d, const Side& s, int64_t k0, int64_t k1) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int64_t k = k0 + (chunk0 + i * (256 / CG)) * 8;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if (ok && k + j < k1) w[i][j] = *(const pair_t*)(storage_row<BF16>(s, k + j) + col * (BF16 ? 2 : 4));
-                else if constexpr (BF16) w[i][j] = 0;
-                else w[i][j] = v2f{0.f, 0.f};
+                const bool in = ok && k + j < k1;
+                const char* src = in ? storage_row<ES>(s, k + j) + col * ES : nullptr;
+#pragma unroll
+                for (int p = 0; p < Q; ++p) {
+                    if (in) w[d][i][p][j] = *(const piece_t*)(src + p * s.plane);
+                    else w[d][i][p][j] = piece_t{};
+                }
             }
         }
     }
-    __device__ __forceinline__ void store(char* lds) {
-        if (TASKS < 256 && chunk0 >= NKB * 4) return;            // a narrow tile leaves some threads without a task
+    __device__ __forceinline__ float value(const piece_t& x, int c) const {
+        if constexpr (COLS == 2 && NUM != RAW) return x[c];
+        else return (float)x;
+    }
+    __device__ __forceinline__ void store(int d, char* lds) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int chunk = chunk0 + i * (256 / CG);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t o[4][PLANES];
+            for (int c = 0; c < COLS; ++c) {
+                uint32_t o[4][PARTS];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if constexpr (BF16) o[j][0] = __builtin_amdgcn_perm(w[i][2 * j + 1], w[i][2 * j], c ? 0x07060302u : 0x05040100u);
-                    else split_pair<PLANES>(w[i][2 * j][c], w[i][2 * j + 1][c], o[j]);
+                    if constexpr (NUM == RAW) {
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p)
+                            o[j][p] = __builtin_amdgcn_perm(w[d][i][p][2 * j + 1], w[d][i][p][2 * j], c ? 0x07060302u : 0x05040100u);
+                    } else split_pair(value(w[d][i][0][2 * j], c), value(w[d][i][0][2 * j + 1], c), o[j]);
                 }
 #pragma unroll
-                for (int p = 0; p < PLANES; ++p)
-                    *(v4u*)(lds + lds_at<R, NKB>(p, cg * 2 + c, chunk)) = v4u{o[0][p], o[1][p], o[2][p], o[3][p]};
+                for (int p = 0; p < PARTS; ++p)
+                    *(v4u*)(lds + lds_at<R, NKB>(p, cg * COLS + c, chunk)) = v4u{o[0][p], o[1][p], o[2][p], o[3][p]};
             }
         }
     }
+    __device__ __forceinline__ bool outside() { return false; }
 };
 
 struct GemmArgs {
@@ -172,37 +227,42 @@ struct GemmArgs {
     int splits;
     int64_t kstep;                   // values of k a split takes (a multiple of the stage)
     int nm, nn;                      // tiles
-    void* out;                       // splits == 1: out[m * ldo + n]; otherwise fp32 slabs of `slab` values
+    void* out;                       // out[m * ldo + n]; splits > 1: fp32 slabs of `slab` values
     int64_t ldo, slab;
-    unsigned* clear;                 // set to zero by the first workgroup (the arrival counter of the next launch), or null
+    float scale;                     // of every sum
+    const float *f0, *f1, *f2;       // splits == 1, f0 given: times f0[0] f1[0] / f2[0]
 };
 
-// out[m][n] = sum_k A(m, k) B(n, k): tiles of TM x TN, four waves as 2 x 2, 16x16x32 bf16 MFMAs over every pair of planes whose
-// indices add up to less than KEEP.  An MFMA rounds its accumulator once (to nearest), so the products of the lower parts have an
-// accumulator of their own: the sum of the leading ones is rounded K / 32 times, not 6 K / 32.  One LDS stage; the next stage's values
-// are on their way in registers while the current one is multiplied, and two workgroups a CU fill each other's waits.
-template <class LA, class LB, int PA, int PB, int KEEP, int TM, int TN, int NKB, bool OUT_BF16>
-__global__ __launch_bounds__(256, 2) void distill_gemm_kernel(const GemmArgs g) {
-    extern __shared__ __attribute__((aligned(16))) char smem_raw[];
-    char* la = smem_raw;
-    char* lb = smem_raw + PA * NKB * TM * 64;
-    constexpr int WM = TM / 32, WN = TN / 32, TWO = KEEP > 1;   // 16 x 16 blocks a wave holds along m and n
-    if (g.clear && blockIdx.x == 0 && threadIdx.x == 0) *g.clear = 0u;
-    // an XCD (every eighth id) takes a run of neighbouring tiles, those of one n tile and split next to each other, so that the larger
-    // operand's values are fetched once into its L2
-    const int per = g.nm * g.splits, chunk = gridDim.x >> 3;
-    const int item = (blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
-    if (item >= g.nn * per) return;
-    const int tn = item / per, inner = item % per;
+__device__ __forceinline__ float factor_of(const float* f0, const float* f1, const float* f2) { return __fdiv_rn(f0[0] * f1[0], f2[0]); }
+
+// out[m][n] = sum_k A(m, k) B(n, k): tiles of TM x TN, four waves as 2 x 2, 16x16x32 MFMAs over every pair of parts whose indices add up
+// to less than KEEP.  The next DEPTH stages' values are on their way in registers while one is multiplied out of LDS (LBUF buffers of
+// it: two need one barrier a stage), and two or more workgroups a CU fill each other's waits.
+template <class LA_, class LB_, int PA_, int PB_, int KEEP_, int TM_, int TN_, int NKB_, int DEPTH_, int LBUF_, bool F16_, bool OUT_BF16_>
+struct Cfg {
+    typedef LA_ LA;
+    typedef LB_ LB;
+    static constexpr int PA = PA_, PB = PB_, KEEP = KEEP_, TM = TM_, TN = TN_, NKB = NKB_, DEPTH = DEPTH_, LBUF = LBUF_;
+    static constexpr bool F16 = F16_, OUT_BF16 = OUT_BF16_;
+    static constexpr int LDS = LBUF * (PA * TM + PB * TN) * NKB * 64;
+};
+
+template <class C>
+__device__ __forceinline__ bool gemm_tile(const GemmArgs& g, int item, char* smem) {
+    constexpr int WM = C::TM / 32, WN = C::TN / 32, STAGE = C::NKB * 32;    // 16 x 16 blocks a wave holds along m and n
+    constexpr bool TWO = C::KEEP > 1;
+    constexpr int BUF = C::LDS / C::LBUF, LB0 = C::PA * C::NKB * C::TM * 64;
+    typedef typename std::conditional<C::F16, v8h, v8bf>::type frag_t;
+    const int per = g.nm * g.splits, tn = item / per, inner = item % per;
     const int tm = inner % g.nm, sp = inner / g.nm;
     const int64_t k0 = sp * g.kstep, k1 = min(g.k, k0 + g.kstep);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int l15 = lane & 15, h = lane >> 4;
     const int wm = wave & 1, wn = wave >> 1;
-    LA A;
-    LB B;
-    A.init(g.a, (int64_t)tm * TM, threadIdx.x);
-    B.init(g.b, (int64_t)tn * TN, threadIdx.x);
+    typename C::LA A;
+    typename C::LB B;
+    A.init(g.a, (int64_t)tm * C::TM, threadIdx.x);
+    B.init(g.b, (int64_t)tn * C::TN, threadIdx.x);
     v4f acc[WM][WN], low[TWO ? WM : 1][TWO ? WN : 1];
 #pragma unroll
     for (int i = 0; i < WM; ++i)
@@ -211,63 +271,144 @@ __global__ __launch_bounds__(256, 2) void distill_gemm_kernel(const GemmArgs g) 
             acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
             if constexpr (TWO) low[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
         }
-    A.load(g.a, k0, k1);
-    B.load(g.b, k0, k1);
-    for (int64_t k = k0; k < k1; k += NKB * 32) {
-        A.store(la);
-        B.store(lb);
-        __syncthreads();
-        if (k + NKB * 32 < k1) {
-            A.load(g.a, k + NKB * 32, k1);
-            B.load(g.b, k + NKB * 32, k1);
-        }
 #pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) {
-            v8bf fb[WN][PB];
-#pragma unroll
-            for (int j = 0; j < WN; ++j)
-#pragma unroll
-                for (int p = 0; p < PB; ++p) fb[j][p] = *(const v8bf*)(lb + lds_at<TN, NKB>(p, (wn * WN + j) * 16 + l15, kb * 4 + h));
-#pragma unroll
-            for (int i = 0; i < WM; ++i) {
-                v8bf fa[PA];
-#pragma unroll
-                for (int p = 0; p < PA; ++p) fa[p] = *(const v8bf*)(la + lds_at<TM, NKB>(p, (wm * WM + i) * 16 + l15, kb * 4 + h));
-#pragma unroll
-                for (int pa = 0; pa < PA; ++pa)
-#pragma unroll
-                    for (int pb = 0; pb < PB; ++pb)
-                        if (pa + pb < KEEP)
-#pragma unroll
-                            for (int j = 0; j < WN; ++j) {
-                                v4f& c = pa + pb == 0 ? acc[i][j] : low[TWO ? i : 0][TWO ? j : 0];
-                                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[pa], fb[j][pb], c, 0, 0, 0);
-                            }
-            }
-        }
-        __syncthreads();
+    for (int d = 0; d < C::DEPTH; ++d) {
+        A.load(d, g.a, k0 + d * STAGE, k1);
+        B.load(d, g.b, k0 + d * STAGE, k1);
     }
+    int buf = 0;
+    for (int64_t kb0 = k0; kb0 < k1; kb0 += STAGE * C::DEPTH) {
+#pragma unroll
+        for (int d = 0; d < C::DEPTH; ++d) {
+            const int64_t k = kb0 + d * STAGE;
+            if (k >= k1) break;
+            char* la = smem + buf * BUF;
+            char* lb = la + LB0;
+            A.store(d, la);
+            B.store(d, lb);
+            __syncthreads();
+            if (k + C::DEPTH * STAGE < k1) {
+                A.load(d, g.a, k + C::DEPTH * STAGE, k1);
+                B.load(d, g.b, k + C::DEPTH * STAGE, k1);
+            }
+#pragma unroll
+            for (int kb = 0; kb < C::NKB; ++kb) {
+                frag_t fb[WN][C::PB];
+#pragma unroll
+                for (int j = 0; j < WN; ++j)
+#pragma unroll
+                    for (int p = 0; p < C::PB; ++p)
+                        fb[j][p] = *(const frag_t*)(lb + lds_at<C::TN, C::NKB>(p, (wn * WN + j) * 16 + l15, kb * 4 + h));
+#pragma unroll
+                for (int i = 0; i < WM; ++i) {
+                    frag_t fa[C::PA];
+#pragma unroll
+                    for (int p = 0; p < C::PA; ++p)
+                        fa[p] = *(const frag_t*)(la + lds_at<C::TM, C::NKB>(p, (wm * WM + i) * 16 + l15, kb * 4 + h));
+#pragma unroll
+                    for (int pa = 0; pa < C::PA; ++pa)
+#pragma unroll
+                        for (int pb = 0; pb < C::PB; ++pb)
+                            if (pa + pb < C::KEEP)
+#pragma unroll
+                                for (int j = 0; j < WN; ++j) {
+                                    v4f& c = pa + pb == 0 ? acc[i][j] : low[TWO ? i : 0][TWO ? j : 0];
+                                    if constexpr (C::F16) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[pa], fb[j][pb], c, 0, 0, 0);
+                                    else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[pa], fb[j][pb], c, 0, 0, 0);
+                                }
+                }
+            }
+            if constexpr (C::LBUF == 1) __syncthreads();
+            else buf ^= 1;
+        }
+    }
+    const float f = g.scale * (g.splits == 1 && g.f0 ? factor_of(g.f0, g.f1, g.f2) : 1.f);
 #pragma unroll
     for (int i = 0; i < WM; ++i)
 #pragma unroll
         for (int j = 0; j < WN; ++j) {
-            const int64_t n = (int64_t)tn * TN + (wn * WN + j) * 16 + l15;
-            if constexpr (TWO) acc[i][j] += low[i][j];
+            const int64_t n = (int64_t)tn * C::TN + (wn * WN + j) * 16 + l15;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int64_t m = (int64_t)tm * TM + (wm * WM + i) * 16 + 4 * h + r;
+                const int64_t m = (int64_t)tm * C::TM + (wm * WM + i) * 16 + 4 * h + r;
+                float v = acc[i][j][r];
+                if constexpr (TWO) v = C::F16 ? fmaf(low[i][j][r], 0x1p-11f, v) : v + low[i][j][r];
+                v *= f;
                 if (m < g.a.rows && n < g.b.rows) {
-                    if constexpr (OUT_BF16) ((uint16_t*)g.out)[m * g.ldo + n] = (uint16_t)f32_to_bf16_bits(acc[i][j][r]);
-                    else ((float*)g.out)[sp * g.slab + m * g.ldo + n] = acc[i][j][r];
+                    if (C::OUT_BF16 && g.splits == 1) ((uint16_t*)g.out)[m * g.ldo + n] = (uint16_t)f32_to_bf16_bits(v);
+                    else ((float*)g.out)[sp * g.slab + m * g.ldo + n] = v;
                 }
             }
         }
+    const bool out_a = A.outside(), out_b = B.outside();
+    return out_a || out_b;
+}
+
+// an XCD (every eighth id) takes a run of neighbouring tiles, those of one n tile and split next to each other, so that the larger
+// operand's values are fetched once into its L2
+__device__ __forceinline__ int item_of(int id, int n) { return (id & 7) * ((n + 7) >> 3) + (id >> 3); }
+
+// flag: null, or the word that says whether the fp16 parts hold the values; the launch runs where it equals run_if
+template <class C>
+__global__ __launch_bounds__(256, 2) void distill_scores_kernel(const GemmArgs g, const unsigned* flag, unsigned run_if, unsigned* raise,
+                                                                const unsigned* rows_out, int64_t nrows_out, unsigned* clear, int nclear) {
+    extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+    if (flag && *flag != run_if) return;
+    if (clear && blockIdx.x == 0)                                 // the arrival counters of the next launch
+        for (int i = threadIdx.x; i < nclear; i += 256) clear[i] = 0u;
+    const int n = g.nn * g.nm * g.splits, item = item_of(blockIdx.x, n);
+    bool bad = false;
+    if (raise && blockIdx.x == 0)
+        for (int64_t i = threadIdx.x; i < nrows_out; i += 256) bad |= rows_out[i] != 0u;
+    if (item < n) bad |= gemm_tile<C>(g, item, smem_raw);
+    if (raise && bad) __hip_atomic_store(raise, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// both gradients' products in one launch: the first n0 workgroups (a multiple of 8) take dq
+template <class CQ, class CP>
+__global__ __launch_bounds__(256, 2) void distill_grads_kernel(const GemmArgs gq, const GemmArgs gp, int n0, const unsigned* flag, unsigned run_if) {
+    extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+    if (flag && *flag != run_if) return;
+    if ((int)blockIdx.x < n0) {
+        const int n = gq.nn * gq.nm * gq.splits, item = item_of(blockIdx.x, n);
+        if (item < n) gemm_tile<CQ>(gq, item, smem_raw);
+    } else {
+        const int n = gp.nn * gp.nm * gp.splits, item = item_of(blockIdx.x - n0, n);
+        if (item < n) gemm_tile<CP>(gp, item, smem_raw);
+    }
+}
+
+// the queries' fp16 parts, once for all tiles of the two products that read them; rows_out[b]: row b does not fit them
+__global__ __launch_bounds__(256) void distill_split_kernel(const float* __restrict__ q, int d, int64_t n, uint16_t* __restrict__ out,
+                                                            unsigned* __restrict__ rows_out, unsigned* __restrict__ flag) {
+    __shared__ float red[4];
+    const int64_t b = blockIdx.x;
+    if (b == 0 && threadIdx.x == 0) *flag = 0u;
+    float top = 0.f;
+    for (int k = threadIdx.x * 4; k < d; k += 1024) {
+        const v4f x = *(const v4f*)(q + b * d + k);
+        uint32_t lo[2], hi[2];
+        split_pair(x[0], x[1], lo);
+        split_pair(x[2], x[3], hi);
+        *(uint2*)(out + b * d + k) = uint2{lo[0], hi[0]};
+        *(uint2*)(out + n + b * d + k) = uint2{lo[1], hi[1]};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) top = fmaxf(top, fabsf(x[c]));
+    }
+    for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        rows_out[b] = top > 0.f && !(top >= H_MIN && top <= H_LOW) ? 1u : 0u;
+    }
 }
 
 // ---- the rows: logsumexp, the teacher's list, the loss -------------------------------------------------------------------
 struct RowArgs {
-    float* s;                        // slabs [splits][B][lds]; slab 0 holds the sum afterwards
-    int splits;
+    const float* part;               // slabs [splits][B][lds] of s
+    float* s;                        // their sum (part itself where there is one)
+    int splits, segs;
     int64_t slab, lds;
     const float* temp;
     const int64_t* idx;
@@ -275,219 +416,307 @@ struct RowArgs {
     float teacher_temp;
     int64_t B, T;
     int k;
+    float* seg;                      // [B][segs][4]: maximum, sum of exp(z - maximum), its first column, 1 where a z is NaN
     float* lse;                      // [B]
-    float* t;                        // [B][k]; 0 = no entry
+    float* t;                        // [B][k]: the teacher's share of column li (all of a column's entries at the first of them), or 0
+    int* li;                         // [B][k]: the column, -1 = nothing
     float* row;                      // [B] row losses, then [B] agreement, then [B] 1 where the row has an entry
     float* stat;                     // [0]: 1 / rows that have an entry
-    unsigned* cnt;
+    unsigned* cnt;                   // [B] segments that have arrived, [1] rows
     float* out_loss;
     float* out_agree;
 };
 
-__device__ __forceinline__ float block_max(float v, float* red) {
-    for (int m = 32; m > 0; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+// Values handed to another workgroup of the same launch: stored and loaded past the caches that are not common to the chip.
+__device__ __forceinline__ void put(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float get(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// Whether this workgroup is the last of n to arrive; its thread 0 made the put()s that the last one get()s.
+__device__ __forceinline__ bool arrive_last(unsigned* cnt, unsigned n, unsigned* flag) {
+    if (threadIdx.x == 0) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // the puts have reached the chip's common memory before the arrival counts
+        *flag = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1 ? 1u : 0u;
+    }
     __syncthreads();
-    v = red[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v = fmaxf(v, red[w]);
-    __syncthreads();
-    return v;
-}
-__device__ __forceinline__ float block_sum(float v, float* red) {     // fixed order
-    for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m, 64);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.f;
-    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) v += red[w];
-    __syncthreads();
-    return v;
+    return *flag != 0u;
 }
 
-__global__ __launch_bounds__(512) void distill_row_kernel(const RowArgs a) {
-    __shared__ float red[8];
-    __shared__ int64_t redi[8];
-    __shared__ float ts[DISTILL_MAX_K];
-    __shared__ unsigned last;
-    const int64_t b = blockIdx.x;
-    float* s = a.s + b * a.lds;
-    const float t = a.temp[0];
-    // one pass: running maximum, its first column, and the sum of exp(z - maximum)
-    float mx = -INFINITY, se = 0.f;
-    int64_t am = 0;
-    bool nan = false;
-    for (int64_t j = threadIdx.x * 4; j < a.T; j += 2048) {
-        v4f x = *(const v4f*)(s + j);
-        for (int p = 1; p < a.splits; ++p) x += *(const v4f*)(s + p * a.slab + j);
-        if (a.splits > 1) *(v4f*)(s + j) = x;
+struct Red { float a, b; int c; };
+// maximum, sum and minimum over the workgroup of 256 threads, in one round; fixed order
+__device__ __forceinline__ Red block_red(float mx, float sum, int mn, Red* red) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (j + i >= a.T) break;
-            const float z = __fdiv_rn(x[i], t);
-            if (z > mx) { se *= expf(mx - z); mx = z; am = j + i; }
-            if (z > -INFINITY) se += expf(z - mx);
-            nan |= z != z;
-        }
-    }
-    const float top = block_max(mx, red);
-    int64_t cand = mx == top && top > -INFINITY ? am : INT64_MAX;
     for (int m = 32; m > 0; m >>= 1) {
-        const int lo = __shfl_xor((int)(uint32_t)cand, m, 64), hi = __shfl_xor((int)(cand >> 32), m, 64);
-        const int64_t o = ((int64_t)hi << 32) | (uint32_t)lo;
-        cand = o < cand ? o : cand;
+        mx = fmaxf(mx, __shfl_xor(mx, m, 64));
+        sum += __shfl_xor(sum, m, 64);
+        mn = min(mn, __shfl_xor(mn, m, 64));
     }
-    if ((threadIdx.x & 63) == 0) redi[threadIdx.x >> 6] = cand;
+    __syncthreads();                                             // the last round has been read
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = Red{mx, sum, mn};
     __syncthreads();
-    for (int w = 0; w < 8; ++w) cand = redi[w] < cand ? redi[w] : cand;
-    const float sum = block_sum(mx > -INFINITY ? se * expf(mx - top) : 0.f, red);
-    float l = top + logf(sum);
-    if (block_max(nan ? 1.f : 0.f, red) > 0.f) l = __uint_as_float(0x7FC00000u);
-    // the teacher's list: softmax over its entries, the best of them, the row's loss
+    Red r = red[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) { r.a = fmaxf(r.a, red[w].a); r.b += red[w].b; r.c = min(r.c, red[w].c); }
+    return r;
+}
+
+__global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
+    __shared__ Red red[4];
+    __shared__ float le[DISTILL_MAX_K];
+    __shared__ __attribute__((aligned(16))) int li[DISTILL_MAX_K];
+    __shared__ unsigned last;
+    const int64_t b = blockIdx.y;
+    const int tid = threadIdx.x;
+    const float inv = __fdiv_rn(1.f, a.temp[0]);
+    const float* part = a.part + b * a.lds;
+    // ---- this segment's columns: the slabs' sum, the maximum of z and its first column, the sum of exp
+    float mx, se;
+    int am;
+    bool nan;
+    {
+        const int64_t j0 = (int64_t)blockIdx.x * DISTILL_SEG + tid * 4;
+        v4f x[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+        bool in[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) in[u] = j0 + u * 1024 < a.T;
+        for (int p = 0; p < a.splits; p += 4) {                   // four slabs' loads in flight; slabs in order
+            v4f y[4][2];
+#pragma unroll
+            for (int o = 0; o < 4; ++o)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if (p + o < a.splits && in[u]) y[o][u] = *(const v4f*)(part + (p + o) * a.slab + j0 + u * 1024);
+#pragma unroll
+            for (int o = 0; o < 4; ++o)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if (p + o < a.splits && in[u]) x[u] += y[o][u];
+        }
+        mx = -INFINITY;
+        nan = false;
+        am = INT32_MAX;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (!in[u]) continue;
+            if (a.splits > 1) *(v4f*)(a.s + b * a.lds + j0 + u * 1024) = x[u];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (j0 + u * 1024 + c >= a.T) { x[u][c] = -INFINITY; continue; }
+                x[u][c] *= inv;
+                if (x[u][c] > mx) { mx = x[u][c]; am = (int)(j0 + u * 1024 + c); }
+                nan |= x[u][c] != x[u][c];
+            }
+        }
+        const float mine = mx;
+        const Red r = block_red(mx, 0.f, 0, red);
+        mx = r.a;
+        se = 0.f;
+        if (mx > -INFINITY)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                if (in[u])
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) se += exp_neg(x[u][c] - mx);
+        const Red r2 = block_red(nan ? 1.f : 0.f, se, mine == mx && mx > -INFINITY ? am : INT32_MAX, red);
+        nan = r2.a > 0.f;
+        se = r2.b;
+        am = r2.c;
+    }
+    if (a.segs > 1) {
+        float* seg = a.seg + b * a.segs * 4;
+        if (tid == 0) {
+            put(seg + blockIdx.x * 4, mx);
+            put(seg + blockIdx.x * 4 + 1, se);
+            put(seg + blockIdx.x * 4 + 2, __int_as_float(am));
+            put(seg + blockIdx.x * 4 + 3, nan ? 1.f : 0.f);
+        }
+        if (!arrive_last(a.cnt + b, (unsigned)a.segs, &last)) return;
+        // ---- the last segment of the row: all of them together
+        mx = -INFINITY;
+        float any = 0.f;
+        for (int i = tid; i < a.segs; i += 256) { mx = fmaxf(mx, get(seg + i * 4)); any = fmaxf(any, get(seg + i * 4 + 3)); }
+        const Red r = block_red(mx, any, 0, red);
+        mx = r.a;
+        nan = r.b > 0.f;
+        se = 0.f;
+        am = INT32_MAX;
+        if (mx > -INFINITY)
+            for (int i = tid; i < a.segs; i += 256) {
+                const float m = get(seg + i * 4);
+                if (m > -INFINITY) se += get(seg + i * 4 + 1) * exp_neg(m - mx);
+                if (m == mx) am = min(am, __float_as_int(get(seg + i * 4 + 2)));
+            }
+        const Red r2 = block_red(0.f, se, am, red);
+        se = r2.b;
+        am = r2.c;
+    }
+    float l = nan ? __uint_as_float(0x7FC00000u) : mx + logf(se);
+    // ---- the teacher's list: softmax over its entries, the best of them, the row's loss
     const int64_t* idx = a.idx + b * a.k;
     const float* score = a.score + b * a.k;
-    float best = -INFINITY;
-    float bad = 0.f, some = 0.f, tnan = 0.f;
-    for (int i = threadIdx.x; i < a.k; i += 512) {
-        const int64_t at = idx[i];
-        const float v = score[i];
-        const bool on = at >= 0 && !(v == -INFINITY);
-        if (on) {
-            some = 1.f;
-            if (at >= a.T) bad = 1.f;                            // a column that is not there: the row becomes NaN
-            if (!(v < INFINITY)) tnan = 1.f;                     // so does a score that is no number to weigh
-            best = fmaxf(best, v);
+    float v[4], best = -INFINITY, bad = 0.f;
+    int at[4], some = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int i = tid + u * 256;
+        at[u] = -1;
+        v[u] = -INFINITY;
+        if (i >= a.k) continue;
+        const int64_t j = idx[i];
+        const float x = score[i];
+        if (j >= 0 && !(x == -INFINITY)) {
+            some = 1;
+            if (j >= a.T || !(x < INFINITY)) bad = 1.f;          // a column that is not there, a score that is no number: the row is NaN
+            else { at[u] = (int)j; v[u] = x; best = fmaxf(best, x); }
         }
-        ts[i] = on ? v : -INFINITY;
+        li[i] = at[u];
     }
-    some = block_max(some, red);
-    best = block_max(best, red);
-    bad = block_max(fmaxf(bad, tnan), red);
-    float e = 0.f;
-    int64_t first = INT64_MAX;
-    for (int i = threadIdx.x; i < a.k; i += 512) {
-        const float v = ts[i];
-        if (v == -INFINITY) continue;
-        e += expf(__fdiv_rn(v - best, a.teacher_temp));
-        if (v == best && i < first) first = i;
+    {
+        const Red r = block_red(best, bad, -some, red);
+        best = r.a;
+        bad = r.b;
+        some = -r.c;
     }
-    e = block_sum(e, red);
-    for (int m = 32; m > 0; m >>= 1) {
-        const int o = __shfl_xor((int)(first > 0x7FFFFFFF ? 0x7FFFFFFF : first), m, 64);
-        first = o < first ? o : first;
+    float z[4];                                                  // on their way while the shares are summed
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        z[u] = 0.f;
+        if (at[u] >= 0)
+            for (int p = 0; p < a.splits; ++p) z[u] += part[p * a.slab + at[u]];
+        z[u] *= inv;
     }
-    if ((threadIdx.x & 63) == 0) redi[threadIdx.x >> 6] = first;
-    __syncthreads();
-    for (int w = 0; w < 8; ++w) first = redi[w] < first ? redi[w] : first;
-    const float loge = logf(e);
-    float part = 0.f;
-    for (int i = threadIdx.x; i < a.k; i += 512) {
-        const float v = ts[i];
-        float p = 0.f;
-        if (v != -INFINITY && bad == 0.f) {
-            const float x = __fdiv_rn(v - best, a.teacher_temp);
-            p = expf(x) / e;
-            if (p > 0.f) part += p * ((x - loge) - __fdiv_rn(s[idx[i]], t));
+    float e[4], esum = 0.f;
+    int first = INT32_MAX;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int i = tid + u * 256;
+        e[u] = 0.f;
+        v[u] = __fdiv_rn(v[u] - best, a.teacher_temp);
+        if (at[u] >= 0) {
+            e[u] = exp_neg(v[u]);
+            if (v[u] == 0.f) first = min(first, i);
         }
-        a.t[b * a.k + i] = p;
+        esum += e[u];
+        if (i < a.k) le[i] = e[u];
     }
-    part = block_sum(part, red);
+    {
+        const Red r = block_red(0.f, esum, first, red);
+        esum = r.b;
+        first = r.c;
+    }
+    const float loge = logf(esum);
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int i = tid + u * 256;
+        if (i >= a.k) continue;
+        const float p = bad == 0.f && at[u] >= 0 ? __fdiv_rn(e[u], esum) : 0.f;
+        if (p > 0.f) sum += p * ((v[u] - loge) - z[u]);
+        // a column's shares together, at its first entry
+        float all = 0.f;
+        bool mine = at[u] >= 0 && bad == 0.f;
+        if (mine)
+            for (int o = 0; o < a.k; ++o)
+                if (li[o] == at[u]) { mine = mine && o >= i; all += le[o]; }
+        a.t[b * a.k + i] = mine ? __fdiv_rn(all, esum) : 0.f;
+        a.li[b * a.k + i] = mine ? at[u] : -1;
+    }
+    sum = block_red(0.f, sum, 0, red).b;
     if (bad > 0.f) l = __uint_as_float(0x7FC00000u);
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         a.lse[b] = l;
-        const bool hit = some > 0.f && bad == 0.f && cand == idx[first];
-        __hip_atomic_store(a.row + b, some > 0.f ? part + l : 0.f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(a.row + a.B + b, hit ? 1.f : 0.f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(a.row + 2 * a.B + b, some, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // the three stores have left (device scope) before the arrival counts
-        last = __hip_atomic_fetch_add(a.cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)a.B - 1 ? 1u : 0u;
+        put(a.row + b, some ? sum + l : 0.f);
+        put(a.row + a.B + b, some && bad == 0.f && am == li[first] ? 1.f : 0.f);
+        put(a.row + 2 * a.B + b, some ? 1.f : 0.f);
     }
-    __syncthreads();
-    if (!last) return;
-    // the last row to arrive sums them, in fixed order; its loads go past the caches like the stores did
-    float ls = 0.f, hs = 0.f, ns = 0.f;
-    for (int64_t i = threadIdx.x; i < a.B; i += 512) {
-        ls += __hip_atomic_load(a.row + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        hs += __hip_atomic_load(a.row + a.B + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        ns += __hip_atomic_load(a.row + 2 * a.B + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (!arrive_last(a.cnt + a.B, (unsigned)a.B, &last)) return;
+    // ---- the last row: the means
+    float ls = 0.f, hs = 0.f;
+    int ns = 0;
+    for (int64_t i = tid; i < a.B; i += 256) {
+        ls += get(a.row + i);
+        hs += get(a.row + a.B + i);
+        ns += get(a.row + 2 * a.B + i) > 0.f ? 1 : 0;
     }
-    ls = block_sum(ls, red);
-    hs = block_sum(hs, red);
-    ns = block_sum(ns, red);
-    if (threadIdx.x == 0) {
-        const float n = fmaxf(ns, 1.f);
+    ls = block_red(0.f, ls, 0, red).b;
+    hs = block_red(0.f, hs, 0, red).b;
+    const float n = fmaxf(block_red(0.f, (float)ns, 0, red).b, 1.f);
+    if (tid == 0) {
         a.out_loss[0] = __fdiv_rn(ls, n);
         a.out_agree[0] = __fdiv_rn(hs, n);
         a.stat[0] = __fdiv_rn(1.f, n);
     }
 }
 
-// ---- the gradient of the logits ------------------------------------------------------------------------------------------
+// ---- softmax - target ----------------------------------------------------------------------------------------------------
+enum { G_F32, G_F16, G_BF16 };
 struct GradArgs {
     const float* s;                  // [B][lds]
     int64_t lds;
     const float* lse;
     const float* t;
-    const int64_t* idx;
+    const int* li;
     const float* has;                // [B]: 1 where the row has an entry
-    const float* stat;
     const float* temp;
-    const float* grad_out;
-    int64_t T, ldg;
+    int64_t B, T, ldg;
     int k;
-    float* g;                        // [B][ldg]: (g / temp); zeros from T on
-    float* dt;                       // [B][segments]: sums of g z
+    int form;                        // G_F32, G_F16 (G_F32 where flag is set) or G_BF16
+    const unsigned* flag;
+    void* g;                         // fp32 [B][ldg], or two parts of 16 bits; zeros from T on
+    float* dt;                       // [B][segments]: sums of (softmax - target) z
 };
 
 __global__ __launch_bounds__(256) void distill_grad_kernel(const GradArgs a) {
-    __shared__ __attribute__((aligned(16))) float buf[DISTILL_SEG];
-    __shared__ int li[DISTILL_MAX_K];
-    __shared__ float lt[DISTILL_MAX_K];
-    __shared__ float red[4];
+    __shared__ __attribute__((aligned(16))) float target[DISTILL_SEG];
+    __shared__ Red red[4];
     const int64_t b = blockIdx.y, j0 = (int64_t)blockIdx.x * DISTILL_SEG;
-    const float* s = a.s + b * a.lds + j0;
-    float* g = a.g + b * a.ldg + j0;
-    const int n = (int)min((int64_t)DISTILL_SEG, a.ldg - j0), valid = (int)max((int64_t)0, min((int64_t)DISTILL_SEG, a.T - j0));
+    const int tid = threadIdx.x;
     const bool has = a.has[b] > 0.f;
-    const float w = has ? a.grad_out[0] * a.stat[0] : 0.f;
-    const float temp = a.temp[0], l = a.lse[b];
-    if (has)
-        for (int i = threadIdx.x; i < a.k; i += 256) {
-            const int64_t at = a.idx[b * a.k + i] - j0;
-            const float p = a.t[b * a.k + i];
-            li[i] = p != 0.f && at >= 0 && at < valid ? (int)at : -1;
-            lt[i] = p;
-        }
-    for (int i = threadIdx.x * 4; i < n; i += 1024) {
-        v4f x = *(const v4f*)(s + i), y;                          // ldg columns are there in s too
+    const float inv = __fdiv_rn(1.f, a.temp[0]), l = a.lse[b];
+    const int form = a.form == G_F16 && *a.flag ? G_F32 : a.form;
+    v4f x[2];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) y[c] = i + c < valid && has ? expf(__fdiv_rn(x[c], temp) - l) : 0.f;
-        *(v4f*)(buf + i) = y;
-    }
+    for (int u = 0; u < 2; ++u)
+        if (j0 + tid * 4 + u * 1024 < a.ldg) x[u] = *(const v4f*)(a.s + b * a.lds + j0 + tid * 4 + u * 1024);   // ldg columns are there in s too
+#pragma unroll
+    for (int u = 0; u < 2; ++u) *(v4f*)(target + tid * 4 + u * 1024) = v4f{0.f, 0.f, 0.f, 0.f};
     __syncthreads();
     if (has)
-        for (int i = threadIdx.x; i < a.k; i += 256) {
-            const int at = li[i];
-            if (at < 0) continue;
-            float p = 0.f;
-            bool mine = true;                                    // the first of the entries that name this column takes them all
-            for (int o = 0; o < a.k; ++o)
-                if (li[o] == at) { if (o < i) { mine = false; break; } p += lt[o]; }
-            if (mine) buf[at] -= p;
+        for (int i = tid; i < a.k; i += 256) {
+            const int at = a.li[b * a.k + i];                    // no column twice
+            if (at >= j0 && at < j0 + DISTILL_SEG) target[at - j0] = a.t[b * a.k + i];
         }
     __syncthreads();
     float dt = 0.f;
-    for (int i = threadIdx.x * 4; i < n; i += 1024) {
-        const v4f x = *(const v4f*)(s + i);
-        v4f y = *(const v4f*)(buf + i);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int64_t j = j0 + tid * 4 + u * 1024;
+        if (j >= a.ldg) continue;
+        const v4f tg = *(const v4f*)(target + tid * 4 + u * 1024);
+        v4f y;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            y[c] = has ? y[c] * w : 0.f;
-            if (i + c < valid && has) dt += y[c] * __fdiv_rn(x[c], temp);
-            y[c] = __fdiv_rn(y[c], temp);
+            const float z = x[u][c] * inv;
+            y[c] = j + c < a.T && has ? exp_neg(z - l) - tg[c] : 0.f;
+            if (j + c < a.T && has) dt += y[c] * z;
         }
-        *(v4f*)(g + i) = y;
+        if (form == G_F32) *(v4f*)((float*)a.g + b * a.ldg + j) = y;
+        else {
+            uint32_t lo[2], hi[2];
+            if (form == G_F16) {
+                split_pair(y[0] * G_SCALE, y[1] * G_SCALE, lo);
+                split_pair(y[2] * G_SCALE, y[3] * G_SCALE, hi);
+            } else {
+                uint32_t l3[3], h3[3];
+                split_pair(y[0], y[1], l3);
+                split_pair(y[2], y[3], h3);
+                lo[0] = l3[0]; lo[1] = l3[1]; hi[0] = h3[0]; hi[1] = h3[1];
+            }
+            uint16_t* out = (uint16_t*)a.g + b * a.ldg + j;
+            *(uint2*)out = uint2{lo[0], hi[0]};
+            *(uint2*)(out + a.B * a.ldg) = uint2{lo[1], hi[1]};
+        }
     }
-    dt = block_sum(dt, red);
-    if (threadIdx.x == 0) a.dt[b * gridDim.x + blockIdx.x] = dt;
+    dt = block_red(0.f, dt, 0, red).b;
+    if (tid == 0) a.dt[b * gridDim.x + blockIdx.x] = dt;
 }
 
 // ---- sums of the split products' slabs, and of the temperature's gradient ------------------------------------------------
@@ -499,26 +728,36 @@ struct SumArgs {
     int blocks0;                     // workgroups of the first
     const float* dt;
     int64_t ndt;
-    const float* temp;
+    const float *f0, *f1, *f2;       // grad_out, 1 / rows, temp
     float* d_temp;                   // null: not wanted
 };
 
 template <bool BF16>
 __global__ __launch_bounds__(256) void distill_sum_kernel(const SumArgs a) {
-    __shared__ float red[4];
+    __shared__ Red red[4];
+    const float f = factor_of(a.f0, a.f1, a.f2);
     if (blockIdx.x == gridDim.x - 1) {                            // the last workgroup: the temperature
         if (!a.d_temp) return;
         float v = 0.f;
         for (int64_t i = threadIdx.x; i < a.ndt; i += 256) v += a.dt[i];
-        v = block_sum(v, red);
-        if (threadIdx.x == 0) a.d_temp[0] = -__fdiv_rn(v, a.temp[0]);
+        v = block_red(0.f, v, 0, red).b;
+        if (threadIdx.x == 0) a.d_temp[0] = -v * f;
         return;
     }
     const int which = (int)blockIdx.x >= a.blocks0;
     const int64_t i = ((int64_t)(blockIdx.x - (which ? a.blocks0 : 0)) * 256 + threadIdx.x) * 4;
     if (i >= a.n[which]) return;
-    v4f x = *(const v4f*)(a.part[which] + i);
-    for (int p = 1; p < a.splits[which]; ++p) x += *(const v4f*)(a.part[which] + p * a.n[which] + i);
+    v4f x = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < a.splits[which]; p += 4) {
+        v4f y[4];
+#pragma unroll
+        for (int o = 0; o < 4; ++o)
+            if (p + o < a.splits[which]) y[o] = *(const v4f*)(a.part[which] + (p + o) * a.n[which] + i);
+#pragma unroll
+        for (int o = 0; o < 4; ++o)
+            if (p + o < a.splits[which]) x += y[o];
+    }
+    x *= f;
     if constexpr (BF16) {
         uint32_t lo = f32_to_bf16_bits(x[0]) | f32_to_bf16_bits(x[1]) << 16, hi = f32_to_bf16_bits(x[2]) | f32_to_bf16_bits(x[3]) << 16;
         *(uint2*)((uint16_t*)a.out[which] + i) = uint2{lo, hi};
@@ -528,52 +767,86 @@ __global__ __launch_bounds__(256) void distill_sum_kernel(const SumArgs a) {
 // ---- plans ---------------------------------------------------------------------------------------------------------------
 struct Plan { int tile, splits; int64_t kstep; int nm, nn; };
 
-// Tiles of 128 x 128 where they fill the chip, 64 x 64 otherwise; k is split until there are two workgroups a CU (512), as long as a
-// split keeps four stages.
-static Plan plan(int64_t m, int64_t n, int64_t k, int stage) {
+// Tiles of 128 x 128 where two workgroups of them a CU (512) come together, 64 x 64 otherwise (four a CU); k is split until that many
+// workgroups run, as long as a split keeps four stages of 64.
+static Plan plan(int64_t m, int64_t n, int64_t k) {
     Plan p;
     auto tiles = [&](int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-    p.tile = m > 64 && n > 64 && tiles(128) * (k / (4 * stage) + 1) >= 512 ? 128 : 64;
+    const int64_t stages = (k + 63) / 64;
+    p.tile = m > 64 && n > 64 && tiles(128) * (stages / 8 + 1) >= 512 ? 128 : 64;
     p.nm = (int)((m + p.tile - 1) / p.tile);
     p.nn = (int)((n + p.tile - 1) / p.tile);
-    const int64_t stages = (k + stage - 1) / stage;
-    int64_t sp = 512 / ((int64_t)p.nm * p.nn);
-    if (sp > stages / 4) sp = stages / 4;
+    int64_t sp = (p.tile == 128 ? 512 : 1024) / ((int64_t)p.nm * p.nn);
+    const int64_t most = p.tile == 128 ? stages / 8 : stages / 2;
+    if (sp > most) sp = most;
     if (sp > 32) sp = 32;
     if (sp < 1) sp = 1;
     const int64_t per = (stages + sp - 1) / sp;
-    p.kstep = per * stage;
+    p.kstep = per * 64;
     p.splits = (int)((stages + per - 1) / per);
     return p;
 }
 
 static inline size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 
-struct FwdLayout { Plan s; int64_t lds; size_t off_lse, off_t, off_row, off_stat, off_cnt, total; };
-static int stage_of(int dtype, bool fwd) { (void)fwd; return dtype == ABC_DT_BF16 ? 64 : 32; }
+struct FwdLayout {
+    Plan s;
+    bool fast;                       // fp32 by fp16 parts
+    int64_t lds;
+    int segs;
+    size_t off_s, off_seg, off_lse, off_t, off_li, off_row, off_stat, off_cnt, off_q, off_qout, off_flag, total;
+};
 
 static FwdLayout fwd_layout(int dtype, int64_t B, int64_t T, int d, int k) {
     FwdLayout L;
-    L.s = plan(B, T, d, stage_of(dtype, true));
+    L.s = plan(B, T, d);
     L.lds = (T + 7) / 8 * 8;
+    L.segs = (int)((T + DISTILL_SEG - 1) / DISTILL_SEG);
+    // from about 8 GFLOP a product on, half the matrix work is worth the launches that find out and then return
+    L.fast = dtype == ABC_DT_F32 && L.s.tile == 128 && 2.0 * (double)B * (double)T * d >= 8e9;
     size_t o = up((size_t)L.s.splits * B * L.lds * 4);
+    L.off_s = 0;
+    if (L.s.splits > 1) { L.off_s = o; o += up((size_t)B * L.lds * 4); }
+    L.off_seg = o; o += up((size_t)B * L.segs * 16);
     L.off_lse = o; o += up((size_t)B * 4);
     L.off_t = o; o += up((size_t)B * k * 4);
+    L.off_li = o; o += up((size_t)B * k * 4);
     L.off_row = o; o += up((size_t)B * 12);
     L.off_stat = o; o += 256;
-    L.off_cnt = o; o += 256;
+    L.off_cnt = o; o += up((size_t)(B + 1) * 4);
+    L.off_q = o; o += L.fast ? up((size_t)B * d * 4) : 0;
+    L.off_qout = o; o += L.fast ? up((size_t)B * 4) : 0;
+    L.off_flag = o; o += 256;
     L.total = o;
     return L;
 }
 
 struct BwdLayout { Plan q, p; int64_t ldg; int segs; size_t off_g, off_dt, off_pq, off_pp, total; };
-static BwdLayout bwd_layout(int dtype, int64_t B, int64_t C, int64_t T, int d, bool dq, bool dp) {
+static BwdLayout bwd_layout(int64_t B, int64_t C, int64_t T, int d, bool fast, bool dq, bool dp) {
     BwdLayout L;
     L.ldg = (T + 7) / 8 * 8;
-    L.segs = (int)((T + DISTILL_SEG - 1) / DISTILL_SEG);
-    L.q = plan(B, d, L.ldg, 32);
-    L.p = plan(C, d, B, 32);
-    (void)dtype;
+    L.segs = (int)((L.ldg + DISTILL_SEG - 1) / DISTILL_SEG);
+    L.q = plan(B, d, T);
+    L.p = plan(C, d, B);
+    if (fast || (L.q.tile == 128) != (L.p.tile == 128)) {         // one launch, one kind of tile: that of the larger product
+        const int tile = fast || (T > C && B > 64 ? L.q.tile : L.p.tile) == 128 ? 128 : 64;
+        auto with = [&](Plan& x, int64_t m, int64_t n, int64_t k) {
+            if (x.tile == tile) return;
+            x.tile = tile;
+            x.nm = (int)((m + tile - 1) / tile);
+            x.nn = (int)((n + tile - 1) / tile);
+            int64_t sp = (tile == 128 ? 512 : 1024) / ((int64_t)x.nm * x.nn);
+            const int64_t stages = (k + 63) / 64;
+            if (sp > stages / 2) sp = stages / 2;
+            if (sp > 32) sp = 32;
+            if (sp < 1) sp = 1;
+            const int64_t per = (stages + sp - 1) / sp;
+            x.kstep = per * 64;
+            x.splits = (int)((stages + per - 1) / per);
+        };
+        with(L.q, B, d, T);
+        with(L.p, C, d, B);
+    }
     size_t o = up((size_t)B * L.ldg * 4);
     L.off_g = 0;
     L.off_dt = o; o += up((size_t)B * L.segs * 4);
@@ -586,7 +859,7 @@ static BwdLayout bwd_layout(int dtype, int64_t B, int64_t C, int64_t T, int d, b
 static int distill_check(int dtype, int64_t B, int64_t C, int64_t M, int d, int k) {
     if (dtype != ABC_DT_F32 && dtype != ABC_DT_BF16) return abc_fail_invalid("distill: embeddings must be f32 or bf16");
     if (B < 1 || C < 1 || M < 0) return abc_fail_invalid("distill: need at least one query and one candidate");
-    if (B > 65535 || C + M > 0x7FFFFFF0ll) return abc_fail_invalid("distill: at most 65535 queries and 2^31 - 16 candidates");
+    if (B > 65535 || C > 0x7FFFFFF0ll || M > 0x7FFFFFF0ll || C + M > 0x7FFFFFF0ll) return abc_fail_invalid("distill: at most 65535 queries and 2^31 - 16 candidates");
     if (d < 8 || d % 8 || d > 65536) return abc_fail_invalid("distill: d must be a multiple of 8 in [8, 65536]");
     if (k < 1 || k > DISTILL_MAX_K) return abc_fail_invalid("distill: a list has 1 to 1024 entries");
     return ABC_OK;
@@ -598,21 +871,46 @@ extern "C" size_t abc_distill_workspace_bytes(int dtype, int64_t B, int64_t C, i
 }
 extern "C" size_t abc_distill_bwd_workspace_bytes(int dtype, int64_t B, int64_t C, int64_t M, int d, int k) {
     if (distill_check(dtype, B, C, M, d, k)) return 0;
-    return bwd_layout(dtype, B, C, C + M, d, true, true).total;
-}
-
-template <class LA, class LB, int PA, int PB, int KEEP, int T, int NKB, bool OUT_BF16>
-static void launch_tile(const GemmArgs& g, hipStream_t st) {
-    const unsigned grid = (unsigned)((g.nn * g.nm * g.splits + 7) / 8 * 8);
-    hipLaunchKernelGGL((distill_gemm_kernel<LA, LB, PA, PB, KEEP, T, T, NKB, OUT_BF16>), dim3(grid), dim3(256), (PA + PB) * NKB * T * 64, st, g);
+    return bwd_layout(B, C, C + M, d, fwd_layout(dtype, B, C + M, d, k).fast, true, true).total;
 }
 
 static GemmArgs gemm_args(const Side& a, const Side& b, int64_t k, const Plan& p, void* out, int64_t ldo, int64_t slab) {
-    GemmArgs g;
+    GemmArgs g = {};
     g.a = a; g.b = b; g.k = k; g.splits = p.splits; g.kstep = p.kstep; g.nm = p.nm; g.nn = p.nn;
-    g.out = out; g.ldo = ldo; g.slab = slab; g.clear = nullptr;
+    g.out = out; g.ldo = ldo; g.slab = slab; g.scale = 1.f;
     return g;
 }
+static unsigned groups_of(const GemmArgs& g) { return (unsigned)(((int64_t)g.nn * g.nm * g.splits + 7) / 8 * 8); }
+
+template <class C>
+static void launch_scores(const GemmArgs& g, const unsigned* flag, unsigned run_if, unsigned* raise, const unsigned* rows_out, int64_t B,
+                          unsigned* clear, int nclear, hipStream_t st) {
+    hipLaunchKernelGGL((distill_scores_kernel<C>), dim3(groups_of(g)), dim3(256), C::LDS, st, g, flag, run_if, raise, rows_out, B, clear, nclear);
+}
+template <class CQ, class CP>
+static void launch_grads(const GemmArgs& gq, const GemmArgs& gp, bool dq, bool dp, const unsigned* flag, unsigned run_if, hipStream_t st) {
+    const unsigned n0 = dq ? groups_of(gq) : 0, n1 = dp ? groups_of(gp) : 0;
+    const size_t lds = (size_t)(CQ::LDS > CP::LDS ? CQ::LDS : CP::LDS);
+    hipLaunchKernelGGL((distill_grads_kernel<CQ, CP>), dim3(n0 + n1), dim3(256), lds, st, gq, gp, (int)n0, flag, run_if);
+}
+
+// s: bf16; fp32 by three bf16 parts (128 / 64 wide tiles); fp32 by two fp16 parts (the queries' are ready)
+typedef Cfg<LoadKC<RAW, 1, 128, 2, 1>, LoadKC<RAW, 1, 128, 2, 1>, 1, 1, 1, 128, 128, 2, 1, 2, false, false> ScoresB128;
+typedef Cfg<LoadKC<RAW, 1, 64, 2, 2>, LoadKC<RAW, 1, 64, 2, 2>, 1, 1, 1, 64, 64, 2, 2, 2, false, false> ScoresB64;
+typedef Cfg<LoadKC<SPLIT_B3, 3, 128, 1, 1>, LoadKC<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, false, false> ScoresF128;
+typedef Cfg<LoadKC<SPLIT_B3, 3, 64, 1, 3>, LoadKC<SPLIT_B3, 3, 64, 1, 3>, 3, 3, 3, 64, 64, 1, 3, 1, false, false> ScoresF64;
+typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKC<SPLIT_H2, 2, 128, 1, 1, true>, 2, 2, 2, 128, 128, 1, 1, 2, true, false> ScoresH128;
+// dq = g cand, dc = g^T q
+typedef Cfg<LoadKC<RAW, 2, 128, 2, 1>, LoadKS<RAW, 1, 128, 2, 1>, 2, 1, 2, 128, 128, 2, 1, 1, false, true> GradQB128;
+typedef Cfg<LoadKS<RAW, 2, 128, 2, 1>, LoadKS<RAW, 1, 128, 2, 1>, 2, 1, 2, 128, 128, 2, 1, 1, false, true> GradPB128;
+typedef Cfg<LoadKC<RAW, 2, 64, 2, 2>, LoadKS<RAW, 1, 64, 2, 2>, 2, 1, 2, 64, 64, 2, 2, 1, false, true> GradQB64;
+typedef Cfg<LoadKS<RAW, 2, 64, 2, 2>, LoadKS<RAW, 1, 64, 2, 2>, 2, 1, 2, 64, 64, 2, 2, 1, false, true> GradPB64;
+typedef Cfg<LoadKC<SPLIT_B3, 3, 128, 1, 1>, LoadKS<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, false, false> GradQF128;
+typedef Cfg<LoadKS<SPLIT_B3, 3, 128, 1, 1>, LoadKS<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, false, false> GradPF128;
+typedef Cfg<LoadKC<SPLIT_B3, 3, 64, 1, 2>, LoadKS<SPLIT_B3, 3, 64, 1, 2>, 3, 3, 3, 64, 64, 1, 2, 1, false, false> GradQF64;
+typedef Cfg<LoadKS<SPLIT_B3, 3, 64, 1, 2>, LoadKS<SPLIT_B3, 3, 64, 1, 2>, 3, 3, 3, 64, 64, 1, 2, 1, false, false> GradPF64;
+typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKS<SPLIT_H2, 2, 128, 1, 1>, 2, 2, 2, 128, 128, 1, 1, 2, true, false> GradQH128;
+typedef Cfg<LoadKS<RAW, 2, 128, 1, 1>, LoadKS<RAW, 2, 128, 1, 1>, 2, 2, 2, 128, 128, 1, 1, 2, true, false> GradPH128;
 
 extern "C" int abc_distill_fwd(int dtype, const void* q, const void* p, const void* memory, const float* temp, const int64_t* teacher_idx,
                                const float* teacher_score, float teacher_temp, int64_t B, int64_t C, int64_t M, int d, int k,
@@ -628,86 +926,85 @@ extern "C" int abc_distill_fwd(int dtype, const void* q, const void* p, const vo
     if ((uintptr_t)ws & 15) return abc_fail_invalid("distill_fwd: workspace must be 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;
     char* w = (char*)ws;
-    const Side sq{q, q, B, d, B}, sc{p, memory, C, d, T};
-    GemmArgs g = gemm_args(sq, sc, d, L.s, w, L.lds, B * L.lds);
-    g.clear = (unsigned*)(w + L.off_cnt);
+    unsigned* cnt = (unsigned*)(w + L.off_cnt);
+    unsigned* flag = (unsigned*)(w + L.off_flag);
+    const int nc = (int)B + 1;
+    const Side sq{q, q, B, d, B, 0}, sc{p, memory, C, d, T, 0};
+    const GemmArgs g = gemm_args(sq, sc, d, L.s, w, L.lds, B * L.lds);
     if (dtype == ABC_DT_BF16) {
-        if (L.s.tile == 128) launch_tile<LoadKC<true, 1, 128, 2>, LoadKC<true, 1, 128, 2>, 1, 1, 1, 128, 2, false>(g, st);
-        else launch_tile<LoadKC<true, 1, 64, 2>, LoadKC<true, 1, 64, 2>, 1, 1, 1, 64, 2, false>(g, st);
-    } else {
-        if (L.s.tile == 128) launch_tile<LoadKC<false, 3, 128, 1>, LoadKC<false, 3, 128, 1>, 3, 3, 3, 128, 1, false>(g, st);
-        else launch_tile<LoadKC<false, 3, 64, 1>, LoadKC<false, 3, 64, 1>, 3, 3, 3, 64, 1, false>(g, st);
-    }
+        if (L.s.tile == 128) launch_scores<ScoresB128>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
+        else launch_scores<ScoresB64>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
+    } else if (L.fast) {
+        unsigned* qout = (unsigned*)(w + L.off_qout);
+        hipLaunchKernelGGL(distill_split_kernel, dim3((unsigned)B), dim3(256), 0, st, (const float*)q, d, B * d, (uint16_t*)(w + L.off_q), qout, flag);
+        GemmArgs h = g;
+        h.a = Side{w + L.off_q, w + L.off_q, B, d, B, B * d * 2};
+        launch_scores<ScoresH128>(h, nullptr, 0, flag, qout, B, cnt, nc, st);
+        launch_scores<ScoresF128>(g, flag, 1, nullptr, nullptr, 0, nullptr, 0, st);
+    } else if (L.s.tile == 128) launch_scores<ScoresF128>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
+    else launch_scores<ScoresF64>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
     RowArgs r;
-    r.s = (float*)w; r.splits = L.s.splits; r.slab = B * L.lds; r.lds = L.lds; r.temp = temp; r.idx = teacher_idx; r.score = teacher_score;
-    r.teacher_temp = teacher_temp; r.B = B; r.T = T; r.k = k; r.lse = (float*)(w + L.off_lse); r.t = (float*)(w + L.off_t);
-    r.row = (float*)(w + L.off_row); r.stat = (float*)(w + L.off_stat); r.cnt = (unsigned*)(w + L.off_cnt);
-    r.out_loss = out_loss; r.out_agree = out_agree;
-    hipLaunchKernelGGL(distill_row_kernel, dim3((unsigned)B), dim3(512), 0, st, r);
+    r.part = (const float*)w; r.s = (float*)(w + L.off_s); r.splits = L.s.splits; r.segs = L.segs; r.slab = B * L.lds; r.lds = L.lds;
+    r.temp = temp; r.idx = teacher_idx; r.score = teacher_score; r.teacher_temp = teacher_temp; r.B = B; r.T = T; r.k = k;
+    r.seg = (float*)(w + L.off_seg); r.lse = (float*)(w + L.off_lse); r.t = (float*)(w + L.off_t); r.li = (int*)(w + L.off_li);
+    r.row = (float*)(w + L.off_row); r.stat = (float*)(w + L.off_stat); r.cnt = cnt; r.out_loss = out_loss; r.out_agree = out_agree;
+    hipLaunchKernelGGL(distill_row_kernel, dim3((unsigned)L.segs, (unsigned)B), dim3(256), 0, st, r);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? ABC_OK : abc_fail_hip(e, "distill_fwd launch");
 }
 
-extern "C" int abc_distill_bwd(int dtype, const void* q, const void* p, const void* memory, const float* temp, const int64_t* teacher_idx,
-                               const float* grad_out, int64_t B, int64_t C, int64_t M, int d, int k, void* dq, void* dp, float* d_temp,
-                               const void* fwd_ws, size_t fwd_ws_bytes, void* ws, size_t ws_bytes, void* stream) {
+extern "C" int abc_distill_bwd(int dtype, const void* q, const void* p, const void* memory, const float* temp, const float* grad_out,
+                               int64_t B, int64_t C, int64_t M, int d, int k, void* dq, void* dp, float* d_temp, const void* fwd_ws,
+                               size_t fwd_ws_bytes, void* ws, size_t ws_bytes, void* stream) {
     int rc = distill_check(dtype, B, C, M, d, k);
     if (rc) return rc;
-    if (!q || !p || (M && !memory) || !temp || !teacher_idx || !grad_out || !fwd_ws) return abc_fail_invalid("distill_bwd: null pointer");
+    if (!q || !p || (M && !memory) || !temp || !grad_out || !fwd_ws) return abc_fail_invalid("distill_bwd: null pointer");
     if (((uintptr_t)q | (uintptr_t)p | (uintptr_t)(M ? memory : nullptr) | (uintptr_t)dq | (uintptr_t)dp) & 15)
         return abc_fail_invalid("distill_bwd: embeddings and gradients must be 16-byte aligned");
     const int64_t T = C + M;
     const FwdLayout F = fwd_layout(dtype, B, T, d, k);
     if (fwd_ws_bytes < F.total) return abc_fail_ws(F.total, fwd_ws_bytes);
-    const BwdLayout L = bwd_layout(dtype, B, C, T, d, dq, dp);
+    const BwdLayout L = bwd_layout(B, C, T, d, F.fast, dq, dp);
     if (!ws || ws_bytes < L.total) return abc_fail_ws(L.total, ws_bytes);
     if (((uintptr_t)ws | (uintptr_t)fwd_ws) & 15) return abc_fail_invalid("distill_bwd: workspaces must be 16-byte aligned");
     if (!dq && !dp && !d_temp) return ABC_OK;
     hipStream_t st = (hipStream_t)stream;
     const char* f = (const char*)fwd_ws;
     char* w = (char*)ws;
-    GradArgs a;
-    a.s = (const float*)f; a.lds = F.lds; a.lse = (const float*)(f + F.off_lse); a.t = (const float*)(f + F.off_t); a.idx = teacher_idx;
-    a.has = (const float*)(f + F.off_row) + 2 * B; a.stat = (const float*)(f + F.off_stat); a.temp = temp; a.grad_out = grad_out;
-    a.T = T; a.ldg = L.ldg; a.k = k; a.g = (float*)(w + L.off_g); a.dt = (float*)(w + L.off_dt);
-    hipLaunchKernelGGL(distill_grad_kernel, dim3((unsigned)L.segs, (unsigned)B), dim3(256), 0, st, a);
     const bool bf = dtype == ABC_DT_BF16;
+    const unsigned* flag = F.fast ? (const unsigned*)(f + F.off_flag) : nullptr;
+    const float* stat = (const float*)(f + F.off_stat);
+    GradArgs a;
+    a.s = (const float*)(f + F.off_s); a.lds = F.lds; a.lse = (const float*)(f + F.off_lse); a.t = (const float*)(f + F.off_t);
+    a.li = (const int*)(f + F.off_li); a.has = (const float*)(f + F.off_row) + 2 * B; a.temp = temp;
+    a.B = B; a.T = T; a.ldg = L.ldg; a.k = k; a.form = bf ? G_BF16 : F.fast ? G_F16 : G_F32; a.flag = flag;
+    a.g = w + L.off_g; a.dt = (float*)(w + L.off_dt);
+    hipLaunchKernelGGL(distill_grad_kernel, dim3((unsigned)L.segs, (unsigned)B), dim3(256), 0, st, a);
     SumArgs sa = {};
-    if (dq) {
-        const Side ga{a.g, a.g, B, L.ldg, B}, cb{p, memory, C, d, d};
-        // the candidates' K-strided side ends at T rows; g's columns from T on are zero and multiply zeros
-        GemmArgs g = gemm_args(ga, cb, T, L.q, L.q.splits > 1 ? (void*)(w + L.off_pq) : dq, d, B * d);
-        if (!bf) {
-            if (L.q.tile == 128) launch_tile<LoadKC<false, 3, 128, 1>, LoadKS<false, 3, 128, 1>, 3, 3, 3, 128, 1, false>(g, st);
-            else launch_tile<LoadKC<false, 3, 64, 1>, LoadKS<false, 3, 64, 1>, 3, 3, 3, 64, 1, false>(g, st);
-        } else if (L.q.splits > 1) {
-            if (L.q.tile == 128) launch_tile<LoadKC<false, 2, 128, 1>, LoadKS<true, 1, 128, 1>, 2, 1, 2, 128, 1, false>(g, st);
-            else launch_tile<LoadKC<false, 2, 64, 1>, LoadKS<true, 1, 64, 1>, 2, 1, 2, 64, 1, false>(g, st);
-        } else {
-            if (L.q.tile == 128) launch_tile<LoadKC<false, 2, 128, 1>, LoadKS<true, 1, 128, 1>, 2, 1, 2, 128, 1, true>(g, st);
-            else launch_tile<LoadKC<false, 2, 64, 1>, LoadKS<true, 1, 64, 1>, 2, 1, 2, 64, 1, true>(g, st);
-        }
-        if (L.q.splits > 1) { sa.part[0] = (const float*)(w + L.off_pq); sa.out[0] = dq; sa.n[0] = B * d; sa.splits[0] = L.q.splits; }
-    }
-    if (dp) {
-        const Side ga{a.g, a.g, B, L.ldg, C}, qb{q, q, B, d, d};
-        GemmArgs g = gemm_args(ga, qb, B, L.p, L.p.splits > 1 ? (void*)(w + L.off_pp) : dp, d, C * d);
-        if (!bf) {
-            if (L.p.tile == 128) launch_tile<LoadKS<false, 3, 128, 1>, LoadKS<false, 3, 128, 1>, 3, 3, 3, 128, 1, false>(g, st);
-            else launch_tile<LoadKS<false, 3, 64, 1>, LoadKS<false, 3, 64, 1>, 3, 3, 3, 64, 1, false>(g, st);
-        } else if (L.p.splits > 1) {
-            if (L.p.tile == 128) launch_tile<LoadKS<false, 2, 128, 1>, LoadKS<true, 1, 128, 1>, 2, 1, 2, 128, 1, false>(g, st);
-            else launch_tile<LoadKS<false, 2, 64, 1>, LoadKS<true, 1, 64, 1>, 2, 1, 2, 64, 1, false>(g, st);
-        } else {
-            if (L.p.tile == 128) launch_tile<LoadKS<false, 2, 128, 1>, LoadKS<true, 1, 128, 1>, 2, 1, 2, 128, 1, true>(g, st);
-            else launch_tile<LoadKS<false, 2, 64, 1>, LoadKS<true, 1, 64, 1>, 2, 1, 2, 64, 1, true>(g, st);
-        }
-        if (L.p.splits > 1) { sa.part[1] = (const float*)(w + L.off_pp); sa.out[1] = dp; sa.n[1] = C * d; sa.splits[1] = L.p.splits; }
+    if (dq || dp) {
+        const Side gq{a.g, a.g, B, L.ldg, B, B * L.ldg * 2}, gp{a.g, a.g, B, L.ldg, C, B * L.ldg * 2};
+        const Side cand{p, memory, C, d, d, 0}, query{q, q, B, d, d, 0};
+        GemmArgs xq = gemm_args(gq, cand, T, L.q, L.q.splits > 1 ? (void*)(w + L.off_pq) : dq, d, B * d);
+        GemmArgs xp = gemm_args(gp, query, B, L.p, L.p.splits > 1 ? (void*)(w + L.off_pp) : dp, d, C * d);
+        for (GemmArgs* x : {&xq, &xp}) { x->f0 = grad_out; x->f1 = stat; x->f2 = temp; }
+        if (bf) {
+            if (L.q.tile == 128) launch_grads<GradQB128, GradPB128>(xq, xp, dq, dp, nullptr, 0, st);
+            else launch_grads<GradQB64, GradPB64>(xq, xp, dq, dp, nullptr, 0, st);
+        } else if (F.fast) {
+            GemmArgs hq = xq, hp = xp;
+            hq.scale = hp.scale = 1.0f / G_SCALE;
+            hp.b = Side{f + F.off_q, f + F.off_q, B, d, d, B * d * 2};
+            launch_grads<GradQH128, GradPH128>(hq, hp, dq, dp, flag, 0, st);
+            launch_grads<GradQF128, GradPF128>(xq, xp, dq, dp, flag, 1, st);
+        } else if (L.q.tile == 128) launch_grads<GradQF128, GradPF128>(xq, xp, dq, dp, nullptr, 0, st);
+        else launch_grads<GradQF64, GradPF64>(xq, xp, dq, dp, nullptr, 0, st);
+        if (dq && L.q.splits > 1) { sa.part[0] = (const float*)(w + L.off_pq); sa.out[0] = dq; sa.n[0] = B * d; sa.splits[0] = L.q.splits; }
+        if (dp && L.p.splits > 1) { sa.part[1] = (const float*)(w + L.off_pp); sa.out[1] = dp; sa.n[1] = C * d; sa.splits[1] = L.p.splits; }
     }
     if (sa.n[0] || sa.n[1] || d_temp) {
         sa.blocks0 = (int)((sa.n[0] + 1023) / 1024);
         const int blocks1 = (int)((sa.n[1] + 1023) / 1024);
-        sa.dt = a.dt; sa.ndt = B * L.segs; sa.temp = temp; sa.d_temp = d_temp;
+        sa.dt = a.dt; sa.ndt = B * L.segs; sa.f0 = grad_out; sa.f1 = stat; sa.f2 = temp; sa.d_temp = d_temp;
         if (bf) hipLaunchKernelGGL(distill_sum_kernel<true>, dim3(sa.blocks0 + blocks1 + 1), dim3(256), 0, st, sa);
         else hipLaunchKernelGGL(distill_sum_kernel<false>, dim3(sa.blocks0 + blocks1 + 1), dim3(256), 0, st, sa);
     }
