@@ -87,61 +87,67 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[2]) {
     w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{ra, rb}, v2h));
 }
 
-// A tile side in LDS: [part][k block of 32][row][32 k], 64 bytes a row, its four 16-byte chunks permuted with the row so
-// that neither the fragments' reads (8 neighbouring rows, one chunk) nor the writes of turned columns (every second row) meet in a bank.
+// A tile side in LDS: [part][k block of 32][row][32 k], 64 bytes a row, four 16-byte chunks permuted with the row.  A 16-byte access of
+// a wave goes in phases of 16 lanes, {0-3, 12-15, 20-27} and {4-11, 16-19, 28-31} and the same of the upper half; a phase of a fragment's
+// read holds rows r, r + 12 of one chunk and r + 4, r + 8 of the next, and with -(row / 4) mod 4 those four never share a bank.
 template <int R, int NKB>
 __device__ __forceinline__ int lds_at(int part, int row, int chunk) {
-    return (((part * NKB + (chunk >> 2)) * R + row) << 6) + (((chunk & 3) ^ ((row >> 1) & 3) ^ ((row >> 3) & 3)) << 4);
+    return (((part * NKB + (chunk >> 2)) * R + row) << 6) + (((chunk ^ (0 - (row >> 2))) & 3) << 4);
 }
 
-// KC: a thread holds chunks of 8 values along k of one row, DEPTH stages of them.  Storage goes on to a multiple of 8 values with zeros.
+// The loaders hold DEPTH stages of a side's values in registers (load), and put them into LDS, turned and split into parts as the
+// matrix instructions take them, in UNITS steps (store).  Rows past the end are the last row again: their results are not kept.
+// TAIL: the stage may reach past k1, where the values are zero.
+
+// KC: a thread holds chunks of 8 values along k of one row.  Storage goes on to a multiple of 8 values with zeros.
 // RANGE: keeps the largest magnitude of what it reads.
 template <int NUM, int PARTS, int R, int NKB, int DEPTH, bool RANGE = false>
 struct LoadKC {
-    static constexpr int ES = bytes_of(NUM), CH = NKB * 4, N = R * CH / 256, Q = NUM == RAW ? PARTS : 2;
+    static constexpr int ES = bytes_of(NUM), N = R / 64, Q = NUM == RAW ? PARTS : 2, UNITS = N * NKB;
     const char* at[N];
-    v4u w[DEPTH][N][Q];
+    v4u w[DEPTH][NKB][N][Q];
     float top[RANGE ? N : 1];
     int row0, chunk;
+    static __host__ __device__ constexpr int tile_index(int lds_row) { return lds_row; }
     __device__ __forceinline__ void init(const Side& s, int64_t r0, int tid) {
-        chunk = tid % CH;
-        row0 = tid / CH;
+        chunk = tid & 3;
+        row0 = tid >> 2;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int64_t r = r0 + row0 + i * (256 / CH);
-            at[i] = r < s.rows ? storage_row<ES>(s, r) : nullptr;
+            const int64_t r = r0 + row0 + i * 64;
+            at[i] = storage_row<ES>(s, r < s.rows ? r : s.rows - 1) + chunk * 8 * ES;
             if constexpr (RANGE) top[i] = 0.f;
         }
     }
+    template <bool TAIL>
     __device__ __forceinline__ void load(int d, const Side& s, int64_t k0, int64_t k1) {
-        const int64_t k = k0 + chunk * 8;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+        for (int b = 0; b < NKB; ++b)
 #pragma unroll
-            for (int p = 0; p < Q; ++p) {
-                if (at[i] && k < k1) w[d][i][p] = *(const v4u*)(at[i] + (NUM == RAW ? p * s.plane : p * 16) + k * ES);
-                else w[d][i][p] = v4u{0, 0, 0, 0};
-            }
-    }
-    __device__ __forceinline__ void store(int d, char* lds) {
+            for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int row = row0 + i * (256 / CH);
-            if constexpr (NUM == RAW) {
-#pragma unroll
-                for (int p = 0; p < PARTS; ++p) *(v4u*)(lds + lds_at<R, NKB>(p, row, chunk)) = w[d][i][p];
-            } else {
-                uint32_t o[4][PARTS];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float a = __uint_as_float(w[d][i][j >> 1][(2 * j) & 3]), b = __uint_as_float(w[d][i][j >> 1][(2 * j + 1) & 3]);
-                    split_pair(a, b, o[j]);
-                    if constexpr (RANGE) top[i] = fmaxf(fmaxf(fabsf(a), fabsf(b)), top[i]);
+                for (int p = 0; p < Q; ++p) {
+                    if (!TAIL || k0 + b * 32 + chunk * 8 < k1)
+                        w[d][b][i][p] = *(const v4u*)(at[i] + (NUM == RAW ? p * s.plane : p * 16) + (k0 + b * 32) * ES);
+                    else w[d][b][i][p] = v4u{0, 0, 0, 0};
                 }
+    }
+    __device__ __forceinline__ void store(int d, int unit, char* lds) {
+        const int b = unit / N, i = unit % N, row = row0 + i * 64;
+        if constexpr (NUM == RAW) {
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p)
-                    *(v4u*)(lds + lds_at<R, NKB>(p, row, chunk)) = v4u{o[0][p], o[1][p], o[2][p], o[3][p]};
+            for (int p = 0; p < PARTS; ++p) *(v4u*)(lds + lds_at<R, NKB>(p, row, b * 4 + chunk)) = w[d][b][i][p];
+        } else {
+            uint32_t o[4][PARTS];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x = __uint_as_float(w[d][b][i][j >> 1][(2 * j) & 3]), y = __uint_as_float(w[d][b][i][j >> 1][(2 * j + 1) & 3]);
+                split_pair(x, y, o[j]);
+                if constexpr (RANGE) top[i] = fmaxf(fmaxf(fabsf(x), fabsf(y)), top[i]);
             }
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                *(v4u*)(lds + lds_at<R, NKB>(p, row, b * 4 + chunk)) = v4u{o[0][p], o[1][p], o[2][p], o[3][p]};
         }
     }
     // whether a row that this thread has a part in does not fit the fp16 parts
@@ -151,8 +157,8 @@ struct LoadKC {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 float v = top[i];
-#pragma unroll
-                for (int m = 1; m < CH; m <<= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
+                v = fmaxf(v, __shfl_xor(v, 1, 64));
+                v = fmaxf(v, __shfl_xor(v, 2, 64));
                 bad |= v > 0.f && !(v >= H_MIN && v <= H_LOW);
             }
         return bad;
@@ -160,35 +166,39 @@ struct LoadKC {
 };
 
 // KS: a thread holds 8 storage rows (k) of two neighbouring columns (one, where a narrow fp32 tile has too few) and turns them round
-// in its registers.  `rows` is even or storage goes on past it.
+// in its registers.  `rows` is even or storage goes on past it.  Columns 2x and 2x + 1 of 32 lie in LDS rows x and 16 + x, so that a
+// wave's writes go to neighbouring rows, and a lane's accumulators of two neighbouring blocks are neighbours in memory again.
 template <int NUM, int PARTS, int R, int NKB, int DEPTH>
 struct LoadKS {
     static constexpr int ES = bytes_of(NUM), COLS = NUM != RAW && R * NKB * 2 < 256 ? 1 : 2, CG = R / COLS, N = CG * NKB * 4 / 256;
-    static constexpr int Q = NUM == RAW ? PARTS : 1;
+    static constexpr int Q = NUM == RAW ? PARTS : 1, UNITS = N * COLS;
     static_assert(N >= 1, "a tile too narrow for 256 threads");
     typedef typename std::conditional<NUM == RAW, uint32_t, typename std::conditional<COLS == 2, v2f, float>::type>::type piece_t;
     piece_t w[DEPTH][N][Q][8];
-    int64_t col;
-    int cg, chunk0;
-    bool ok;
+    int64_t off;
+    int row, chunk0;
+    static __host__ __device__ constexpr int tile_index(int r) { return COLS == 1 ? r : (r & ~31) + ((r & 15) << 1) + ((r >> 4) & 1); }
     __device__ __forceinline__ void init(const Side& s, int64_t r0, int tid) {
-        cg = tid % CG;
+        const int cg = tid % CG;
         chunk0 = CG >= 64 ? __builtin_amdgcn_readfirstlane(tid / CG) : tid / CG;   // a wave's storage rows are scalar then
-        col = r0 + cg * COLS;
-        ok = col < s.rows;
+        row = COLS == 1 ? cg : (cg >> 4) * 32 + (cg & 15);
+        const int64_t last = COLS == 1 ? s.rows - 1 : (s.rows - 1) & ~(int64_t)1, col = r0 + cg * COLS;
+        off = (col < last ? col : last) * ES;
     }
+    template <bool TAIL>
     __device__ __forceinline__ void load(int d, const Side& s, int64_t k0, int64_t k1) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int64_t k = k0 + (chunk0 + i * (256 / CG)) * 8;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const bool in = ok && k + j < k1;
-                const char* src = in ? storage_row<ES>(s, k + j) + col * ES : nullptr;
+                if (!TAIL || k + j < k1) {
+                    const char* src = storage_row<ES>(s, k + j) + off;
 #pragma unroll
-                for (int p = 0; p < Q; ++p) {
-                    if (in) w[d][i][p][j] = *(const piece_t*)(src + p * s.plane);
-                    else w[d][i][p][j] = piece_t{};
+                    for (int p = 0; p < Q; ++p) w[d][i][p][j] = *(const piece_t*)(src + p * s.plane);
+                } else {
+#pragma unroll
+                    for (int p = 0; p < Q; ++p) w[d][i][p][j] = piece_t{};
                 }
             }
         }
@@ -197,26 +207,19 @@ struct LoadKS {
         if constexpr (COLS == 2 && NUM != RAW) return x[c];
         else return (float)x;
     }
-    __device__ __forceinline__ void store(int d, char* lds) {
+    __device__ __forceinline__ void store(int d, int unit, char* lds) {
+        const int i = unit / COLS, c = unit % COLS, chunk = chunk0 + i * (256 / CG);
+        uint32_t o[4][PARTS];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int chunk = chunk0 + i * (256 / CG);
-#pragma unroll
-            for (int c = 0; c < COLS; ++c) {
-                uint32_t o[4][PARTS];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if constexpr (NUM == RAW) {
-#pragma unroll
-                        for (int p = 0; p < PARTS; ++p)
-                            o[j][p] = __builtin_amdgcn_perm(w[d][i][p][2 * j + 1], w[d][i][p][2 * j], c ? 0x07060302u : 0x05040100u);
-                    } else split_pair(value(w[d][i][0][2 * j], c), value(w[d][i][0][2 * j + 1], c), o[j]);
-                }
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (NUM == RAW) {
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p)
-                    *(v4u*)(lds + lds_at<R, NKB>(p, cg * COLS + c, chunk)) = v4u{o[0][p], o[1][p], o[2][p], o[3][p]};
-            }
+                    o[j][p] = __builtin_amdgcn_perm(w[d][i][p][2 * j + 1], w[d][i][p][2 * j], c ? 0x07060302u : 0x05040100u);
+            } else split_pair(value(w[d][i][0][2 * j], c), value(w[d][i][0][2 * j + 1], c), o[j]);
         }
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) *(v4u*)(lds + lds_at<R, NKB>(p, row + c * 16, chunk)) = v4u{o[0][p], o[1][p], o[2][p], o[3][p]};
     }
     __device__ __forceinline__ bool outside() { return false; }
 };
@@ -236,8 +239,9 @@ struct GemmArgs {
 __device__ __forceinline__ float factor_of(const float* f0, const float* f1, const float* f2) { return __fdiv_rn(f0[0] * f1[0], f2[0]); }
 
 // out[m][n] = sum_k A(m, k) B(n, k): tiles of TM x TN, four waves as 2 x 2, 16x16x32 MFMAs over every pair of parts whose indices add up
-// to less than KEEP.  The next DEPTH stages' values are on their way in registers while one is multiplied out of LDS (LBUF buffers of
-// it: two need one barrier a stage), and two or more workgroups a CU fill each other's waits.
+// to less than KEEP.  While a stage is multiplied out of one LDS buffer, the next one's values go from registers into the other, a
+// step of it after each row of MFMAs (the vector unit works in their shadow), and the loads of DEPTH stages further on are on their
+// way: one barrier a stage, which waits for LDS alone.  LBUF 1: one buffer and two barriers, where two would leave a CU one workgroup.
 template <class LA_, class LB_, int PA_, int PB_, int KEEP_, int TM_, int TN_, int NKB_, int DEPTH_, int LBUF_, bool F16_, bool OUT_BF16_>
 struct Cfg {
     typedef LA_ LA;
@@ -247,15 +251,20 @@ struct Cfg {
     static constexpr int LDS = LBUF * (PA * TM + PB * TN) * NKB * 64;
 };
 
+// every wave's LDS accesses are done, and its loads from memory still on their way
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 template <class C>
 __device__ __forceinline__ bool gemm_tile(const GemmArgs& g, int item, char* smem) {
     constexpr int WM = C::TM / 32, WN = C::TN / 32, STAGE = C::NKB * 32;    // 16 x 16 blocks a wave holds along m and n
     constexpr bool TWO = C::KEEP > 1;
     constexpr int BUF = C::LDS / C::LBUF, LB0 = C::PA * C::NKB * C::TM * 64;
+    constexpr int UA = C::LA::UNITS, UNITS = UA + C::LB::UNITS, STEPS = C::NKB * WM;
     typedef typename std::conditional<C::F16, v8h, v8bf>::type frag_t;
     const int per = g.nm * g.splits, tn = item / per, inner = item % per;
     const int tm = inner % g.nm, sp = inner / g.nm;
     const int64_t k0 = sp * g.kstep, k1 = min(g.k, k0 + g.kstep);
+    const int ns = k1 > k0 ? (int)((k1 - k0 + STAGE - 1) / STAGE) : 0, nfull = k1 > k0 ? (int)((k1 - k0) / STAGE) : 0;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int l15 = lane & 15, h = lane >> 4;
     const int wm = wave & 1, wn = wave >> 1;
@@ -271,26 +280,42 @@ __device__ __forceinline__ bool gemm_tile(const GemmArgs& g, int item, char* sme
             acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
             if constexpr (TWO) low[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
         }
+    auto fetch = [&](int d, int st) {
+        const int64_t k = k0 + (int64_t)st * STAGE;
+        if (st < nfull) {
+            A.template load<false>(d, g.a, k, k1);
+            B.template load<false>(d, g.b, k, k1);
+        } else if (st < ns) {
+            A.template load<true>(d, g.a, k, k1);
+            B.template load<true>(d, g.b, k, k1);
+        }
+    };
+    auto store = [&](int d, int u0, int u1, char* to) {
 #pragma unroll
-    for (int d = 0; d < C::DEPTH; ++d) {
-        A.load(d, g.a, k0 + d * STAGE, k1);
-        B.load(d, g.b, k0 + d * STAGE, k1);
+        for (int u = 0; u < UNITS; ++u)
+            if (u >= u0 && u < u1) {
+                if (u < UA) A.store(d, u, to);
+                else B.store(d, u - UA, to + LB0);
+            }
+    };
+#pragma unroll
+    for (int d = 0; d < C::DEPTH; ++d) fetch(d, d);
+    if (C::LBUF == 2 && ns) {
+        store(0, 0, UNITS, smem);
+        fetch(0, C::DEPTH);
     }
-    int buf = 0;
-    for (int64_t kb0 = k0; kb0 < k1; kb0 += STAGE * C::DEPTH) {
+    for (int s0 = 0; s0 < ns; s0 += C::DEPTH) {
 #pragma unroll
         for (int d = 0; d < C::DEPTH; ++d) {
-            const int64_t k = kb0 + d * STAGE;
-            if (k >= k1) break;
-            char* la = smem + buf * BUF;
-            char* lb = la + LB0;
-            A.store(d, la);
-            B.store(d, lb);
-            __syncthreads();
-            if (k + C::DEPTH * STAGE < k1) {
-                A.load(d, g.a, k + C::DEPTH * STAGE, k1);
-                B.load(d, g.b, k + C::DEPTH * STAGE, k1);
-            }
+            const int st = s0 + d, next = (d + 1) % C::DEPTH;
+            if (st >= ns) break;
+            char* la = smem + (C::LBUF == 2 ? (st & 1) * BUF : 0);
+            char* other = smem + (C::LBUF == 2 ? (~st & 1) * BUF : 0);
+            if constexpr (C::LBUF == 1) {
+                store(d, 0, UNITS, la);
+                lds_barrier();
+                fetch(d, st + C::DEPTH);
+            } else lds_barrier();
 #pragma unroll
             for (int kb = 0; kb < C::NKB; ++kb) {
                 frag_t fb[WN][C::PB];
@@ -298,7 +323,7 @@ __device__ __forceinline__ bool gemm_tile(const GemmArgs& g, int item, char* sme
                 for (int j = 0; j < WN; ++j)
 #pragma unroll
                     for (int p = 0; p < C::PB; ++p)
-                        fb[j][p] = *(const frag_t*)(lb + lds_at<C::TN, C::NKB>(p, (wn * WN + j) * 16 + l15, kb * 4 + h));
+                        fb[j][p] = *(const frag_t*)(la + LB0 + lds_at<C::TN, C::NKB>(p, (wn * WN + j) * 16 + l15, kb * 4 + h));
 #pragma unroll
                 for (int i = 0; i < WM; ++i) {
                     frag_t fa[C::PA];
@@ -316,27 +341,40 @@ __device__ __forceinline__ bool gemm_tile(const GemmArgs& g, int item, char* sme
                                     if constexpr (C::F16) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[pa], fb[j][pb], c, 0, 0, 0);
                                     else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[pa], fb[j][pb], c, 0, 0, 0);
                                 }
+                    if constexpr (C::LBUF == 2) {                // (past the last stage: into a buffer that nothing reads)
+                        const int step = kb * WM + i;
+                        store(next, step * UNITS / STEPS, (step + 1) * UNITS / STEPS, other);
+                    }
                 }
             }
-            if constexpr (C::LBUF == 1) __syncthreads();
-            else buf ^= 1;
+            if constexpr (C::LBUF == 1) lds_barrier();
+            else fetch(next, st + 1 + C::DEPTH);
         }
     }
     const float f = g.scale * (g.splits == 1 && g.f0 ? factor_of(g.f0, g.f1, g.f2) : 1.f);
+    constexpr bool PAIR = C::LB::tile_index(16) == 1;            // a lane's blocks j and j + 1 hold neighbouring columns
 #pragma unroll
     for (int i = 0; i < WM; ++i)
 #pragma unroll
-        for (int j = 0; j < WN; ++j) {
-            const int64_t n = (int64_t)tn * C::TN + (wn * WN + j) * 16 + l15;
+        for (int j = 0; j < WN; j += PAIR ? 2 : 1) {
+            const int64_t n = (int64_t)tn * C::TN + C::LB::tile_index((wn * WN + j) * 16 + l15);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int64_t m = (int64_t)tm * C::TM + (wm * WM + i) * 16 + 4 * h + r;
-                float v = acc[i][j][r];
-                if constexpr (TWO) v = C::F16 ? fmaf(low[i][j][r], 0x1p-11f, v) : v + low[i][j][r];
-                v *= f;
-                if (m < g.a.rows && n < g.b.rows) {
-                    if (C::OUT_BF16 && g.splits == 1) ((uint16_t*)g.out)[m * g.ldo + n] = (uint16_t)f32_to_bf16_bits(v);
-                    else ((float*)g.out)[sp * g.slab + m * g.ldo + n] = v;
+                const int64_t m = (int64_t)tm * C::TM + C::LA::tile_index((wm * WM + i) * 16 + 4 * h + r);
+                float v[PAIR ? 2 : 1];
+#pragma unroll
+                for (int c = 0; c < (PAIR ? 2 : 1); ++c) {
+                    v[c] = acc[i][j + c][r];
+                    if constexpr (TWO) v[c] = C::F16 ? fmaf(low[i][j + c][r], 0x1p-11f, v[c]) : v[c] + low[i][j + c][r];
+                    v[c] *= f;
+                }
+                if (m >= g.a.rows || n >= g.b.rows) continue;
+                if constexpr (PAIR) {                            // b.rows (d) is even
+                    if (C::OUT_BF16 && g.splits == 1) *(uint32_t*)((uint16_t*)g.out + m * g.ldo + n) = f32_to_bf16_bits(v[0]) | f32_to_bf16_bits(v[1]) << 16;
+                    else *(v2f*)((float*)g.out + sp * g.slab + m * g.ldo + n) = v2f{v[0], v[1]};
+                } else {
+                    if (C::OUT_BF16 && g.splits == 1) ((uint16_t*)g.out)[m * g.ldo + n] = (uint16_t)f32_to_bf16_bits(v[0]);
+                    else ((float*)g.out)[sp * g.slab + m * g.ldo + n] = v[0];
                 }
             }
         }
@@ -422,7 +460,7 @@ struct RowArgs {
     int* li;                         // [B][k]: the column, -1 = nothing
     float* row;                      // [B] row losses, then [B] agreement, then [B] 1 where the row has an entry
     float* stat;                     // [0]: 1 / rows that have an entry
-    unsigned* cnt;                   // [B] segments that have arrived, [1] rows
+    unsigned* cnt;                   // [B] segments that have arrived, [1] groups of 32 rows, [groups] their rows
     float* out_loss;
     float* out_agree;
 };
@@ -627,7 +665,11 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
         put(a.row + a.B + b, some && bad == 0.f && am == li[first] ? 1.f : 0.f);
         put(a.row + 2 * a.B + b, some ? 1.f : 0.f);
     }
-    if (!arrive_last(a.cnt + a.B, (unsigned)a.B, &last)) return;
+    // 32 rows arrive on a counter of theirs, the last of them on the common one (arrivals on one word follow each other some 40 ns apart)
+    const int64_t group = b / 32, groups = (a.B + 31) / 32;
+    if (!arrive_last(a.cnt + a.B + 1 + group, (unsigned)min((int64_t)32, a.B - group * 32), &last)) return;
+    __syncthreads();
+    if (!arrive_last(a.cnt + a.B, (unsigned)groups, &last)) return;
     // ---- the last row: the means
     float ls = 0.f, hs = 0.f;
     int ns = 0;
@@ -813,7 +855,7 @@ static FwdLayout fwd_layout(int dtype, int64_t B, int64_t T, int d, int k) {
     L.off_li = o; o += up((size_t)B * k * 4);
     L.off_row = o; o += up((size_t)B * 12);
     L.off_stat = o; o += 256;
-    L.off_cnt = o; o += up((size_t)(B + 1) * 4);
+    L.off_cnt = o; o += up((size_t)(B + 1 + (B + 31) / 32) * 4);
     L.off_q = o; o += L.fast ? up((size_t)B * d * 4) : 0;
     L.off_qout = o; o += L.fast ? up((size_t)B * 4) : 0;
     L.off_flag = o; o += 256;
@@ -898,17 +940,17 @@ static void launch_grads(const GemmArgs& gq, const GemmArgs& gp, bool dq, bool d
 typedef Cfg<LoadKC<RAW, 1, 128, 2, 1>, LoadKC<RAW, 1, 128, 2, 1>, 1, 1, 1, 128, 128, 2, 1, 2, false, false> ScoresB128;
 typedef Cfg<LoadKC<RAW, 1, 64, 2, 2>, LoadKC<RAW, 1, 64, 2, 2>, 1, 1, 1, 64, 64, 2, 2, 2, false, false> ScoresB64;
 typedef Cfg<LoadKC<SPLIT_B3, 3, 128, 1, 1>, LoadKC<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, false, false> ScoresF128;
-typedef Cfg<LoadKC<SPLIT_B3, 3, 64, 1, 3>, LoadKC<SPLIT_B3, 3, 64, 1, 3>, 3, 3, 3, 64, 64, 1, 3, 1, false, false> ScoresF64;
+typedef Cfg<LoadKC<SPLIT_B3, 3, 64, 1, 3>, LoadKC<SPLIT_B3, 3, 64, 1, 3>, 3, 3, 3, 64, 64, 1, 3, 2, false, false> ScoresF64;
 typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKC<SPLIT_H2, 2, 128, 1, 1, true>, 2, 2, 2, 128, 128, 1, 1, 2, true, false> ScoresH128;
 // dq = g cand, dc = g^T q
-typedef Cfg<LoadKC<RAW, 2, 128, 2, 1>, LoadKS<RAW, 1, 128, 2, 1>, 2, 1, 2, 128, 128, 2, 1, 1, false, true> GradQB128;
-typedef Cfg<LoadKS<RAW, 2, 128, 2, 1>, LoadKS<RAW, 1, 128, 2, 1>, 2, 1, 2, 128, 128, 2, 1, 1, false, true> GradPB128;
-typedef Cfg<LoadKC<RAW, 2, 64, 2, 2>, LoadKS<RAW, 1, 64, 2, 2>, 2, 1, 2, 64, 64, 2, 2, 1, false, true> GradQB64;
-typedef Cfg<LoadKS<RAW, 2, 64, 2, 2>, LoadKS<RAW, 1, 64, 2, 2>, 2, 1, 2, 64, 64, 2, 2, 1, false, true> GradPB64;
+typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKS<RAW, 1, 128, 1, 1>, 2, 1, 2, 128, 128, 1, 1, 2, false, true> GradQB128;
+typedef Cfg<LoadKS<RAW, 2, 128, 1, 1>, LoadKS<RAW, 1, 128, 1, 1>, 2, 1, 2, 128, 128, 1, 1, 2, false, true> GradPB128;
+typedef Cfg<LoadKC<RAW, 2, 64, 2, 2>, LoadKS<RAW, 1, 64, 2, 2>, 2, 1, 2, 64, 64, 2, 2, 2, false, true> GradQB64;
+typedef Cfg<LoadKS<RAW, 2, 64, 2, 2>, LoadKS<RAW, 1, 64, 2, 2>, 2, 1, 2, 64, 64, 2, 2, 2, false, true> GradPB64;
 typedef Cfg<LoadKC<SPLIT_B3, 3, 128, 1, 1>, LoadKS<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, false, false> GradQF128;
 typedef Cfg<LoadKS<SPLIT_B3, 3, 128, 1, 1>, LoadKS<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, false, false> GradPF128;
-typedef Cfg<LoadKC<SPLIT_B3, 3, 64, 1, 2>, LoadKS<SPLIT_B3, 3, 64, 1, 2>, 3, 3, 3, 64, 64, 1, 2, 1, false, false> GradQF64;
-typedef Cfg<LoadKS<SPLIT_B3, 3, 64, 1, 2>, LoadKS<SPLIT_B3, 3, 64, 1, 2>, 3, 3, 3, 64, 64, 1, 2, 1, false, false> GradPF64;
+typedef Cfg<LoadKC<SPLIT_B3, 3, 64, 1, 2>, LoadKS<SPLIT_B3, 3, 64, 1, 2>, 3, 3, 3, 64, 64, 1, 2, 2, false, false> GradQF64;
+typedef Cfg<LoadKS<SPLIT_B3, 3, 64, 1, 2>, LoadKS<SPLIT_B3, 3, 64, 1, 2>, 3, 3, 3, 64, 64, 1, 2, 2, false, false> GradPF64;
 typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKS<SPLIT_H2, 2, 128, 1, 1>, 2, 2, 2, 128, 128, 1, 1, 2, true, false> GradQH128;
 typedef Cfg<LoadKS<RAW, 2, 128, 1, 1>, LoadKS<RAW, 2, 128, 1, 1>, 2, 2, 2, 128, 128, 1, 1, 2, true, false> GradPH128;
 
@@ -928,7 +970,7 @@ extern "C" int abc_distill_fwd(int dtype, const void* q, const void* p, const vo
     char* w = (char*)ws;
     unsigned* cnt = (unsigned*)(w + L.off_cnt);
     unsigned* flag = (unsigned*)(w + L.off_flag);
-    const int nc = (int)B + 1;
+    const int nc = (int)(B + 1 + (B + 31) / 32);
     const Side sq{q, q, B, d, B, 0}, sc{p, memory, C, d, T, 0};
     const GemmArgs g = gemm_args(sq, sc, d, L.s, w, L.lds, B * L.lds);
     if (dtype == ABC_DT_BF16) {
