@@ -57,8 +57,10 @@ struct Side {
     int64_t n0;                      // storage rows in p0
     int64_t ld;                      // elements between storage rows
     int64_t rows;                    // rows of the product on this side
-    int64_t plane;                   // bytes from one part of the values to the next, where they lie split
 };
+// Values that lie split into two 16-bit parts: blocks of 32 along the row, 64 bytes of the leading parts and then 64 of the others, so that
+// a stage's values of a row are one cache line.  ld counts 16-bit elements (two a value).
+__device__ __forceinline__ int64_t split_at(int64_t k) { return (k >> 5) * 128 + (k & 31) * 2; }
 
 // how the values become the 16-bit parts that are multiplied
 enum { RAW, SPLIT_B3, SPLIT_H2 };    // as they lie; fp32 -> three bf16; fp32 -> two fp16
@@ -99,56 +101,65 @@ __device__ __forceinline__ int lds_at(int part, int row, int chunk) {
 // matrix instructions take them, in UNITS steps (store).  Rows past the end are the last row again: their results are not kept.
 // TAIL: the stage may reach past k1, where the values are zero.
 
-// KC: a thread holds chunks of 8 values along k of one row.  Storage goes on to a multiple of 8 values with zeros.
-// RANGE: keeps the largest magnitude of what it reads.
+// KC: the lanes of a wave read whole 128-byte lines: 16 bytes of a row each, 8 (parts: 4 and 4) neighbouring lanes a row's stage.
+// Storage goes on to a multiple of 8 values (parts: 32) with zeros.  RANGE: keeps the largest magnitude of what it reads.
 template <int NUM, int PARTS, int R, int NKB, int DEPTH, bool RANGE = false>
 struct LoadKC {
-    static constexpr int ES = bytes_of(NUM), N = R / 64, Q = NUM == RAW ? PARTS : 2, UNITS = N * NKB;
+    static constexpr int ES = bytes_of(NUM), LANES = NUM == RAW ? 4 : 8, N = R * LANES / 256, Q = NUM == RAW ? PARTS : 1, UNITS = N * NKB;
     const char* at[N];
     v4u w[DEPTH][NKB][N][Q];
     float top[RANGE ? N : 1];
-    int row0, chunk;
+    int row0, sub;
     static __host__ __device__ constexpr int tile_index(int lds_row) { return lds_row; }
     __device__ __forceinline__ void init(const Side& s, int64_t r0, int tid) {
-        chunk = tid & 3;
-        row0 = tid >> 2;
+        sub = tid % LANES;
+        row0 = tid / LANES;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int64_t r = r0 + row0 + i * 64;
-            at[i] = storage_row<ES>(s, r < s.rows ? r : s.rows - 1) + chunk * 8 * ES;
+            const int64_t r = r0 + row0 + i * (256 / LANES);
+            at[i] = storage_row<ES>(s, r < s.rows ? r : s.rows - 1) + sub * 16;
             if constexpr (RANGE) top[i] = 0.f;
         }
     }
     template <bool TAIL>
     __device__ __forceinline__ void load(int d, const Side& s, int64_t k0, int64_t k1) {
+        constexpr int STEP = NUM == RAW && PARTS == 2 ? 4 : ES;   // bytes a value
 #pragma unroll
         for (int b = 0; b < NKB; ++b)
 #pragma unroll
             for (int i = 0; i < N; ++i)
 #pragma unroll
                 for (int p = 0; p < Q; ++p) {
-                    if (!TAIL || k0 + b * 32 + chunk * 8 < k1)
-                        w[d][b][i][p] = *(const v4u*)(at[i] + (NUM == RAW ? p * s.plane : p * 16) + (k0 + b * 32) * ES);
+                    if (!TAIL || k0 + b * 32 + sub * (16 / ES) < k1) w[d][b][i][p] = *(const v4u*)(at[i] + (k0 + b * 32) * STEP + p * 64);
                     else w[d][b][i][p] = v4u{0, 0, 0, 0};
                 }
     }
     __device__ __forceinline__ void store(int d, int unit, char* lds) {
-        const int b = unit / N, i = unit % N, row = row0 + i * 64;
+        const int b = unit / N, i = unit % N, row = row0 + i * (256 / LANES);
         if constexpr (NUM == RAW) {
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p) *(v4u*)(lds + lds_at<R, NKB>(p, row, b * 4 + chunk)) = w[d][b][i][p];
+            for (int p = 0; p < PARTS; ++p) *(v4u*)(lds + lds_at<R, NKB>(p, row, b * 4 + sub)) = w[d][b][i][p];
         } else {
-            uint32_t o[4][PARTS];
+            const v4u x = w[d][b][i][0];
+            uint32_t o[2][PARTS];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float x = __uint_as_float(w[d][b][i][j >> 1][(2 * j) & 3]), y = __uint_as_float(w[d][b][i][j >> 1][(2 * j + 1) & 3]);
-                split_pair(x, y, o[j]);
-                if constexpr (RANGE) top[i] = fmaxf(fmaxf(fabsf(x), fabsf(y)), top[i]);
+            for (int j = 0; j < 2; ++j) {
+                const float u = __uint_as_float(x[2 * j]), v = __uint_as_float(x[2 * j + 1]);
+                split_pair(u, v, o[j]);
+                if constexpr (RANGE) top[i] = fmaxf(fmaxf(fabsf(u), fabsf(v)), top[i]);
             }
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-                *(v4u*)(lds + lds_at<R, NKB>(p, row, b * 4 + chunk)) = v4u{o[0][p], o[1][p], o[2][p], o[3][p]};
+            for (int p = 0; p < PARTS; ++p) *(uint2*)(lds + lds_at<R, NKB>(p, row, b * 4 + (sub >> 1)) + (sub & 1) * 8) = uint2{o[0][p], o[1][p]};
         }
+    }
+    // the values of a stage, not before here: the compiler would wait for them at the top of the stage
+    __device__ __forceinline__ void pin(int d) {
+#pragma unroll
+        for (int b = 0; b < NKB; ++b)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int p = 0; p < Q; ++p) asm volatile("" : "+v"(w[d][b][i][p]));
     }
     // whether a row that this thread has a part in does not fit the fp16 parts
     __device__ __forceinline__ bool outside() {
@@ -157,8 +168,8 @@ struct LoadKC {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 float v = top[i];
-                v = fmaxf(v, __shfl_xor(v, 1, 64));
-                v = fmaxf(v, __shfl_xor(v, 2, 64));
+#pragma unroll
+                for (int m = 1; m < LANES; m <<= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
                 bad |= v > 0.f && !(v >= H_MIN && v <= H_LOW);
             }
         return bad;
@@ -183,7 +194,7 @@ struct LoadKS {
         chunk0 = CG >= 64 ? __builtin_amdgcn_readfirstlane(tid / CG) : tid / CG;   // a wave's storage rows are scalar then
         row = COLS == 1 ? cg : (cg >> 4) * 32 + (cg & 15);
         const int64_t last = COLS == 1 ? s.rows - 1 : (s.rows - 1) & ~(int64_t)1, col = r0 + cg * COLS;
-        off = (col < last ? col : last) * ES;
+        off = NUM == RAW && PARTS == 2 ? split_at(col < last ? col : last) : (col < last ? col : last) * ES;
     }
     template <bool TAIL>
     __device__ __forceinline__ void load(int d, const Side& s, int64_t k0, int64_t k1) {
@@ -195,7 +206,7 @@ struct LoadKS {
                 if (!TAIL || k + j < k1) {
                     const char* src = storage_row<ES>(s, k + j) + off;
 #pragma unroll
-                    for (int p = 0; p < Q; ++p) w[d][i][p][j] = *(const piece_t*)(src + p * s.plane);
+                    for (int p = 0; p < Q; ++p) w[d][i][p][j] = *(const piece_t*)(src + p * 64);
                 } else {
 #pragma unroll
                     for (int p = 0; p < Q; ++p) w[d][i][p][j] = piece_t{};
@@ -221,6 +232,14 @@ struct LoadKS {
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) *(v4u*)(lds + lds_at<R, NKB>(p, row + c * 16, chunk)) = v4u{o[0][p], o[1][p], o[2][p], o[3][p]};
     }
+    __device__ __forceinline__ void pin(int d) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int p = 0; p < Q; ++p)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(w[d][i][p][j]));
+    }
     __device__ __forceinline__ bool outside() { return false; }
 };
 
@@ -234,7 +253,31 @@ struct GemmArgs {
     int64_t ldo, slab;
     float scale;                     // of every sum
     const float *f0, *f1, *f2;       // splits == 1, f0 given: times f0[0] f1[0] / f2[0]
+    float* seg;                      // splits == 1, given: every wave's part of a row's statistics, [rows][segs][4] (RowArgs), z = value / f2[0]
+    int segs;
 };
+
+// reductions over the 16 lanes that hold a row of an accumulator; every lane gets the result
+template <int CTRL>
+__device__ __forceinline__ int dpp16(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xF, 0xF, true); }
+#define DPP16(x, OP) do { x = OP(x, DPP16_AS(x, 0xB1)); x = OP(x, DPP16_AS(x, 0x4E)); x = OP(x, DPP16_AS(x, 0x141)); x = OP(x, DPP16_AS(x, 0x140)); } while (0)
+__device__ __forceinline__ float add_op(float a, float b) { return a + b; }
+__device__ __forceinline__ float max16(float x) {
+#define DPP16_AS(v, c) __int_as_float(dpp16<c>(__float_as_int(v)))
+    DPP16(x, fmaxf);
+    return x;
+}
+__device__ __forceinline__ float sum16(float x) {
+    DPP16(x, add_op);
+    return x;
+#undef DPP16_AS
+}
+__device__ __forceinline__ int min16(int x) {
+#define DPP16_AS(v, c) dpp16<c>(v)
+    DPP16(x, min);
+    return x;
+#undef DPP16_AS
+}
 
 __device__ __forceinline__ float factor_of(const float* f0, const float* f1, const float* f2) { return __fdiv_rn(f0[0] * f1[0], f2[0]); }
 
@@ -242,11 +285,13 @@ __device__ __forceinline__ float factor_of(const float* f0, const float* f1, con
 // to less than KEEP.  While a stage is multiplied out of one LDS buffer, the next one's values go from registers into the other, a
 // step of it after each row of MFMAs (the vector unit works in their shadow), and the loads of DEPTH stages further on are on their
 // way: one barrier a stage, which waits for LDS alone.  LBUF 1: one buffer and two barriers, where two would leave a CU one workgroup.
-template <class LA_, class LB_, int PA_, int PB_, int KEEP_, int TM_, int TN_, int NKB_, int DEPTH_, int LBUF_, bool F16_, bool OUT_BF16_>
+// FROM: the step (row of MFMAs) of a stage from which on the next stage's values go to LDS.  The later, the longer their loads may
+// take, and the less of the conversion lies in the MFMAs' shadow.
+template <class LA_, class LB_, int PA_, int PB_, int KEEP_, int TM_, int TN_, int NKB_, int DEPTH_, int LBUF_, int FROM_, bool F16_, bool OUT_BF16_>
 struct Cfg {
     typedef LA_ LA;
     typedef LB_ LB;
-    static constexpr int PA = PA_, PB = PB_, KEEP = KEEP_, TM = TM_, TN = TN_, NKB = NKB_, DEPTH = DEPTH_, LBUF = LBUF_;
+    static constexpr int PA = PA_, PB = PB_, KEEP = KEEP_, TM = TM_, TN = TN_, NKB = NKB_, DEPTH = DEPTH_, LBUF = LBUF_, FROM = FROM_;
     static constexpr bool F16 = F16_, OUT_BF16 = OUT_BF16_;
     static constexpr int LDS = LBUF * (PA * TM + PB * TN) * NKB * 64;
 };
@@ -342,8 +387,13 @@ __device__ __forceinline__ bool gemm_tile(const GemmArgs& g, int item, char* sme
                                     else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[pa], fb[j][pb], c, 0, 0, 0);
                                 }
                     if constexpr (C::LBUF == 2) {                // (past the last stage: into a buffer that nothing reads)
-                        const int step = kb * WM + i;
-                        store(next, step * UNITS / STEPS, (step + 1) * UNITS / STEPS, other);
+                        const int step = kb * WM + i - C::FROM, steps = STEPS - C::FROM;
+                        if (C::FROM > 0 && step == 0) {
+                            __builtin_amdgcn_sched_barrier(0);
+                            A.pin(next);
+                            B.pin(next);
+                        }
+                        if (step >= 0) store(next, step * UNITS / steps, (step + 1) * UNITS / steps, other);
                     }
                 }
             }
@@ -377,6 +427,35 @@ __device__ __forceinline__ bool gemm_tile(const GemmArgs& g, int item, char* sme
                     else ((float*)g.out)[sp * g.slab + m * g.ldo + n] = v[0];
                 }
             }
+        }
+    if constexpr (!PAIR)                                         // (the scores' product)
+        if (g.seg) {
+            // the logits are written; this wave's WN * 16 columns of each row: maximum, sum of exp, first column of the maximum
+            const float inv = __fdiv_rn(1.f, g.f2[0]);
+#pragma unroll
+            for (int i = 0; i < WM; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int64_t m = (int64_t)tm * C::TM + (wm * WM + i) * 16 + 4 * h + r;
+                    float z[WN], mx = -INFINITY, se = 0.f;
+                    int am = INT32_MAX;
+#pragma unroll
+                    for (int j = 0; j < WN; ++j) {
+                        const int64_t n = (int64_t)tn * C::TN + (wn * WN + j) * 16 + l15;
+                        z[j] = acc[i][j][r];
+                        if constexpr (TWO) z[j] = C::F16 ? fmaf(low[i][j][r], 0x1p-11f, z[j]) : z[j] + low[i][j][r];
+                        z[j] = n < g.b.rows ? z[j] * f * inv : -INFINITY;
+                        if (z[j] > mx) { mx = z[j]; am = (int)n; }
+                        if (z[j] != z[j]) se = z[j];             // a NaN stays one whatever the maximum is
+                    }
+                    const float top = max16(mx);
+                    am = min16(mx == top ? am : INT32_MAX);
+                    if (top > -INFINITY)
+#pragma unroll
+                        for (int j = 0; j < WN; ++j) se += exp_neg(z[j] - top);
+                    se = sum16(se);
+                    if (l15 == 0 && m < g.a.rows) *(v4f*)(g.seg + (m * g.segs + tn * 2 + wn) * 4) = v4f{top, se, __int_as_float(am), 0.f};
+                }
         }
     const bool out_a = A.outside(), out_b = B.outside();
     return out_a || out_b;
@@ -416,20 +495,21 @@ __global__ __launch_bounds__(256, 2) void distill_grads_kernel(const GemmArgs gq
     }
 }
 
-// the queries' fp16 parts, once for all tiles of the two products that read them; rows_out[b]: row b does not fit them
-__global__ __launch_bounds__(256) void distill_split_kernel(const float* __restrict__ q, int d, int64_t n, uint16_t* __restrict__ out,
+// the queries' fp16 parts, once for all tiles of the two products that read them; rows_out[b]: row b does not fit them.  dpad: d up to 32s
+__global__ __launch_bounds__(256) void distill_split_kernel(const float* __restrict__ q, int d, int dpad, char* __restrict__ out,
                                                             unsigned* __restrict__ rows_out, unsigned* __restrict__ flag) {
     __shared__ float red[4];
     const int64_t b = blockIdx.x;
     if (b == 0 && threadIdx.x == 0) *flag = 0u;
     float top = 0.f;
-    for (int k = threadIdx.x * 4; k < d; k += 1024) {
-        const v4f x = *(const v4f*)(q + b * d + k);
+    for (int k = threadIdx.x * 4; k < dpad; k += 1024) {
+        const v4f x = k < d ? *(const v4f*)(q + b * d + k) : v4f{0.f, 0.f, 0.f, 0.f};
         uint32_t lo[2], hi[2];
         split_pair(x[0], x[1], lo);
         split_pair(x[2], x[3], hi);
-        *(uint2*)(out + b * d + k) = uint2{lo[0], hi[0]};
-        *(uint2*)(out + n + b * d + k) = uint2{lo[1], hi[1]};
+        char* to = out + b * dpad * 4 + split_at(k);
+        *(uint2*)to = uint2{lo[0], hi[0]};
+        *(uint2*)(to + 64) = uint2{lo[1], hi[1]};
 #pragma unroll
         for (int c = 0; c < 4; ++c) top = fmaxf(top, fabsf(x[c]));
     }
@@ -447,6 +527,7 @@ struct RowArgs {
     const float* part;               // slabs [splits][B][lds] of s
     float* s;                        // their sum (part itself where there is one)
     int splits, segs;
+    bool ready;                      // seg is there: one workgroup a row
     int64_t slab, lds;
     const float* temp;
     const int64_t* idx;
@@ -508,8 +589,8 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
     // ---- this segment's columns: the slabs' sum, the maximum of z and its first column, the sum of exp
     float mx, se;
     int am;
-    bool nan;
-    {
+    bool nan = false;
+    if (!a.ready) {
         const int64_t j0 = (int64_t)blockIdx.x * DISTILL_SEG + tid * 4;
         v4f x[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
         bool in[2];
@@ -529,7 +610,6 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
                     if (p + o < a.splits && in[u]) x[u] += y[o][u];
         }
         mx = -INFINITY;
-        nan = false;
         am = INT32_MAX;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -558,7 +638,23 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
         se = r2.b;
         am = r2.c;
     }
-    if (a.segs > 1) {
+    if (a.ready) {
+        // ---- the product's waves have left a record for each of their stretches of the row
+        const v4f* seg = (const v4f*)a.seg + b * a.segs;
+        mx = -INFINITY;
+        for (int i = tid; i < a.segs; i += 256) mx = fmaxf(mx, seg[i][0]);
+        mx = block_red(mx, 0.f, 0, red).a;
+        se = 0.f;
+        am = INT32_MAX;
+        for (int i = tid; i < a.segs; i += 256) {
+            const v4f x = seg[i];
+            if (x[0] == mx) am = min(am, __float_as_int(x[2]));
+            se += x[0] > -INFINITY ? x[1] * exp_neg(x[0] - mx) : x[1];   // (nothing but NaN there: x[1] is NaN, else 0)
+        }
+        const Red r = block_red(0.f, se, am, red);
+        se = r.b;
+        am = r.c;
+    } else if (a.segs > 1) {
         float* seg = a.seg + b * a.segs * 4;
         if (tid == 0) {
             put(seg + blockIdx.x * 4, mx);
@@ -698,11 +794,11 @@ struct GradArgs {
     const int* li;
     const float* has;                // [B]: 1 where the row has an entry
     const float* temp;
-    int64_t B, T, ldg;
+    int64_t T, ldg;
     int k;
     int form;                        // G_F32, G_F16 (G_F32 where flag is set) or G_BF16
     const unsigned* flag;
-    void* g;                         // fp32 [B][ldg], or two parts of 16 bits; zeros from T on
+    void* g;                         // [B][ldg] fp32 or two parts of 16 bits; zeros from T on
     float* dt;                       // [B][segments]: sums of (softmax - target) z
 };
 
@@ -752,9 +848,9 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(const GradArgs a) {
                 split_pair(y[2], y[3], h3);
                 lo[0] = l3[0]; lo[1] = l3[1]; hi[0] = h3[0]; hi[1] = h3[1];
             }
-            uint16_t* out = (uint16_t*)a.g + b * a.ldg + j;
+            char* out = (char*)a.g + b * a.ldg * 4 + split_at(j);
             *(uint2*)out = uint2{lo[0], hi[0]};
-            *(uint2*)(out + a.B * a.ldg) = uint2{lo[1], hi[1]};
+            *(uint2*)(out + 64) = uint2{lo[1], hi[1]};
         }
     }
     dt = block_red(0.f, dt, 0, red).b;
@@ -842,8 +938,8 @@ struct FwdLayout {
 static FwdLayout fwd_layout(int dtype, int64_t B, int64_t T, int d, int k) {
     FwdLayout L;
     L.s = plan(B, T, d);
-    L.lds = (T + 7) / 8 * 8;
-    L.segs = (int)((T + DISTILL_SEG - 1) / DISTILL_SEG);
+    L.lds = (T + 31) / 32 * 32;
+    L.segs = L.s.splits == 1 ? L.s.nn * 2 : (int)((T + DISTILL_SEG - 1) / DISTILL_SEG);
     // from about 8 GFLOP a product on, half the matrix work is worth the launches that find out and then return
     L.fast = dtype == ABC_DT_F32 && L.s.tile == 128 && 2.0 * (double)B * (double)T * d >= 8e9;
     size_t o = up((size_t)L.s.splits * B * L.lds * 4);
@@ -856,7 +952,7 @@ static FwdLayout fwd_layout(int dtype, int64_t B, int64_t T, int d, int k) {
     L.off_row = o; o += up((size_t)B * 12);
     L.off_stat = o; o += 256;
     L.off_cnt = o; o += up((size_t)(B + 1 + (B + 31) / 32) * 4);
-    L.off_q = o; o += L.fast ? up((size_t)B * d * 4) : 0;
+    L.off_q = o; o += L.fast ? up((size_t)B * ((d + 31) / 32 * 32) * 4) : 0;
     L.off_qout = o; o += L.fast ? up((size_t)B * 4) : 0;
     L.off_flag = o; o += 256;
     L.total = o;
@@ -866,7 +962,7 @@ static FwdLayout fwd_layout(int dtype, int64_t B, int64_t T, int d, int k) {
 struct BwdLayout { Plan q, p; int64_t ldg; int segs; size_t off_g, off_dt, off_pq, off_pp, total; };
 static BwdLayout bwd_layout(int64_t B, int64_t C, int64_t T, int d, bool fast, bool dq, bool dp) {
     BwdLayout L;
-    L.ldg = (T + 7) / 8 * 8;
+    L.ldg = (T + 31) / 32 * 32;                                // as the logits' rows
     L.segs = (int)((L.ldg + DISTILL_SEG - 1) / DISTILL_SEG);
     L.q = plan(B, d, T);
     L.p = plan(C, d, B);
@@ -937,22 +1033,22 @@ static void launch_grads(const GemmArgs& gq, const GemmArgs& gp, bool dq, bool d
 }
 
 // s: bf16; fp32 by three bf16 parts (128 / 64 wide tiles); fp32 by two fp16 parts (the queries' are ready)
-typedef Cfg<LoadKC<RAW, 1, 128, 2, 1>, LoadKC<RAW, 1, 128, 2, 1>, 1, 1, 1, 128, 128, 2, 1, 2, false, false> ScoresB128;
-typedef Cfg<LoadKC<RAW, 1, 64, 2, 2>, LoadKC<RAW, 1, 64, 2, 2>, 1, 1, 1, 64, 64, 2, 2, 2, false, false> ScoresB64;
-typedef Cfg<LoadKC<SPLIT_B3, 3, 128, 1, 1>, LoadKC<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, false, false> ScoresF128;
-typedef Cfg<LoadKC<SPLIT_B3, 3, 64, 1, 3>, LoadKC<SPLIT_B3, 3, 64, 1, 3>, 3, 3, 3, 64, 64, 1, 3, 2, false, false> ScoresF64;
-typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKC<SPLIT_H2, 2, 128, 1, 1, true>, 2, 2, 2, 128, 128, 1, 1, 2, true, false> ScoresH128;
+typedef Cfg<LoadKC<RAW, 1, 128, 2, 1>, LoadKC<RAW, 1, 128, 2, 1>, 1, 1, 1, 128, 128, 2, 1, 2, 0, false, false> ScoresB128;
+typedef Cfg<LoadKC<RAW, 1, 64, 2, 2>, LoadKC<RAW, 1, 64, 2, 2>, 1, 1, 1, 64, 64, 2, 2, 2, 0, false, false> ScoresB64;
+typedef Cfg<LoadKC<SPLIT_B3, 3, 128, 1, 1>, LoadKC<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, 0, false, false> ScoresF128;
+typedef Cfg<LoadKC<SPLIT_B3, 3, 64, 1, 3>, LoadKC<SPLIT_B3, 3, 64, 1, 3>, 3, 3, 3, 64, 64, 1, 3, 2, 1, false, false> ScoresF64;
+typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKC<SPLIT_H2, 2, 128, 1, 1, true>, 2, 2, 2, 128, 128, 1, 1, 2, 3, true, false> ScoresH128;
 // dq = g cand, dc = g^T q
-typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKS<RAW, 1, 128, 1, 1>, 2, 1, 2, 128, 128, 1, 1, 2, false, true> GradQB128;
-typedef Cfg<LoadKS<RAW, 2, 128, 1, 1>, LoadKS<RAW, 1, 128, 1, 1>, 2, 1, 2, 128, 128, 1, 1, 2, false, true> GradPB128;
-typedef Cfg<LoadKC<RAW, 2, 64, 2, 2>, LoadKS<RAW, 1, 64, 2, 2>, 2, 1, 2, 64, 64, 2, 2, 2, false, true> GradQB64;
-typedef Cfg<LoadKS<RAW, 2, 64, 2, 2>, LoadKS<RAW, 1, 64, 2, 2>, 2, 1, 2, 64, 64, 2, 2, 2, false, true> GradPB64;
-typedef Cfg<LoadKC<SPLIT_B3, 3, 128, 1, 1>, LoadKS<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, false, false> GradQF128;
-typedef Cfg<LoadKS<SPLIT_B3, 3, 128, 1, 1>, LoadKS<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, false, false> GradPF128;
-typedef Cfg<LoadKC<SPLIT_B3, 3, 64, 1, 2>, LoadKS<SPLIT_B3, 3, 64, 1, 2>, 3, 3, 3, 64, 64, 1, 2, 2, false, false> GradQF64;
-typedef Cfg<LoadKS<SPLIT_B3, 3, 64, 1, 2>, LoadKS<SPLIT_B3, 3, 64, 1, 2>, 3, 3, 3, 64, 64, 1, 2, 2, false, false> GradPF64;
-typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKS<SPLIT_H2, 2, 128, 1, 1>, 2, 2, 2, 128, 128, 1, 1, 2, true, false> GradQH128;
-typedef Cfg<LoadKS<RAW, 2, 128, 1, 1>, LoadKS<RAW, 2, 128, 1, 1>, 2, 2, 2, 128, 128, 1, 1, 2, true, false> GradPH128;
+typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKS<RAW, 1, 128, 1, 1>, 2, 1, 2, 128, 128, 1, 1, 2, 1, false, true> GradQB128;
+typedef Cfg<LoadKS<RAW, 2, 128, 1, 1>, LoadKS<RAW, 1, 128, 1, 1>, 2, 1, 2, 128, 128, 1, 1, 2, 1, false, true> GradPB128;
+typedef Cfg<LoadKC<RAW, 2, 64, 2, 2>, LoadKS<RAW, 1, 64, 2, 2>, 2, 1, 2, 64, 64, 2, 2, 2, 1, false, true> GradQB64;
+typedef Cfg<LoadKS<RAW, 2, 64, 2, 2>, LoadKS<RAW, 1, 64, 2, 2>, 2, 1, 2, 64, 64, 2, 2, 2, 1, false, true> GradPB64;
+typedef Cfg<LoadKC<SPLIT_B3, 3, 128, 1, 1>, LoadKS<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, 0, false, false> GradQF128;
+typedef Cfg<LoadKS<SPLIT_B3, 3, 128, 1, 1>, LoadKS<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, 0, false, false> GradPF128;
+typedef Cfg<LoadKC<SPLIT_B3, 3, 64, 1, 2>, LoadKS<SPLIT_B3, 3, 64, 1, 2>, 3, 3, 3, 64, 64, 1, 2, 2, 1, false, false> GradQF64;
+typedef Cfg<LoadKS<SPLIT_B3, 3, 64, 1, 2>, LoadKS<SPLIT_B3, 3, 64, 1, 2>, 3, 3, 3, 64, 64, 1, 2, 2, 1, false, false> GradPF64;
+typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKS<SPLIT_H2, 2, 128, 1, 1>, 2, 2, 2, 128, 128, 1, 1, 2, 1, true, false> GradQH128;
+typedef Cfg<LoadKS<RAW, 2, 128, 1, 1>, LoadKS<RAW, 2, 128, 1, 1>, 2, 2, 2, 128, 128, 1, 1, 2, 1, true, false> GradPH128;
 
 extern "C" int abc_distill_fwd(int dtype, const void* q, const void* p, const void* memory, const float* temp, const int64_t* teacher_idx,
                                const float* teacher_score, float teacher_temp, int64_t B, int64_t C, int64_t M, int d, int k,
@@ -971,26 +1067,28 @@ extern "C" int abc_distill_fwd(int dtype, const void* q, const void* p, const vo
     unsigned* cnt = (unsigned*)(w + L.off_cnt);
     unsigned* flag = (unsigned*)(w + L.off_flag);
     const int nc = (int)(B + 1 + (B + 31) / 32);
-    const Side sq{q, q, B, d, B, 0}, sc{p, memory, C, d, T, 0};
-    const GemmArgs g = gemm_args(sq, sc, d, L.s, w, L.lds, B * L.lds);
+    const Side sq{q, q, B, d, B}, sc{p, memory, C, d, T};
+    GemmArgs g = gemm_args(sq, sc, d, L.s, w, L.lds, B * L.lds);
+    const bool ready = L.s.splits == 1;
+    if (ready) { g.seg = (float*)(w + L.off_seg); g.segs = L.segs; g.f2 = temp; }
     if (dtype == ABC_DT_BF16) {
         if (L.s.tile == 128) launch_scores<ScoresB128>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
         else launch_scores<ScoresB64>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
     } else if (L.fast) {
         unsigned* qout = (unsigned*)(w + L.off_qout);
-        hipLaunchKernelGGL(distill_split_kernel, dim3((unsigned)B), dim3(256), 0, st, (const float*)q, d, B * d, (uint16_t*)(w + L.off_q), qout, flag);
+        hipLaunchKernelGGL(distill_split_kernel, dim3((unsigned)B), dim3(256), 0, st, (const float*)q, d, (d + 31) / 32 * 32, w + L.off_q, qout, flag);
         GemmArgs h = g;
-        h.a = Side{w + L.off_q, w + L.off_q, B, d, B, B * d * 2};
+        h.a = Side{w + L.off_q, w + L.off_q, B, (d + 31) / 32 * 64, B};
         launch_scores<ScoresH128>(h, nullptr, 0, flag, qout, B, cnt, nc, st);
         launch_scores<ScoresF128>(g, flag, 1, nullptr, nullptr, 0, nullptr, 0, st);
     } else if (L.s.tile == 128) launch_scores<ScoresF128>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
     else launch_scores<ScoresF64>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
     RowArgs r;
-    r.part = (const float*)w; r.s = (float*)(w + L.off_s); r.splits = L.s.splits; r.segs = L.segs; r.slab = B * L.lds; r.lds = L.lds;
+    r.part = (const float*)w; r.s = (float*)(w + L.off_s); r.splits = L.s.splits; r.segs = L.segs; r.ready = ready; r.slab = B * L.lds; r.lds = L.lds;
     r.temp = temp; r.idx = teacher_idx; r.score = teacher_score; r.teacher_temp = teacher_temp; r.B = B; r.T = T; r.k = k;
     r.seg = (float*)(w + L.off_seg); r.lse = (float*)(w + L.off_lse); r.t = (float*)(w + L.off_t); r.li = (int*)(w + L.off_li);
     r.row = (float*)(w + L.off_row); r.stat = (float*)(w + L.off_stat); r.cnt = cnt; r.out_loss = out_loss; r.out_agree = out_agree;
-    hipLaunchKernelGGL(distill_row_kernel, dim3((unsigned)L.segs, (unsigned)B), dim3(256), 0, st, r);
+    hipLaunchKernelGGL(distill_row_kernel, dim3(ready ? 1u : (unsigned)L.segs, (unsigned)B), dim3(256), 0, st, r);
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? ABC_OK : abc_fail_hip(e, "distill_fwd launch");
 }
@@ -1019,24 +1117,29 @@ extern "C" int abc_distill_bwd(int dtype, const void* q, const void* p, const vo
     GradArgs a;
     a.s = (const float*)(f + F.off_s); a.lds = F.lds; a.lse = (const float*)(f + F.off_lse); a.t = (const float*)(f + F.off_t);
     a.li = (const int*)(f + F.off_li); a.has = (const float*)(f + F.off_row) + 2 * B; a.temp = temp;
-    a.B = B; a.T = T; a.ldg = L.ldg; a.k = k; a.form = bf ? G_BF16 : F.fast ? G_F16 : G_F32; a.flag = flag;
+    a.T = T; a.ldg = L.ldg; a.k = k; a.form = bf ? G_BF16 : F.fast ? G_F16 : G_F32; a.flag = flag;
     a.g = w + L.off_g; a.dt = (float*)(w + L.off_dt);
     hipLaunchKernelGGL(distill_grad_kernel, dim3((unsigned)L.segs, (unsigned)B), dim3(256), 0, st, a);
     SumArgs sa = {};
     if (dq || dp) {
-        const Side gq{a.g, a.g, B, L.ldg, B, B * L.ldg * 2}, gp{a.g, a.g, B, L.ldg, C, B * L.ldg * 2};
-        const Side cand{p, memory, C, d, d, 0}, query{q, q, B, d, d, 0};
+        const Side gq{a.g, a.g, B, L.ldg, B}, gp{a.g, a.g, B, L.ldg, C};                       // fp32
+        const Side hq{a.g, a.g, B, L.ldg * 2, B}, hp{a.g, a.g, B, L.ldg * 2, C};               // two parts
+        const Side cand{p, memory, C, d, d}, query{q, q, B, d, d};
         GemmArgs xq = gemm_args(gq, cand, T, L.q, L.q.splits > 1 ? (void*)(w + L.off_pq) : dq, d, B * d);
         GemmArgs xp = gemm_args(gp, query, B, L.p, L.p.splits > 1 ? (void*)(w + L.off_pp) : dp, d, C * d);
         for (GemmArgs* x : {&xq, &xp}) { x->f0 = grad_out; x->f1 = stat; x->f2 = temp; }
         if (bf) {
+            xq.a = hq;
+            xp.a = hp;
             if (L.q.tile == 128) launch_grads<GradQB128, GradPB128>(xq, xp, dq, dp, nullptr, 0, st);
             else launch_grads<GradQB64, GradPB64>(xq, xp, dq, dp, nullptr, 0, st);
         } else if (F.fast) {
-            GemmArgs hq = xq, hp = xp;
-            hq.scale = hp.scale = 1.0f / G_SCALE;
-            hp.b = Side{f + F.off_q, f + F.off_q, B, d, d, B * d * 2};
-            launch_grads<GradQH128, GradPH128>(hq, hp, dq, dp, flag, 0, st);
+            GemmArgs yq = xq, yp = xp;
+            yq.scale = yp.scale = 1.0f / G_SCALE;
+            yq.a = hq;
+            yp.a = hp;
+            yp.b = Side{f + F.off_q, f + F.off_q, B, (d + 31) / 32 * 64, d};
+            launch_grads<GradQH128, GradPH128>(yq, yp, dq, dp, flag, 0, st);
             launch_grads<GradQF128, GradPF128>(xq, xp, dq, dp, flag, 1, st);
         } else if (L.q.tile == 128) launch_grads<GradQF128, GradPF128>(xq, xp, dq, dp, nullptr, 0, st);
         else launch_grads<GradQF64, GradPF64>(xq, xp, dq, dp, nullptr, 0, st);
