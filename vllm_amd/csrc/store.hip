@@ -22,6 +22,7 @@ int abc_fail_invalid(const char* msg);
 int abc_fail_ws(size_t need, size_t have);
 
 #define STORE_MAX_DIM 8192
+#define SCORE_LDS 163840              // a workgroup's LDS in the scoring kernel: a CU's
 #define STORE_SCAN_MAX 1024          // writes of up to this many rows look for repeated slots inside the writing kernel
 
 typedef __attribute__((ext_vector_type(8))) __bf16 v8bf;
@@ -374,18 +375,47 @@ __device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uin
 // queries up to 16 fp32 (64 bf16).  A wave owns a tile of 16 rows: its lanes load 16 bytes of codes, four conversions a word make a
 // bf16 B fragment of them (e2m1 values are exact in bf16), and 16x16x32 MFMAs multiply it with the queries' fragments out of LDS.
 // fp32 queries stand in LDS as three bf16 parts (24 bits), in rows 4 q + part of the A tile, so that a lane's accumulators hold the
-// parts' sums of one query; products and sums are fp32.  A group's sum is scaled once.
+// parts' sums of one query; products and sums are fp32.  A group's sum is scaled once.  The loads of the next four pieces (the next
+// tile's, at a tile's end) are on their way while four are multiplied: 8 KB a wave, 128 KB a CU.  Scales come 16 bytes a lane, 32 of
+// a row at a time, and go through a strip of LDS of the wave's own (read where they are needed, 2 bytes a lane, they cost a third of the
+// time: every access touches 16 lines).
+#define SCORE_WAVES 16               // a workgroup: all that a CU holds of this kernel, so that the queries stand in its LDS once
+#define SCORE_STRIP 1280             // bytes of scales a wave: 16 rows of 32, 80 bytes apart
+
+template <int GROUP>
+struct ScorePieces {
+    static constexpr int G = 128 / GROUP;
+    v4u code[4];
+    // four pieces of a row from piece cb on, n of them there (scalar, at least 1): the last again past them
+    __device__ __forceinline__ void fetch(const char* dr, int cb, int n) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) code[u] = *(const v4u*)(dr + (cb + (u < n ? u : n - 1)) * 64);
+    }
+};
+// 8 of the 32 scales from `at` on (in 2-byte units from the first row's first scale; `total` of them in all)
+__device__ __forceinline__ v4u fetch_scales(const uint16_t* scale, int64_t at, int64_t total) {
+    if (at + 8 <= total) return *(const v4u_u*)(scale + at);
+    v4u w = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (at + j < total) w[j >> 1] |= (uint32_t)scale[at + j] << (16 * (j & 1));
+    return w;
+}
+
 template <bool QBF16, int GROUP, int MT>
-__global__ __launch_bounds__(512) void store_scores_kernel(const StoreScoreArgs a) {
+__global__ __launch_bounds__(64 * SCORE_WAVES) void store_scores_kernel(const StoreScoreArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
-    constexpr int P = QBF16 ? 1 : 3, G = 128 / GROUP, U = 4;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int P = QBF16 ? 1 : 3, G = 128 / GROUP, R = QBF16 ? 4 : 3;    // R: accumulators of a lane that mean something
+    constexpr int EACH = 8 / G;                                  // groups of four pieces that 32 scales of a row serve
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l15 = lane & 15, c = lane >> 4;
+    char* strip = smem_raw + wave * SCORE_STRIP;
+    char* const qlds = smem_raw + SCORE_WAVES * SCORE_STRIP;
     const int pitch = a.slice * 256 + 16;                        // bytes a query part
     const int lrows = a.nq * P;
     typedef typename std::conditional<QBF16, v4f, float>::type red_t;      // fp32 queries: the parts are summed first
-    red_t* red = (red_t*)(smem_raw + lrows * pitch);
-    const int ks = wave & (a.ks - 1), sub = wave / a.ks, per = 8 / a.ks;
+    red_t* red = (red_t*)(qlds + lrows * pitch);
+    const int ks = wave & (a.ks - 1), sub = wave / a.ks, per = SCORE_WAVES / a.ks;
     const int64_t tiles = (a.rows + 15) / 16;
     const int nslices = (a.chunks + a.slice - 1) / a.slice;
     int arow[MT];                                                // byte offset of this lane's row of each A tile
@@ -402,11 +432,11 @@ __global__ __launch_bounds__(512) void store_scores_kernel(const StoreScoreArgs 
     }
     auto fill = [&](int s) {
         const int c0 = s * a.slice, nc = min(a.slice, a.chunks - c0);
-        for (int i = threadIdx.x; i < a.nq * nc * 16; i += 512) {
+        for (int i = threadIdx.x; i < a.nq * nc * 16; i += 64 * SCORE_WAVES) {
             const int qi = i / (nc * 16), p = i - qi * (nc * 16);
             float v[8];
             load8<QBF16>((const char*)a.q + qi * a.ldq * (QBF16 ? 2 : 4), (c0 * 16 + p) * 8, a.dim, v);
-            char* dst = smem_raw + qi * P * pitch + p * 16;
+            char* dst = qlds + qi * P * pitch + p * 16;
             if constexpr (QBF16) {
                 v4u w;
 #pragma unroll
@@ -422,71 +452,105 @@ __global__ __launch_bounds__(512) void store_scores_kernel(const StoreScoreArgs 
             }
         }
     };
-    if (nslices == 1) {
+    auto row_of = [&](int64_t tile) { const int64_t n = tile * 16 + l15; return n < a.rows ? n : a.rows - 1; };
+    auto data_of = [&](int64_t row) { return a.data + row * (int64_t)(a.chunks * 64) + c * 16; };
+    const int64_t total = a.rows * (int64_t)(a.chunks * G);
+    auto scales = [&](int64_t row, int cb) { return fetch_scales(a.scale, (row * a.chunks + cb) * G + c * 8, total); };
+    // the waves that share a tile take runs of pieces of a slice
+    auto first_of = [&](int c0, int c1, int w) { return c0 + min(c1 - c0, w * ((c1 - c0 + a.ks - 1) / a.ks)); };
+
+    v4f sum[MT];
+    ScorePieces<GROUP> cur, next;
+    v4u nscale = {0, 0, 0, 0};
+    // at: the first piece's place in the queries' LDS; j: the group's place in the strip
+    auto multiply = [&](int at, int j, int n) {
+        uint32_t sc[2 * G];
+        if constexpr (G == 1) { const v2u w = *(const v2u*)(strip + l15 * 80 + j * 8); sc[0] = w[0]; sc[1] = w[1]; }
+        else {
+#pragma unroll
+            for (int i = 0; i < G / 2; ++i) {
+                const v4u w = *(const v4u*)(strip + l15 * 80 + j * 8 * G + i * 16);
+                sc[4 * i] = w[0]; sc[4 * i + 1] = w[1]; sc[4 * i + 2] = w[2]; sc[4 * i + 3] = w[3];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int lbase = at + u * 256;
+            v4f acc[MT];
+            if (u >= n) continue;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                union { v8bf f; v2bf h[4]; } b;
+                b.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cur.code[u][m], 1.0f, 0);
+                b.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cur.code[u][m], 1.0f, 1);
+                b.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cur.code[u][m], 1.0f, 2);
+                b.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cur.code[u][m], 1.0f, 3);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    if (m % (4 / G) == 0) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+                    const v8bf av = *(const v8bf*)(qlds + arow[t] + lbase + m * 64);
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, b.f, acc[t], 0, 0, 0);
+                }
+                if (m % (4 / G) == 4 / G - 1) {
+                    const int k = u * G + m / (4 / G);
+                    const float f = __uint_as_float((k & 1) ? (sc[k / 2] & 0xFFFF0000u) : (sc[k / 2] << 16));
+#pragma unroll
+                    for (int t = 0; t < MT; ++t)
+#pragma unroll
+                        for (int r = 0; r < R; ++r) sum[t][r] = fmaf(f, acc[t][r], sum[t][r]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);                   // fragments of one piece at a time: four waves a SIMD hide their reads
+        }
+    };
+
+    const bool whole = nslices == 1;                             // the queries stand in LDS for good
+    const int64_t first0 = (int64_t)blockIdx.x * per, step = (int64_t)gridDim.x * per;
+    if (whole) {
+        const int w0 = first_of(0, a.chunks, ks), w1 = first_of(0, a.chunks, ks + 1);
+        if (first0 + sub < tiles && w0 < w1) {
+            const int64_t row = row_of(first0 + sub);
+            nscale = scales(row, w0);
+            next.fetch(data_of(row), w0, w1 - w0);
+        }
         fill(0);
         __syncthreads();
     }
     // every workgroup makes the same number of rounds for all of its waves: the barriers inside are met by all of them
-    for (int64_t first = (int64_t)blockIdx.x * per; first < tiles; first += (int64_t)gridDim.x * per) {
+    for (int64_t first = first0; first < tiles; first += step) {
         const int64_t tile = first + sub;
         const int64_t n = tile * 16 + l15;
-        const int64_t row = n < a.rows ? n : a.rows - 1;
-        const char* dr = a.data + row * (int64_t)(a.chunks * 64) + c * 16;
-        const uint16_t* sr = a.scale + row * (int64_t)(a.chunks * G);
-        v4f sum[MT];
 #pragma unroll
         for (int t = 0; t < MT; ++t) sum[t] = v4f{0.f, 0.f, 0.f, 0.f};
         for (int s = 0; s < nslices; ++s) {
-            if (nslices > 1) {
+            const int c0 = s * a.slice, c1 = min(a.chunks, c0 + a.slice);
+            const int e0 = first_of(c0, c1, ks), e1 = first_of(c0, c1, ks + 1);
+            const int64_t row = row_of(tile < tiles ? tile : tiles - 1);
+            const char* dr = data_of(row);
+            if (!whole) {
+                if (e0 < e1) {
+                    nscale = scales(row, e0);
+                    next.fetch(dr, e0, e1 - e0);
+                }
                 __syncthreads();                                 // the last slice has been read
                 fill(s);
                 __syncthreads();
             }
             if (tile >= tiles) continue;
-            const int c0 = s * a.slice, c1 = min(a.chunks, c0 + a.slice);
-            v4u code[U];
-            uint32_t sc[U][(G + 1) / 2];
-            auto fetch = [&](int ch, int u) {
-                const int at = ch < c1 ? ch : c1 - 1;
-                code[u] = *(const v4u*)(dr + at * 64);
-                if constexpr (G == 1) sc[u][0] = sr[at];
-                else if constexpr (G == 2) sc[u][0] = *(const uint32_t*)(sr + at * 2);
-                else { const v2u w = *(const v2u*)(sr + at * 4); sc[u][0] = w[0]; sc[u][1] = w[1]; }
-            };
-            for (int cb = c0 + ks; cb < c1; cb += U * a.ks) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) fetch(cb + u * a.ks, u);
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int ch = cb + u * a.ks;
-                    if (ch < c1) {
-                        const int lbase = (ch - c0) * 256;
-                        v4f acc[MT];
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) {
-                            union { v8bf f; v2bf h[4]; } b;
-                            b.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[u][m], 1.0f, 0);
-                            b.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[u][m], 1.0f, 1);
-                            b.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[u][m], 1.0f, 2);
-                            b.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[u][m], 1.0f, 3);
-#pragma unroll
-                            for (int t = 0; t < MT; ++t) {
-                                if (m % (4 / G) == 0) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
-                                const v8bf av = *(const v8bf*)(smem_raw + arow[t] + lbase + m * 64);
-                                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, b.f, acc[t], 0, 0, 0);
-                            }
-                            if (m % (4 / G) == 4 / G - 1) {
-                                const int g = m / (4 / G);
-                                const uint32_t w = sc[u][g / 2];
-                                const float f = __uint_as_float((g & 1) ? (w & 0xFFFF0000u) : (w << 16));
-#pragma unroll
-                                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                                    for (int r = 0; r < 4; ++r) sum[t][r] = fmaf(f, acc[t][r], sum[t][r]);
-                            }
-                        }
-                    }
+            for (int cb = e0, j = 0; cb < e1; cb += 4) {
+                cur = next;
+                if (j == 0) *(v4u*)(strip + l15 * 80 + c * 16) = nscale;     // (a wave's LDS accesses are carried out in order)
+                const int jn = j + 1 == EACH ? 0 : j + 1;
+                if (cb + 4 < e1) {
+                    if (jn == 0) nscale = scales(row, cb + 4);
+                    next.fetch(dr, cb + 4, e1 - cb - 4);
+                } else if (whole && tile + step < tiles) {
+                    const int64_t r2 = row_of(tile + step);
+                    nscale = scales(r2, e0);
+                    next.fetch(data_of(r2), e0, e1 - e0);
                 }
+                multiply((cb - c0) * 256, j, e1 - cb);
+                j = jn;
             }
         }
         red_t res[MT];
@@ -524,11 +588,21 @@ __global__ __launch_bounds__(512) void store_scores_kernel(const StoreScoreArgs 
     }
 }
 
+template <bool QBF16, int GROUP, int MT>
+static hipError_t scores_launch_mt(const StoreScoreArgs& a, unsigned grid, size_t lds, hipStream_t st) {
+    if (lds > 65536) {                                            // of the current device's copy of the kernel
+        const hipError_t e = hipFuncSetAttribute((const void*)store_scores_kernel<QBF16, GROUP, MT>, hipFuncAttributeMaxDynamicSharedMemorySize, SCORE_LDS);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((store_scores_kernel<QBF16, GROUP, MT>), dim3(grid), dim3(64 * SCORE_WAVES), lds, st, a);
+    return hipGetLastError();
+}
 template <bool QBF16, int GROUP>
-static void scores_launch(const StoreScoreArgs& a, int mt, unsigned grid, size_t lds, hipStream_t st) {
-    if (mt == 1) hipLaunchKernelGGL((store_scores_kernel<QBF16, GROUP, 1>), dim3(grid), dim3(512), lds, st, a);
-    else if (mt == 2) hipLaunchKernelGGL((store_scores_kernel<QBF16, GROUP, 2>), dim3(grid), dim3(512), lds, st, a);
-    else hipLaunchKernelGGL((store_scores_kernel<QBF16, GROUP, 4>), dim3(grid), dim3(512), lds, st, a);
+static hipError_t scores_launch(const StoreScoreArgs& a, int mt, unsigned grid, size_t lds, hipStream_t st) {
+    if (mt == 1) return scores_launch_mt<QBF16, GROUP, 1>(a, grid, lds, st);
+    if (mt == 2) return scores_launch_mt<QBF16, GROUP, 2>(a, grid, lds, st);
+    if (mt == 3) return scores_launch_mt<QBF16, GROUP, 3>(a, grid, lds, st);
+    return scores_launch_mt<QBF16, GROUP, 4>(a, grid, lds, st);
 }
 
 extern "C" int abc_store_scores(int q_dtype, const void* q, int64_t ldq, int64_t nq, const void* data, const void* scale, int64_t rows,
@@ -555,30 +629,30 @@ extern "C" int abc_store_scores(int q_dtype, const void* q, int64_t ldq, int64_t
         a.data = (const char*)data; a.scale = (const uint16_t*)scale; a.rows = rows;
         a.dim = dim; a.chunks = chunks; a.out = out + q0 * ldo; a.ldo = ldo;
         const int tiles16 = bf ? (a.nq + 15) / 16 : (a.nq + 3) / 4;
-        const int mt = tiles16 > 2 ? 4 : tiles16;
-        // 64 KB of LDS, so that two workgroups of 8 waves stand on a CU: the queries, and the sums of waves that share a tile
+        const int mt = tiles16;
+        // LDS: the waves' strips of scales, the queries (in slices of a row where they are too many), the sums of waves that share a tile
         const int64_t tiles = (rows + 15) / 16;
         int slice = 0, ks = 1;
         size_t red = 0;
-        auto fit = [&] {
-            slice = (int)((65536 - red) / (a.nq * parts) - 16) / 256;      // 1 at least: 64 rows of 272 bytes fit beside 32 KB
+        auto fit = [&] {                                          // 1 piece at least: 64 rows of 272 bytes fit beside 84 KB
+            slice = (int)((SCORE_LDS - SCORE_WAVES * SCORE_STRIP - red) / (a.nq * parts) - 16) / 256;
             if (slice > chunks) slice = chunks;
         };
         fit();
         if (tiles < 2048 && chunks > 1) {
-            red = (size_t)8 * mt * 64 * (bf ? 16 : 4);
+            red = (size_t)SCORE_WAVES * mt * 64 * (bf ? 16 : 4);
             fit();
             while (ks < 8 && tiles * ks < 4096 && ks * 2 <= slice) ks *= 2;
         }
         a.slice = slice;
         a.ks = ks;
-        const int64_t wgs = (tiles + 8 / ks - 1) / (8 / ks);
-        const unsigned grid = (unsigned)(wgs < 512 ? wgs : 512);
-        const size_t lds = (size_t)a.nq * parts * (slice * 256 + 16) + red;
-        if (group == 32) { if (bf) scores_launch<true, 32>(a, mt, grid, lds, st); else scores_launch<false, 32>(a, mt, grid, lds, st); }
-        else if (group == 64) { if (bf) scores_launch<true, 64>(a, mt, grid, lds, st); else scores_launch<false, 64>(a, mt, grid, lds, st); }
-        else { if (bf) scores_launch<true, 128>(a, mt, grid, lds, st); else scores_launch<false, 128>(a, mt, grid, lds, st); }
-        hipError_t e = hipGetLastError();
+        const int64_t wgs = (tiles + SCORE_WAVES / ks - 1) / (SCORE_WAVES / ks);
+        const unsigned grid = (unsigned)(wgs < 256 ? wgs : 256);
+        const size_t lds = (size_t)SCORE_WAVES * SCORE_STRIP + (size_t)a.nq * parts * (slice * 256 + 16) + red;
+        hipError_t e;
+        if (group == 32) e = bf ? scores_launch<true, 32>(a, mt, grid, lds, st) : scores_launch<false, 32>(a, mt, grid, lds, st);
+        else if (group == 64) e = bf ? scores_launch<true, 64>(a, mt, grid, lds, st) : scores_launch<false, 64>(a, mt, grid, lds, st);
+        else e = bf ? scores_launch<true, 128>(a, mt, grid, lds, st) : scores_launch<false, 128>(a, mt, grid, lds, st);
         if (e != hipSuccess) return abc_fail_hip(e, "store_scores launch");
     }
     return ABC_OK;
