@@ -305,12 +305,15 @@ __global__ __launch_bounds__(256) void store_read_kernel(const StoreReadArgs a) 
     } else {
         const char* src = (const char*)a.data + row * (int64_t)a.width;
         const float s = ((const float*)a.scale)[row];
-        for (int p = t; p < pieces; p += tx) {
-            const v2u w = *(const v2u*)(src + p * 8);
-            float v[8];
+        for (int p = 2 * t; p < pieces; p += 2 * tx) {           // 16 codes a lane
+            const v4u w = *(const v4u*)(src + p * 8);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = (float)(int8_t)(w[j >> 2] >> (8 * (j & 3))) * s;
-            store8<BF16>(out, p * 8, a.dim, v);
+            for (int h = 0; h < 2; ++h) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = (float)(int8_t)(w[2 * h + (j >> 2)] >> (8 * (j & 3))) * s;
+                store8<BF16>(out, (p + h) * 8, a.dim, v);
+            }
         }
     }
 }
@@ -329,7 +332,7 @@ extern "C" int abc_store_read(const int64_t* index, int64_t first, int64_t n, co
     StoreReadArgs a;
     a.index = index; a.first = first; a.n = n; a.capacity = capacity; a.data = data; a.scale = scale;
     a.dim = dim; a.width = (dim + 127) / 128 * 128; a.out = out; a.ldo = ldo;
-    a.tx = row_threads((dim + 7) / 8);
+    a.tx = row_threads(group ? (dim + 7) / 8 : (dim + 15) / 16);
     const unsigned grid = (unsigned)((n + 256 / a.tx - 1) / (256 / a.tx));
     hipStream_t st = (hipStream_t)stream;
     const bool bf = out_dtype == ABC_DT_BF16;
