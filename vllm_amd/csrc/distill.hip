@@ -34,6 +34,7 @@ typedef __attribute__((ext_vector_type(8))) _Float16 v8h;
 typedef __attribute__((ext_vector_type(2))) _Float16 v2h;
 typedef __attribute__((ext_vector_type(2))) float v2f;
 typedef __attribute__((ext_vector_type(4))) unsigned int v4u;
+typedef __attribute__((ext_vector_type(2))) unsigned int v2u;
 
 #define DISTILL_MAX_K 1024
 #define DISTILL_SEG 2048            // columns of a row that one workgroup of the row and gradient kernels takes
@@ -57,6 +58,7 @@ struct Side {
     int64_t n0;                      // storage rows in p0
     int64_t ld;                      // elements between storage rows
     int64_t rows;                    // rows of the product on this side
+    int64_t width;                   // values of a storage row that may be read (a multiple of 8)
 };
 // Values that lie split into two 16-bit parts: blocks of 32 along the row, 64 bytes of the leading parts and then 64 of the others, so that
 // a stage's values of a row are one cache line.  ld counts 16-bit elements (two a value).
@@ -105,6 +107,7 @@ __device__ __forceinline__ int lds_at(int part, int row, int chunk) {
 // Storage goes on to a multiple of 8 values (parts: 32) with zeros.  RANGE: keeps the largest magnitude of what it reads.
 template <int NUM, int PARTS, int R, int NKB, int DEPTH, bool RANGE = false>
 struct LoadKC {
+    static constexpr bool KC = true;
     static constexpr int ES = bytes_of(NUM), LANES = NUM == RAW ? 4 : 8, N = R * LANES / 256, Q = NUM == RAW ? PARTS : 1, UNITS = N * NKB;
     const char* at[N];
     v4u w[DEPTH][NKB][N][Q];
@@ -181,6 +184,7 @@ struct LoadKC {
 // wave's writes go to neighbouring rows, and a lane's accumulators of two neighbouring blocks are neighbours in memory again.
 template <int NUM, int PARTS, int R, int NKB, int DEPTH>
 struct LoadKS {
+    static constexpr bool KC = false;
     static constexpr int ES = bytes_of(NUM), COLS = NUM != RAW && R * NKB * 2 < 256 ? 1 : 2, CG = R / COLS, N = CG * NKB * 4 / 256;
     static constexpr int Q = NUM == RAW ? PARTS : 1, UNITS = N * COLS;
     static_assert(N >= 1, "a tile too narrow for 256 threads");
@@ -243,6 +247,128 @@ struct LoadKS {
     __device__ __forceinline__ bool outside() { return false; }
 };
 
+// ---- sides that need no conversion: straight from memory into LDS -------------------------------------------------------
+// 16 bytes a lane, 1 KB a wave's instruction, no register on the way.  A stage is 32 values of k; PARTS of it lie one behind the other.
+// All of a workgroup's four waves take part; a stage's `issue` makes LOADS such instructions a wave.  `tail` brings a last, partial stage
+// through registers, with zeros past k1.
+__device__ __forceinline__ void to_lds(const char* src, char* lds) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+
+// rows in LDS as LoadKC leaves them; a fragment is one 16-byte read
+template <int PARTS, int R>
+struct DmaKC {
+    static constexpr bool KC = true;
+    static constexpr int LOADS = PARTS * R / 64, BYTES = PARTS * R * 64;
+    const char* at[R / 64];
+    int chunk, row0, wave;
+    __device__ __forceinline__ void init(const Side& s, int64_t r0, int tid) {
+        wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int lane = tid & 63;
+#pragma unroll
+        for (int i = 0; i < R / 64; ++i) {
+            row0 = wave * 16 + (lane >> 2);
+            chunk = (lane ^ (0 - (row0 >> 2))) & 3;               // what lds_at puts there (64 rows on, the same)
+            const int64_t r = r0 + row0 + i * 64;
+            at[i] = storage_row<2>(s, r < s.rows ? r : s.rows - 1) + chunk * 16;
+        }
+    }
+    __device__ __forceinline__ void issue(const Side&, int64_t k, char* lds) {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int i = 0; i < R / 64; ++i) to_lds(at[i] + k * (PARTS == 2 ? 4 : 2) + p * 64, lds + ((p * R + i * 64 + wave * 16) << 6));
+    }
+    __device__ __forceinline__ void tail(const Side&, int64_t k, int64_t k1, char* lds) {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int i = 0; i < R / 64; ++i) {
+                v4u x = {0, 0, 0, 0};
+                if (k + chunk * 8 < k1) x = *(const v4u*)(at[i] + k * (PARTS == 2 ? 4 : 2) + p * 64);
+                *(v4u*)(lds + lds_at<R, 1>(p, row0 + i * 64, chunk)) = x;
+            }
+    }
+    // the fragments of N blocks of 16 rows from `block` on
+    template <class F, int N>
+    static __device__ __forceinline__ void frags(F (&out)[N], const char* lds, int part, int block, int lane) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) out[j] = *(const F*)(lds + lds_at<R, 1>(part, (block + j) * 16 + (lane & 15), lane >> 4));
+    }
+};
+
+// storage rows (k) lie in LDS as they are, R values each; ds_read_b64_tr_b16 turns 4 of them by 16 columns on the way to a fragment.
+// 16-byte chunks are permuted with the row so that the 16 rows of a read spread over all banks.
+template <int PARTS, int R>
+struct DmaKS {
+    static constexpr bool KC = false;
+    static constexpr int CH = R / 8, PER = 64 / CH, EACH = 32 / PER / 4, LOADS = PARTS * EACH, BYTES = PARTS * R * 64;   // PER: rows an instruction
+    int64_t off;
+    int row0, wave;
+    static __device__ __forceinline__ int swz(int k) {
+        return R == 128 ? 2 * ((k & 3) | ((k >> 1) & 4)) : 2 * (((k >> 1) & 1) | ((k >> 2) & 2));
+    }
+    __device__ __forceinline__ void init(const Side& s, int64_t r0, int tid) {
+        wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int lane = tid & 63;
+        row0 = wave * PER + lane / CH;                            // and 4 PER rows on: the permutation repeats every 16 rows
+        int64_t col = r0 + ((lane % CH) ^ swz(row0)) * 8;
+        if (col > s.width - 8) col = s.width - 8;
+        off = PARTS == 2 ? split_at(col) : col * 2;
+    }
+    __device__ __forceinline__ void issue(const Side& s, int64_t k, char* lds) {
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const char* src = storage_row<2>(s, k + row0 + e * 4 * PER) + off;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) to_lds(src + p * 64, lds + (p * 32 + wave * PER + e * 4 * PER) * R * 2);
+        }
+    }
+    __device__ __forceinline__ void tail(const Side& s, int64_t k, int64_t k1, char* lds) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const int row = row0 + e * 4 * PER;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+                v4u x = {0, 0, 0, 0};
+                if (k + row < k1) x = *(const v4u*)(storage_row<2>(s, k + row) + off + p * 64);
+                *(v4u*)(lds + (p * 32 + row) * R * 2 + (lane % CH) * 16) = x;
+            }
+        }
+    }
+    // A block's 16 columns are two chunks; lane (i, c) of it addresses row 8 c + i / 4 and, by offset, the row four on.  (In asm, with its
+    // wait inside: for the builtin the compiler waits for every load to LDS that is on its way.)
+    template <class F, int N>
+    static __device__ __forceinline__ void frags(F (&out)[N], const char* lds, int part, int block, int lane) {
+        static_assert(N == 2 || N == 4, "");
+        const int i = lane & 15, row = (lane >> 4) * 8 + (i >> 2);
+        const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds + (part * 32 + row) * R * 2 + (i & 1) * 8;
+        uint32_t x[N];
+        v2u h[2 * N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = at + ((((block + j) * 2 + ((i & 3) >> 1)) ^ swz(row)) << 4);
+        if constexpr (N == 4)
+            asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+                         "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+                         "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+                         "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+                         : "=&v"(h[0]), "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3]), "=&v"(h[4]), "=&v"(h[5]), "=&v"(h[6]), "=&v"(h[7])
+                         : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "n"(8 * R) : "memory");
+        else
+            asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+                         "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
+                         : "=&v"(h[0]), "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3]) : "v"(x[0]), "v"(x[1]), "n"(8 * R) : "memory");
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            union { F f; v2u w[2]; } u;
+            u.w[0] = h[2 * j];
+            u.w[1] = h[2 * j + 1];
+            out[j] = u.f;
+        }
+    }
+};
+
 struct GemmArgs {
     Side a, b;
     int64_t k;
@@ -292,12 +418,84 @@ struct Cfg {
     typedef LA_ LA;
     typedef LB_ LB;
     static constexpr int PA = PA_, PB = PB_, KEEP = KEEP_, TM = TM_, TN = TN_, NKB = NKB_, DEPTH = DEPTH_, LBUF = LBUF_, FROM = FROM_;
-    static constexpr bool F16 = F16_, OUT_BF16 = OUT_BF16_;
+    static constexpr bool F16 = F16_, OUT_BF16 = OUT_BF16_, DMA = false, SCORES = LA::KC && LB::KC;
     static constexpr int LDS = LBUF * (PA * TM + PB * TN) * NKB * 64;
 };
 
 // every wave's LDS accesses are done, and its loads from memory still on their way
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// A tile's results: stored, and (the scores' product) the statistics of its rows.
+template <class C, class LA, class LB, class ACC, class LOW>
+__device__ __forceinline__ void finish(const GemmArgs& g, int tm, int tn, int sp, const ACC& acc, const LOW& low) {
+    constexpr int WM = C::TM / 32, WN = C::TN / 32;
+    constexpr bool TWO = C::KEEP > 1;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, h = lane >> 4, wm = wave & 1, wn = wave >> 1;
+    const float f = g.scale * (g.splits == 1 && g.f0 ? factor_of(g.f0, g.f1, g.f2) : 1.f);
+    constexpr bool PAIR = LB::tile_index(16) == 1;               // a lane's blocks j and j + 1 hold neighbouring columns
+    auto value = [&](int i, int j, int r) {
+        float v = acc[i][j][r];
+        if constexpr (TWO) v = C::F16 ? fmaf(low[i][j][r], 0x1p-11f, v) : v + low[i][j][r];
+        return v * f;
+    };
+    // columns n, n + 1 of row m: g.b.rows is even, or the row goes on
+    auto put_pair = [&](int64_t m, int64_t n, float a, float b) {
+        if (m >= g.a.rows || n >= g.b.rows) return;
+        if (C::OUT_BF16 && g.splits == 1) *(uint32_t*)((uint16_t*)g.out + m * g.ldo + n) = f32_to_bf16_bits(a) | f32_to_bf16_bits(b) << 16;
+        else *(v2f*)((float*)g.out + sp * g.slab + m * g.ldo + n) = v2f{a, b};
+    };
+#pragma unroll
+    for (int i = 0; i < WM; ++i)
+#pragma unroll
+        for (int j = 0; j < WN; j += PAIR ? 2 : 1) {
+            const int64_t n = (int64_t)tn * C::TN + LB::tile_index((wn * WN + j) * 16 + l15);
+            if constexpr (PAIR) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int64_t m = (int64_t)tm * C::TM + LA::tile_index((wm * WM + i) * 16 + 4 * h + r);
+                    put_pair(m, n, value(i, j, r), value(i, j + 1, r));
+                }
+            } else {
+                // two rows at a time, so that a lane stores two neighbouring columns: an even lane takes row r with its neighbour's
+                // column, an odd one row r + 1
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    const float x = value(i, j, r), y = value(i, j, r + 1);
+                    const float px = __int_as_float(dpp16<0xB1>(__float_as_int(x))), py = __int_as_float(dpp16<0xB1>(__float_as_int(y)));
+                    const bool odd = lane & 1;
+                    const int64_t m = (int64_t)tm * C::TM + LA::tile_index((wm * WM + i) * 16 + 4 * h + r) + (odd ? 1 : 0);
+                    put_pair(m, odd ? n - 1 : n, odd ? py : x, odd ? y : px);
+                }
+            }
+        }
+    if constexpr (C::SCORES)
+        if (g.seg) {
+            // the logits are written; this wave's WN * 16 columns of each row: maximum, sum of exp, first column of the maximum
+            const float inv = __fdiv_rn(1.f, g.f2[0]);
+#pragma unroll
+            for (int i = 0; i < WM; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int64_t m = (int64_t)tm * C::TM + (wm * WM + i) * 16 + 4 * h + r;
+                    float z[WN], mx = -INFINITY, se = 0.f;
+                    int am = INT32_MAX;
+#pragma unroll
+                    for (int j = 0; j < WN; ++j) {
+                        const int64_t n = (int64_t)tn * C::TN + (wn * WN + j) * 16 + l15;
+                        z[j] = n < g.b.rows ? value(i, j, r) * inv : -INFINITY;
+                        if (z[j] > mx) { mx = z[j]; am = (int)n; }
+                        if (z[j] != z[j]) se = z[j];             // a NaN stays one whatever the maximum is
+                    }
+                    const float top = max16(mx);
+                    am = min16(mx == top ? am : INT32_MAX);
+                    if (top > -INFINITY)
+#pragma unroll
+                        for (int j = 0; j < WN; ++j) se += exp_neg(z[j] - top);
+                    se = sum16(se);
+                    if (l15 == 0 && m < g.a.rows) *(v4f*)(g.seg + (m * g.segs + tn * 2 + wn) * 4) = v4f{top, se, __int_as_float(am), 0.f};
+                }
+        }
+}
 
 template <class C>
 __device__ __forceinline__ bool gemm_tile(const GemmArgs& g, int item, char* smem) {
@@ -401,64 +599,92 @@ __device__ __forceinline__ bool gemm_tile(const GemmArgs& g, int item, char* sme
             else fetch(next, st + 1 + C::DEPTH);
         }
     }
-    const float f = g.scale * (g.splits == 1 && g.f0 ? factor_of(g.f0, g.f1, g.f2) : 1.f);
-    constexpr bool PAIR = C::LB::tile_index(16) == 1;            // a lane's blocks j and j + 1 hold neighbouring columns
+    finish<C, typename C::LA, typename C::LB>(g, tm, tn, sp, acc, low);
+    const bool out_a = A.outside(), out_b = B.outside();
+    return out_a || out_b;
+}
+
+// The same product where neither side needs a conversion: three LDS buffers of a stage, two stages on their way while one is
+// multiplied.  A wave waits for its own part of a stage by count (the stage after it may still be out), then for the others.
+struct Straight { static __host__ __device__ constexpr int tile_index(int r) { return r; } };
+template <class DA_, class DB_, int PA_, int PB_, int KEEP_, int TM_, int TN_, bool F16_, bool OUT_BF16_>
+struct CfgDma {
+    typedef DA_ DA;
+    typedef DB_ DB;
+    static constexpr int PA = PA_, PB = PB_, KEEP = KEEP_, TM = TM_, TN = TN_, BUF = DA::BYTES + DB::BYTES, LDS = 3 * BUF, LOADS = DA::LOADS + DB::LOADS;
+    static constexpr bool F16 = F16_, OUT_BF16 = OUT_BF16_, DMA = true, SCORES = DA::KC && DB::KC;
+};
+
+template <class C>
+__device__ __forceinline__ bool gemm_straight(const GemmArgs& g, int item, char* smem) {
+    constexpr int WM = C::TM / 32, WN = C::TN / 32;
+    constexpr bool TWO = C::KEEP > 1;
+    typedef typename std::conditional<C::F16, v8h, v8bf>::type frag_t;
+    const int per = g.nm * g.splits, tn = item / per, inner = item % per;
+    const int tm = inner % g.nm, sp = inner / g.nm;
+    const int64_t k0 = sp * g.kstep, k1 = min(g.k, k0 + g.kstep);
+    const int ns = k1 > k0 ? (int)((k1 - k0 + 31) / 32) : 0, nfull = k1 > k0 ? (int)((k1 - k0) / 32) : 0;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
+    typename C::DA A;
+    typename C::DB B;
+    A.init(g.a, (int64_t)tm * C::TM, threadIdx.x);
+    B.init(g.b, (int64_t)tn * C::TN, threadIdx.x);
+    v4f acc[WM][WN], low[TWO ? WM : 1][TWO ? WN : 1];
 #pragma unroll
     for (int i = 0; i < WM; ++i)
 #pragma unroll
-        for (int j = 0; j < WN; j += PAIR ? 2 : 1) {
-            const int64_t n = (int64_t)tn * C::TN + C::LB::tile_index((wn * WN + j) * 16 + l15);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t m = (int64_t)tm * C::TM + C::LA::tile_index((wm * WM + i) * 16 + 4 * h + r);
-                float v[PAIR ? 2 : 1];
-#pragma unroll
-                for (int c = 0; c < (PAIR ? 2 : 1); ++c) {
-                    v[c] = acc[i][j + c][r];
-                    if constexpr (TWO) v[c] = C::F16 ? fmaf(low[i][j + c][r], 0x1p-11f, v[c]) : v[c] + low[i][j + c][r];
-                    v[c] *= f;
-                }
-                if (m >= g.a.rows || n >= g.b.rows) continue;
-                if constexpr (PAIR) {                            // b.rows (d) is even
-                    if (C::OUT_BF16 && g.splits == 1) *(uint32_t*)((uint16_t*)g.out + m * g.ldo + n) = f32_to_bf16_bits(v[0]) | f32_to_bf16_bits(v[1]) << 16;
-                    else *(v2f*)((float*)g.out + sp * g.slab + m * g.ldo + n) = v2f{v[0], v[1]};
-                } else {
-                    if (C::OUT_BF16 && g.splits == 1) ((uint16_t*)g.out)[m * g.ldo + n] = (uint16_t)f32_to_bf16_bits(v[0]);
-                    else ((float*)g.out)[sp * g.slab + m * g.ldo + n] = v[0];
-                }
-            }
+        for (int j = 0; j < WN; ++j) {
+            acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+            if constexpr (TWO) low[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
         }
-    if constexpr (!PAIR)                                         // (the scores' product)
-        if (g.seg) {
-            // the logits are written; this wave's WN * 16 columns of each row: maximum, sum of exp, first column of the maximum
-            const float inv = __fdiv_rn(1.f, g.f2[0]);
+    auto bring = [&](int st, int buf) {
+        char* la = smem + buf * C::BUF;
+        const int64_t k = k0 + (int64_t)st * 32;
+        if (st < nfull) {
+            A.issue(g.a, k, la);
+            B.issue(g.b, k, la + C::DA::BYTES);
+        } else if (st < ns) {
+            A.tail(g.a, k, k1, la);
+            B.tail(g.b, k, k1, la + C::DA::BYTES);
+        }
+    };
+    bring(0, 0);
+    bring(1, 1);
+    int buf = 0;
+    for (int st = 0; st < ns; ++st) {
+        if (st + 1 < nfull) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::LOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        lds_barrier();
+        bring(st + 2, buf == 0 ? 2 : buf - 1);                    // the buffer that every wave has done with
+        const char* la = smem + buf * C::BUF;
+        const char* lb = la + C::DA::BYTES;
+        frag_t fa[C::PA][WM], fb[C::PB][WN];
+#pragma unroll
+        for (int p = 0; p < C::PB; ++p) C::DB::frags(fb[p], lb, p, wn * WN, lane);
+#pragma unroll
+        for (int pa = 0; pa < C::PA; ++pa) {
+            C::DA::frags(fa[pa], la, pa, wm * WM, lane);
 #pragma unroll
             for (int i = 0; i < WM; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int64_t m = (int64_t)tm * C::TM + (wm * WM + i) * 16 + 4 * h + r;
-                    float z[WN], mx = -INFINITY, se = 0.f;
-                    int am = INT32_MAX;
+                for (int pb = 0; pb < C::PB; ++pb)
+                    if (pa + pb < C::KEEP)
 #pragma unroll
-                    for (int j = 0; j < WN; ++j) {
-                        const int64_t n = (int64_t)tn * C::TN + (wn * WN + j) * 16 + l15;
-                        z[j] = acc[i][j][r];
-                        if constexpr (TWO) z[j] = C::F16 ? fmaf(low[i][j][r], 0x1p-11f, z[j]) : z[j] + low[i][j][r];
-                        z[j] = n < g.b.rows ? z[j] * f * inv : -INFINITY;
-                        if (z[j] > mx) { mx = z[j]; am = (int)n; }
-                        if (z[j] != z[j]) se = z[j];             // a NaN stays one whatever the maximum is
-                    }
-                    const float top = max16(mx);
-                    am = min16(mx == top ? am : INT32_MAX);
-                    if (top > -INFINITY)
-#pragma unroll
-                        for (int j = 0; j < WN; ++j) se += exp_neg(z[j] - top);
-                    se = sum16(se);
-                    if (l15 == 0 && m < g.a.rows) *(v4f*)(g.seg + (m * g.segs + tn * 2 + wn) * 4) = v4f{top, se, __int_as_float(am), 0.f};
-                }
+                        for (int j = 0; j < WN; ++j) {
+                            v4f& c = pa + pb == 0 ? acc[i][j] : low[TWO ? i : 0][TWO ? j : 0];
+                            if constexpr (C::F16) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[pa][i], fb[pb][j], c, 0, 0, 0);
+                            else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[pa][i], fb[pb][j], c, 0, 0, 0);
+                        }
         }
-    const bool out_a = A.outside(), out_b = B.outside();
-    return out_a || out_b;
+        buf = buf == 2 ? 0 : buf + 1;
+    }
+    finish<C, Straight, Straight>(g, tm, tn, sp, acc, low);
+    return false;
+}
+template <class C>
+__device__ __forceinline__ bool gemm_any(const GemmArgs& g, int item, char* smem) {
+    if constexpr (C::DMA) return gemm_straight<C>(g, item, smem);
+    else return gemm_tile<C>(g, item, smem);
 }
 
 // an XCD (every eighth id) takes a run of neighbouring tiles, those of one n tile and split next to each other, so that the larger
@@ -477,7 +703,7 @@ __global__ __launch_bounds__(256, 2) void distill_scores_kernel(const GemmArgs g
     bool bad = false;
     if (raise && blockIdx.x == 0)
         for (int64_t i = threadIdx.x; i < nrows_out; i += 256) bad |= rows_out[i] != 0u;
-    if (item < n) bad |= gemm_tile<C>(g, item, smem_raw);
+    if (item < n) bad |= gemm_any<C>(g, item, smem_raw);
     if (raise && bad) __hip_atomic_store(raise, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
@@ -488,10 +714,10 @@ __global__ __launch_bounds__(256, 2) void distill_grads_kernel(const GemmArgs gq
     if (flag && *flag != run_if) return;
     if ((int)blockIdx.x < n0) {
         const int n = gq.nn * gq.nm * gq.splits, item = item_of(blockIdx.x, n);
-        if (item < n) gemm_tile<CQ>(gq, item, smem_raw);
+        if (item < n) gemm_any<CQ>(gq, item, smem_raw);
     } else {
         const int n = gp.nn * gp.nm * gp.splits, item = item_of(blockIdx.x - n0, n);
-        if (item < n) gemm_tile<CP>(gp, item, smem_raw);
+        if (item < n) gemm_any<CP>(gp, item, smem_raw);
     }
 }
 
@@ -1020,29 +1246,35 @@ static GemmArgs gemm_args(const Side& a, const Side& b, int64_t k, const Plan& p
 }
 static unsigned groups_of(const GemmArgs& g) { return (unsigned)(((int64_t)g.nn * g.nm * g.splits + 7) / 8 * 8); }
 
+// dynamic LDS past 64 KB has to be asked for, of the current device's copy of the kernel
+static void allow_lds(const void* kernel, size_t lds) {
+    if (lds > 65536) (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);   // a refusal shows at the launch
+}
 template <class C>
 static void launch_scores(const GemmArgs& g, const unsigned* flag, unsigned run_if, unsigned* raise, const unsigned* rows_out, int64_t B,
                           unsigned* clear, int nclear, hipStream_t st) {
+    allow_lds((const void*)distill_scores_kernel<C>, C::LDS);
     hipLaunchKernelGGL((distill_scores_kernel<C>), dim3(groups_of(g)), dim3(256), C::LDS, st, g, flag, run_if, raise, rows_out, B, clear, nclear);
 }
 template <class CQ, class CP>
 static void launch_grads(const GemmArgs& gq, const GemmArgs& gp, bool dq, bool dp, const unsigned* flag, unsigned run_if, hipStream_t st) {
     const unsigned n0 = dq ? groups_of(gq) : 0, n1 = dp ? groups_of(gp) : 0;
     const size_t lds = (size_t)(CQ::LDS > CP::LDS ? CQ::LDS : CP::LDS);
+    allow_lds((const void*)distill_grads_kernel<CQ, CP>, lds);
     hipLaunchKernelGGL((distill_grads_kernel<CQ, CP>), dim3(n0 + n1), dim3(256), lds, st, gq, gp, (int)n0, flag, run_if);
 }
 
 // s: bf16; fp32 by three bf16 parts (128 / 64 wide tiles); fp32 by two fp16 parts (the queries' are ready)
-typedef Cfg<LoadKC<RAW, 1, 128, 2, 1>, LoadKC<RAW, 1, 128, 2, 1>, 1, 1, 1, 128, 128, 2, 1, 2, 0, false, false> ScoresB128;
-typedef Cfg<LoadKC<RAW, 1, 64, 2, 2>, LoadKC<RAW, 1, 64, 2, 2>, 1, 1, 1, 64, 64, 2, 2, 2, 0, false, false> ScoresB64;
+typedef CfgDma<DmaKC<1, 128>, DmaKC<1, 128>, 1, 1, 1, 128, 128, false, false> ScoresB128;
+typedef CfgDma<DmaKC<1, 64>, DmaKC<1, 64>, 1, 1, 1, 64, 64, false, false> ScoresB64;
 typedef Cfg<LoadKC<SPLIT_B3, 3, 128, 1, 1>, LoadKC<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, 0, false, false> ScoresF128;
 typedef Cfg<LoadKC<SPLIT_B3, 3, 64, 1, 3>, LoadKC<SPLIT_B3, 3, 64, 1, 3>, 3, 3, 3, 64, 64, 1, 3, 2, 1, false, false> ScoresF64;
 typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKC<SPLIT_H2, 2, 128, 1, 1, true>, 2, 2, 2, 128, 128, 1, 1, 2, 3, true, false> ScoresH128;
 // dq = g cand, dc = g^T q
-typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKS<RAW, 1, 128, 1, 1>, 2, 1, 2, 128, 128, 1, 1, 2, 1, false, true> GradQB128;
-typedef Cfg<LoadKS<RAW, 2, 128, 1, 1>, LoadKS<RAW, 1, 128, 1, 1>, 2, 1, 2, 128, 128, 1, 1, 2, 1, false, true> GradPB128;
-typedef Cfg<LoadKC<RAW, 2, 64, 2, 2>, LoadKS<RAW, 1, 64, 2, 2>, 2, 1, 2, 64, 64, 2, 2, 2, 1, false, true> GradQB64;
-typedef Cfg<LoadKS<RAW, 2, 64, 2, 2>, LoadKS<RAW, 1, 64, 2, 2>, 2, 1, 2, 64, 64, 2, 2, 2, 1, false, true> GradPB64;
+typedef CfgDma<DmaKC<2, 128>, DmaKS<1, 128>, 2, 1, 2, 128, 128, false, true> GradQB128;
+typedef CfgDma<DmaKS<2, 128>, DmaKS<1, 128>, 2, 1, 2, 128, 128, false, true> GradPB128;
+typedef CfgDma<DmaKC<2, 64>, DmaKS<1, 64>, 2, 1, 2, 64, 64, false, true> GradQB64;
+typedef CfgDma<DmaKS<2, 64>, DmaKS<1, 64>, 2, 1, 2, 64, 64, false, true> GradPB64;
 typedef Cfg<LoadKC<SPLIT_B3, 3, 128, 1, 1>, LoadKS<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, 0, false, false> GradQF128;
 typedef Cfg<LoadKS<SPLIT_B3, 3, 128, 1, 1>, LoadKS<SPLIT_B3, 3, 128, 1, 1>, 3, 3, 3, 128, 128, 1, 1, 1, 0, false, false> GradPF128;
 typedef Cfg<LoadKC<SPLIT_B3, 3, 64, 1, 2>, LoadKS<SPLIT_B3, 3, 64, 1, 2>, 3, 3, 3, 64, 64, 1, 2, 2, 1, false, false> GradQF64;
@@ -1067,7 +1299,7 @@ extern "C" int abc_distill_fwd(int dtype, const void* q, const void* p, const vo
     unsigned* cnt = (unsigned*)(w + L.off_cnt);
     unsigned* flag = (unsigned*)(w + L.off_flag);
     const int nc = (int)(B + 1 + (B + 31) / 32);
-    const Side sq{q, q, B, d, B}, sc{p, memory, C, d, T};
+    const Side sq{q, q, B, d, B, d}, sc{p, memory, C, d, T, d};
     GemmArgs g = gemm_args(sq, sc, d, L.s, w, L.lds, B * L.lds);
     const bool ready = L.s.splits == 1;
     if (ready) { g.seg = (float*)(w + L.off_seg); g.segs = L.segs; g.f2 = temp; }
@@ -1078,7 +1310,7 @@ extern "C" int abc_distill_fwd(int dtype, const void* q, const void* p, const vo
         unsigned* qout = (unsigned*)(w + L.off_qout);
         hipLaunchKernelGGL(distill_split_kernel, dim3((unsigned)B), dim3(256), 0, st, (const float*)q, d, (d + 31) / 32 * 32, w + L.off_q, qout, flag);
         GemmArgs h = g;
-        h.a = Side{w + L.off_q, w + L.off_q, B, (d + 31) / 32 * 64, B};
+        h.a = Side{w + L.off_q, w + L.off_q, B, (d + 31) / 32 * 64, B, (d + 31) / 32 * 32};
         launch_scores<ScoresH128>(h, nullptr, 0, flag, qout, B, cnt, nc, st);
         launch_scores<ScoresF128>(g, flag, 1, nullptr, nullptr, 0, nullptr, 0, st);
     } else if (L.s.tile == 128) launch_scores<ScoresF128>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
@@ -1122,9 +1354,9 @@ extern "C" int abc_distill_bwd(int dtype, const void* q, const void* p, const vo
     hipLaunchKernelGGL(distill_grad_kernel, dim3((unsigned)L.segs, (unsigned)B), dim3(256), 0, st, a);
     SumArgs sa = {};
     if (dq || dp) {
-        const Side gq{a.g, a.g, B, L.ldg, B}, gp{a.g, a.g, B, L.ldg, C};                       // fp32
-        const Side hq{a.g, a.g, B, L.ldg * 2, B}, hp{a.g, a.g, B, L.ldg * 2, C};               // two parts
-        const Side cand{p, memory, C, d, d}, query{q, q, B, d, d};
+        const Side gq{a.g, a.g, B, L.ldg, B, L.ldg}, gp{a.g, a.g, B, L.ldg, C, L.ldg};                       // fp32
+        const Side hq{a.g, a.g, B, L.ldg * 2, B, L.ldg}, hp{a.g, a.g, B, L.ldg * 2, C, L.ldg};               // two parts
+        const Side cand{p, memory, C, d, d, d}, query{q, q, B, d, d, d};
         GemmArgs xq = gemm_args(gq, cand, T, L.q, L.q.splits > 1 ? (void*)(w + L.off_pq) : dq, d, B * d);
         GemmArgs xp = gemm_args(gp, query, B, L.p, L.p.splits > 1 ? (void*)(w + L.off_pp) : dp, d, C * d);
         for (GemmArgs* x : {&xq, &xp}) { x->f0 = grad_out; x->f1 = stat; x->f2 = temp; }
@@ -1138,7 +1370,7 @@ extern "C" int abc_distill_bwd(int dtype, const void* q, const void* p, const vo
             yq.scale = yp.scale = 1.0f / G_SCALE;
             yq.a = hq;
             yp.a = hp;
-            yp.b = Side{f + F.off_q, f + F.off_q, B, (d + 31) / 32 * 64, d};
+            yp.b = Side{f + F.off_q, f + F.off_q, B, (d + 31) / 32 * 64, d, (d + 31) / 32 * 32};
             launch_grads<GradQH128, GradPH128>(yq, yp, dq, dp, flag, 0, st);
             launch_grads<GradQF128, GradPF128>(xq, xp, dq, dp, flag, 1, st);
         } else if (L.q.tile == 128) launch_grads<GradQF128, GradPF128>(xq, xp, dq, dp, nullptr, 0, st);
