@@ -255,45 +255,45 @@ __device__ __forceinline__ void to_lds(const char* src, char* lds) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 
-// rows in LDS as LoadKC leaves them; a fragment is one 16-byte read
+// Rows of a stage are one cache line, 128 bytes: 64 values, or 32 in two parts.  Their eight chunks of 16 bytes are permuted with the
+// row (chunk ^ row / 2), which keeps the 16 lanes of a read's phase in different banks; a fragment is one 16-byte read.
 template <int PARTS, int R>
 struct DmaKC {
     static constexpr bool KC = true;
-    static constexpr int LOADS = PARTS * R / 64, BYTES = PARTS * R * 64;
-    const char* at[R / 64];
+    static constexpr int KB = 2 / PARTS, BYTES = R * 128, ROW = 64 * 2;   // KB: blocks of 32 values a stage
+    const char* at[R / 32];
     int chunk, row0, wave;
     __device__ __forceinline__ void init(const Side& s, int64_t r0, int tid) {
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int lane = tid & 63;
+        row0 = wave * 8 + (lane >> 3);
+        chunk = (lane ^ (row0 >> 1)) & 7;                         // (32 rows on, the same)
 #pragma unroll
-        for (int i = 0; i < R / 64; ++i) {
-            row0 = wave * 16 + (lane >> 2);
-            chunk = (lane ^ (0 - (row0 >> 2))) & 3;               // what lds_at puts there (64 rows on, the same)
-            const int64_t r = r0 + row0 + i * 64;
+        for (int i = 0; i < R / 32; ++i) {
+            const int64_t r = r0 + row0 + i * 32;
             at[i] = storage_row<2>(s, r < s.rows ? r : s.rows - 1) + chunk * 16;
         }
     }
     __device__ __forceinline__ void issue(const Side&, int64_t k, char* lds) {
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-            for (int i = 0; i < R / 64; ++i) to_lds(at[i] + k * (PARTS == 2 ? 4 : 2) + p * 64, lds + ((p * R + i * 64 + wave * 16) << 6));
+        for (int i = 0; i < R / 32; ++i) to_lds(at[i] + k * (2 * PARTS), lds + (i * 32 + wave * 8) * ROW);
     }
     __device__ __forceinline__ void tail(const Side&, int64_t k, int64_t k1, char* lds) {
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-            for (int i = 0; i < R / 64; ++i) {
-                v4u x = {0, 0, 0, 0};
-                if (k + chunk * 8 < k1) x = *(const v4u*)(at[i] + k * (PARTS == 2 ? 4 : 2) + p * 64);
-                *(v4u*)(lds + lds_at<R, 1>(p, row0 + i * 64, chunk)) = x;
-            }
+        for (int i = 0; i < R / 32; ++i) {
+            v4u x = {0, 0, 0, 0};
+            if (k + (PARTS == 2 ? chunk & 3 : chunk) * 8 < k1) x = *(const v4u*)(at[i] + k * (2 * PARTS));
+            *(v4u*)(lds + (row0 + i * 32) * ROW + ((chunk ^ (row0 >> 1)) & 7) * 16) = x;
+        }
     }
-    // the fragments of N blocks of 16 rows from `block` on
+    // the fragments of N blocks of 16 rows from `block` on; which: the part, or the block of 32 values
     template <class F, int N>
-    static __device__ __forceinline__ void frags(F (&out)[N], const char* lds, int part, int block, int lane) {
+    static __device__ __forceinline__ void frags(F (&out)[N], const char* lds, int which, int block, int lane) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) out[j] = *(const F*)(lds + lds_at<R, 1>(part, (block + j) * 16 + (lane & 15), lane >> 4));
+        for (int j = 0; j < N; ++j) {
+            const int row = (block + j) * 16 + (lane & 15);
+            out[j] = *(const F*)(lds + row * ROW + (((which * 4 + (lane >> 4)) ^ (row >> 1)) & 7) * 16);
+        }
     }
 };
 
@@ -302,7 +302,7 @@ struct DmaKC {
 template <int PARTS, int R>
 struct DmaKS {
     static constexpr bool KC = false;
-    static constexpr int CH = R / 8, PER = 64 / CH, EACH = 32 / PER / 4, LOADS = PARTS * EACH, BYTES = PARTS * R * 64;   // PER: rows an instruction
+    static constexpr int KB = 1, CH = R / 8, PER = 64 / CH, EACH = 32 / PER / 4, LOADS = PARTS * EACH, BYTES = PARTS * R * 64;   // PER: rows an instruction
     int64_t off;
     int row0, wave;
     static __device__ __forceinline__ int swz(int k) {
@@ -604,26 +604,29 @@ __device__ __forceinline__ bool gemm_tile(const GemmArgs& g, int item, char* sme
     return out_a || out_b;
 }
 
-// The same product where neither side needs a conversion: three LDS buffers of a stage, two stages on their way while one is
-// multiplied.  A wave waits for its own part of a stage by count (the stage after it may still be out), then for the others.
+// The same product where neither side needs a conversion: a stage is on its way into one LDS buffer while the other is multiplied,
+// and no register holds it in between.  A third buffer (two stages on their way) leaves one workgroup a CU less and is slower:
+// 512 x 16384 x 3584, scores 112 us for 86, gradients 159 for 155.
 struct Straight { static __host__ __device__ constexpr int tile_index(int r) { return r; } };
 template <class DA_, class DB_, int PA_, int PB_, int KEEP_, int TM_, int TN_, bool F16_, bool OUT_BF16_>
 struct CfgDma {
     typedef DA_ DA;
     typedef DB_ DB;
-    static constexpr int PA = PA_, PB = PB_, KEEP = KEEP_, TM = TM_, TN = TN_, BUF = DA::BYTES + DB::BYTES, LDS = 3 * BUF, LOADS = DA::LOADS + DB::LOADS;
+    static constexpr int PA = PA_, PB = PB_, KEEP = KEEP_, TM = TM_, TN = TN_, BUF = DA::BYTES + DB::BYTES, LDS = 2 * BUF;
+    static constexpr int KB = DA::KB;
     static constexpr bool F16 = F16_, OUT_BF16 = OUT_BF16_, DMA = true, SCORES = DA::KC && DB::KC;
+    static_assert(DA::KB == DB::KB, "");
 };
 
 template <class C>
 __device__ __forceinline__ bool gemm_straight(const GemmArgs& g, int item, char* smem) {
-    constexpr int WM = C::TM / 32, WN = C::TN / 32;
+    constexpr int WM = C::TM / 32, WN = C::TN / 32, STAGE = C::KB * 32;
     constexpr bool TWO = C::KEEP > 1;
     typedef typename std::conditional<C::F16, v8h, v8bf>::type frag_t;
     const int per = g.nm * g.splits, tn = item / per, inner = item % per;
     const int tm = inner % g.nm, sp = inner / g.nm;
     const int64_t k0 = sp * g.kstep, k1 = min(g.k, k0 + g.kstep);
-    const int ns = k1 > k0 ? (int)((k1 - k0 + 31) / 32) : 0, nfull = k1 > k0 ? (int)((k1 - k0) / 32) : 0;
+    const int ns = k1 > k0 ? (int)((k1 - k0 + STAGE - 1) / STAGE) : 0, nfull = k1 > k0 ? (int)((k1 - k0) / STAGE) : 0;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave & 1, wn = wave >> 1;
     typename C::DA A;
     typename C::DB B;
@@ -639,7 +642,7 @@ __device__ __forceinline__ bool gemm_straight(const GemmArgs& g, int item, char*
         }
     auto bring = [&](int st, int buf) {
         char* la = smem + buf * C::BUF;
-        const int64_t k = k0 + (int64_t)st * 32;
+        const int64_t k = k0 + (int64_t)st * STAGE;
         if (st < nfull) {
             A.issue(g.a, k, la);
             B.issue(g.b, k, la + C::DA::BYTES);
@@ -649,34 +652,33 @@ __device__ __forceinline__ bool gemm_straight(const GemmArgs& g, int item, char*
         }
     };
     bring(0, 0);
-    bring(1, 1);
-    int buf = 0;
     for (int st = 0; st < ns; ++st) {
-        if (st + 1 < nfull) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::LOADS) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         lds_barrier();
-        bring(st + 2, buf == 0 ? 2 : buf - 1);                    // the buffer that every wave has done with
-        const char* la = smem + buf * C::BUF;
+        bring(st + 1, (st + 1) & 1);   // into the buffer that every wave has done with
+        const char* la = smem + (st & 1) * C::BUF;
         const char* lb = la + C::DA::BYTES;
-        frag_t fa[C::PA][WM], fb[C::PB][WN];
 #pragma unroll
-        for (int p = 0; p < C::PB; ++p) C::DB::frags(fb[p], lb, p, wn * WN, lane);
+        for (int kb = 0; kb < C::KB; ++kb) {
+            frag_t fa[C::PA][WM], fb[C::PB][WN];
 #pragma unroll
-        for (int pa = 0; pa < C::PA; ++pa) {
-            C::DA::frags(fa[pa], la, pa, wm * WM, lane);
+            for (int p = 0; p < C::PB; ++p) C::DB::frags(fb[p], lb, p + kb, wn * WN, lane);
 #pragma unroll
-            for (int i = 0; i < WM; ++i)
+            for (int pa = 0; pa < C::PA; ++pa) {
+                C::DA::frags(fa[pa], la, pa + kb, wm * WM, lane);
 #pragma unroll
-                for (int pb = 0; pb < C::PB; ++pb)
-                    if (pa + pb < C::KEEP)
+                for (int i = 0; i < WM; ++i)
 #pragma unroll
-                        for (int j = 0; j < WN; ++j) {
-                            v4f& c = pa + pb == 0 ? acc[i][j] : low[TWO ? i : 0][TWO ? j : 0];
-                            if constexpr (C::F16) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[pa][i], fb[pb][j], c, 0, 0, 0);
-                            else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[pa][i], fb[pb][j], c, 0, 0, 0);
-                        }
+                    for (int pb = 0; pb < C::PB; ++pb)
+                        if (pa + pb < C::KEEP)
+#pragma unroll
+                            for (int j = 0; j < WN; ++j) {
+                                v4f& c = pa + pb == 0 ? acc[i][j] : low[TWO ? i : 0][TWO ? j : 0];
+                                if constexpr (C::F16) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[pa][i], fb[pb][j], c, 0, 0, 0);
+                                else c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[pa][i], fb[pb][j], c, 0, 0, 0);
+                            }
+            }
         }
-        buf = buf == 2 ? 0 : buf + 1;
     }
     finish<C, Straight, Straight>(g, tm, tn, sp, acc, low);
     return false;
@@ -1280,7 +1282,7 @@ typedef Cfg<LoadKS<SPLIT_B3, 3, 128, 1, 1>, LoadKS<SPLIT_B3, 3, 128, 1, 1>, 3, 3
 typedef Cfg<LoadKC<SPLIT_B3, 3, 64, 1, 2>, LoadKS<SPLIT_B3, 3, 64, 1, 2>, 3, 3, 3, 64, 64, 1, 2, 2, 1, false, false> GradQF64;
 typedef Cfg<LoadKS<SPLIT_B3, 3, 64, 1, 2>, LoadKS<SPLIT_B3, 3, 64, 1, 2>, 3, 3, 3, 64, 64, 1, 2, 2, 1, false, false> GradPF64;
 typedef Cfg<LoadKC<RAW, 2, 128, 1, 1>, LoadKS<SPLIT_H2, 2, 128, 1, 1>, 2, 2, 2, 128, 128, 1, 1, 2, 1, true, false> GradQH128;
-typedef Cfg<LoadKS<RAW, 2, 128, 1, 1>, LoadKS<RAW, 2, 128, 1, 1>, 2, 2, 2, 128, 128, 1, 1, 2, 1, true, false> GradPH128;
+typedef CfgDma<DmaKS<2, 128>, DmaKS<2, 128>, 2, 2, 2, 128, 128, true, false> GradPH128;
 
 extern "C" int abc_distill_fwd(int dtype, const void* q, const void* p, const void* memory, const float* temp, const int64_t* teacher_idx,
                                const float* teacher_score, float teacher_temp, int64_t B, int64_t C, int64_t M, int d, int k,
