@@ -77,12 +77,14 @@ SHAPES = [(1, 1, 0, 8, 1), (1, 3, 0, 16, 2), (2, 5, 7, 24, 3), (33, 100, 0, 72, 
 
 
 # fp32 products of 8 GFLOP and more go by fp16 parts
-LARGE = [(256, 1000, 15_400, 1024, 40), (520, 2100, 0, 4096, 9)]
+# tiles of 128 and, fp32, of 256 rows of queries; the middle one: of 128 alone, with odd ends on every side
+LARGE = [(256, 1000, 15_400, 1024, 40), (300, 901, 12_000, 1192, 17), (520, 2100, 0, 4096, 9)]
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("shape", LARGE)
-def test_large_fp32(shape):
-    check(*shape, seed=sum(shape))
+def test_large(shape, dtype):
+    check(*shape, seed=sum(shape), dtype=dtype)
 
 
 @pytest.mark.parametrize("what", ["large query", "tiny queries", "large candidate", "tiny memory row", "infinite candidate", "zero rows"])
