@@ -374,16 +374,22 @@ __device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uin
     lo = f32_to_bf16_bits(r - __uint_as_float(mid << 16));
 }
 
-// Memory-bound: dim / 2 bytes of codes and 256 / GROUP bytes of scales a 128 values stream through once, whatever the number of
-// queries up to 16 fp32 (64 bf16).  A wave owns a tile of 16 rows: its lanes load 16 bytes of codes, four conversions a word make a
-// bf16 B fragment of them (e2m1 values are exact in bf16), and 16x16x32 MFMAs multiply it with the queries' fragments out of LDS.
-// fp32 queries stand in LDS as three bf16 parts (24 bits), in rows 4 q + part of the A tile, so that a lane's accumulators hold the
-// parts' sums of one query; products and sums are fp32.  A group's sum is scaled once.  The loads of the next four pieces (the next
-// tile's, at a tile's end) are on their way while four are multiplied: 8 KB a wave, 128 KB a CU.  Scales come 16 bytes a lane, 32 of
-// a row at a time, and go through a strip of LDS of the wave's own (read where they are needed, 2 bytes a lane, they cost a third of the
-// time: every access touches 16 lines).
+// Memory-bound with few queries: dim / 2 bytes of codes and 256 / GROUP bytes of scales a 128 values stream through once, whatever the
+// number of queries up to 16 fp32 (64 bf16).  A wave owns a tile of 16 rows: its lanes load 16 bytes of codes, four conversions a word
+// make a bf16 B fragment of them (e2m1 values are exact in bf16), and 16x16x32 MFMAs multiply it with the queries' fragments out of LDS.
+// fp32 queries stand in LDS as three bf16 parts (24 bits).  Up to four: in rows 4 q + part of one A tile, so that a lane's accumulators
+// hold the parts' sums of one query.  Up to sixteen: a part an A tile, all three into one accumulator, the smallest part first (13
+// queries, 100 003 x 1000: 21 us; four queries a tile, four tiles, reads a third more LDS and spills: 30 us).  Products and sums are
+// fp32.  A group's sum is scaled once.  The loads of the next four pieces (the next tile's, at a tile's end) are on their way while
+// four are multiplied: 8 KB a wave, 128 KB a CU.  Scales come 16 bytes a lane, 32 of a row at a time, and go through a strip of LDS
+// of the wave's own (read where they are needed, 2 bytes a lane, they cost a third of the time: every access touches 16 lines).
+// 1 x 412 500 x 4096: 149 us, 5.8 TB/s.  With more queries the fragments' LDS reads come to bound it: 103 000 x 4096, 1 / 6 / 13 fp32 queries 41 /
+// 69 / 88 us, 16 / 32 / 64 bf16 46 / 75 / 130 us.
 #define SCORE_WAVES 16               // a workgroup: all that a CU holds of this kernel, so that the queries stand in its LDS once
 #define SCORE_STRIP 1280             // bytes of scales a wave: 16 rows of 32, 80 bytes apart
+// between a query part's rows in LDS.  64, with the four 16-byte chunks of a fragment's 64 bytes permuted with the row: a fragment's 16 lanes
+// of a phase ({0-3, 12-15, 20-27}, {4-11, 16-19, 28-31}) touch all banks once
+#define SCORE_PAD(full) ((full) ? 64 : 16)
 
 template <int GROUP>
 struct ScorePieces {
@@ -408,15 +414,17 @@ __device__ __forceinline__ v4u fetch_scales(const uint16_t* scale, int64_t at, i
 template <bool QBF16, int GROUP, int MT>
 __global__ __launch_bounds__(64 * SCORE_WAVES) void store_scores_kernel(const StoreScoreArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
-    constexpr int P = QBF16 ? 1 : 3, G = 128 / GROUP, R = QBF16 ? 4 : 3;    // R: accumulators of a lane that mean something
+    constexpr bool SIDE = !QBF16 && MT == 3;                     // the parts of 16 fp32 queries in A tiles of their own, one accumulator
+    constexpr bool FULL = QBF16 || SIDE;                         // a lane's accumulators hold four queries' scores
+    constexpr int P = QBF16 ? 1 : 3, G = 128 / GROUP, R = FULL ? 4 : 3, NT = SIDE ? 1 : MT;   // R: accumulators of a lane that mean something
     constexpr int EACH = 8 / G;                                  // groups of four pieces that 32 scales of a row serve
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l15 = lane & 15, c = lane >> 4;
     char* strip = smem_raw + wave * SCORE_STRIP;
     char* const qlds = smem_raw + SCORE_WAVES * SCORE_STRIP;
-    const int pitch = a.slice * 256 + 16;                        // bytes a query part
-    const int lrows = a.nq * P;
-    typedef typename std::conditional<QBF16, v4f, float>::type red_t;      // fp32 queries: the parts are summed first
+    const int pitch = a.slice * 256 + SCORE_PAD(FULL);           // bytes a query part
+    const int nq4 = (a.nq + 3) & ~3, lrows = SIDE ? 3 * nq4 : a.nq * P;
+    typedef typename std::conditional<FULL, v4f, float>::type red_t;       // parts in one tile: they are summed first
     red_t* red = (red_t*)(qlds + lrows * pitch);
     const int ks = wave & (a.ks - 1), sub = wave / a.ks, per = SCORE_WAVES / a.ks;
     const int64_t tiles = (a.rows + 15) / 16;
@@ -424,14 +432,14 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void store_scores_kernel(const St
     int arow[MT];                                                // byte offset of this lane's row of each A tile
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        int r;
-        if constexpr (QBF16) { r = t * 16 + l15; if (r >= a.nq) r = a.nq - 1; }
-        else {
+        if constexpr (FULL) {
+            const int qi = min(SIDE ? l15 : t * 16 + l15, a.nq - 1);
+            arow[t] = ((SIDE ? t * nq4 : 0) + qi) * pitch + ((c ^ (0 - (qi >> 2))) & 3) * 16;
+        } else {
             int qi = t * 4 + (l15 >> 2); if (qi >= a.nq) qi = a.nq - 1;
             int part = l15 & 3; if (part > 2) part = 2;
-            r = qi * 3 + part;
+            arow[t] = (qi * 3 + part) * pitch + c * 16;
         }
-        arow[t] = r * pitch + c * 16;
     }
     auto fill = [&](int s) {
         const int c0 = s * a.slice, nc = min(a.slice, a.chunks - c0);
@@ -439,7 +447,8 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void store_scores_kernel(const St
             const int qi = i / (nc * 16), p = i - qi * (nc * 16);
             float v[8];
             load8<QBF16>((const char*)a.q + qi * a.ldq * (QBF16 ? 2 : 4), (c0 * 16 + p) * 8, a.dim, v);
-            char* dst = qlds + qi * P * pitch + p * 16;
+            char* dst = qlds + (SIDE ? qi : qi * P) * pitch + (FULL ? (p & ~3) | ((p ^ (0 - (qi >> 2))) & 3) : p) * 16;
+            const int part = SIDE ? nq4 * pitch : pitch;
             if constexpr (QBF16) {
                 v4u w;
 #pragma unroll
@@ -450,8 +459,8 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void store_scores_kernel(const St
 #pragma unroll
                 for (int j = 0; j < 8; ++j) split3(v[j], h[j], m[j], l[j]);
                 *(v4u*)dst = v4u{h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16};
-                *(v4u*)(dst + pitch) = v4u{m[0] | m[1] << 16, m[2] | m[3] << 16, m[4] | m[5] << 16, m[6] | m[7] << 16};
-                *(v4u*)(dst + 2 * pitch) = v4u{l[0] | l[1] << 16, l[2] | l[3] << 16, l[4] | l[5] << 16, l[6] | l[7] << 16};
+                *(v4u*)(dst + part) = v4u{m[0] | m[1] << 16, m[2] | m[3] << 16, m[4] | m[5] << 16, m[6] | m[7] << 16};
+                *(v4u*)(dst + 2 * part) = v4u{l[0] | l[1] << 16, l[2] | l[3] << 16, l[4] | l[5] << 16, l[6] | l[7] << 16};
             }
         }
     };
@@ -462,7 +471,7 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void store_scores_kernel(const St
     // the waves that share a tile take runs of pieces of a slice
     auto first_of = [&](int c0, int c1, int w) { return c0 + min(c1 - c0, w * ((c1 - c0 + a.ks - 1) / a.ks)); };
 
-    v4f sum[MT];
+    v4f sum[NT];
     ScorePieces<GROUP> cur, next;
     v4u nscale = {0, 0, 0, 0};
     // at: the first piece's place in the queries' LDS; j: the group's place in the strip
@@ -479,40 +488,46 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void store_scores_kernel(const St
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int lbase = at + u * 256;
-            v4f acc[MT];
             if (u >= n) continue;
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                union { v8bf f; v2bf h[4]; } b;
-                b.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cur.code[u][m], 1.0f, 0);
-                b.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cur.code[u][m], 1.0f, 1);
-                b.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cur.code[u][m], 1.0f, 2);
-                b.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cur.code[u][m], 1.0f, 3);
+            for (int group = 0; group < G; ++group) {
+                union { v8bf f; v2bf h[4]; } b[4 / G];
 #pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    if (m % (4 / G) == 0) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
-                    const v8bf av = *(const v8bf*)(qlds + arow[t] + lbase + m * 64);
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, b.f, acc[t], 0, 0, 0);
+                for (int m = 0; m < 4 / G; ++m) {
+                    const uint32_t w = cur.code[u][group * (4 / G) + m];
+                    b[m].h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 0);
+                    b[m].h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 1);
+                    b[m].h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 2);
+                    b[m].h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 3);
                 }
-                if (m % (4 / G) == 4 / G - 1) {
-                    const int k = u * G + m / (4 / G);
-                    const float f = __uint_as_float((k & 1) ? (sc[k / 2] & 0xFFFF0000u) : (sc[k / 2] << 16));
+                const int k = u * G + group;
+                const float f = __uint_as_float((k & 1) ? (sc[k / 2] & 0xFFFF0000u) : (sc[k / 2] << 16));
+                v4f acc;
 #pragma unroll
-                    for (int t = 0; t < MT; ++t)
+                for (int t = MT - 1; t >= 0; --t) {              // SIDE: the smallest parts first, their sum is rounded at the size it has then
+                    if (!SIDE || t == MT - 1) acc = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int r = 0; r < R; ++r) sum[t][r] = fmaf(f, acc[t][r], sum[t][r]);
+                    for (int m = 0; m < 4 / G; ++m) {
+                        const v8bf av = *(const v8bf*)(qlds + arow[t] + lbase + (group * (4 / G) + m) * 64);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, b[m].f, acc, 0, 0, 0);
+                    }
+                    if (!SIDE || t == 0)
+#pragma unroll
+                        for (int r = 0; r < R; ++r) sum[SIDE ? 0 : t][r] = fmaf(f, acc[r], sum[SIDE ? 0 : t][r]);
                 }
+                if (MT > 2 && !SIDE) __builtin_amdgcn_sched_barrier(0);
             }
             __builtin_amdgcn_sched_barrier(0);                   // fragments of one piece at a time: four waves a SIMD hide their reads
         }
     };
 
     const bool whole = nslices == 1;                             // the queries stand in LDS for good
-    const int64_t first0 = (int64_t)blockIdx.x * per, step = (int64_t)gridDim.x * per;
+    const int64_t first0 = blockIdx.x, step = (int64_t)gridDim.x * per;   // neighbouring tiles on different CUs: each gets as many
     if (whole) {
         const int w0 = first_of(0, a.chunks, ks), w1 = first_of(0, a.chunks, ks + 1);
-        if (first0 + sub < tiles && w0 < w1) {
-            const int64_t row = row_of(first0 + sub);
+        const int64_t tile = first0 + (int64_t)sub * gridDim.x;
+        if (tile < tiles && w0 < w1) {
+            const int64_t row = row_of(tile);
             nscale = scales(row, w0);
             next.fetch(data_of(row), w0, w1 - w0);
         }
@@ -521,10 +536,10 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void store_scores_kernel(const St
     }
     // every workgroup makes the same number of rounds for all of its waves: the barriers inside are met by all of them
     for (int64_t first = first0; first < tiles; first += step) {
-        const int64_t tile = first + sub;
+        const int64_t tile = first + (int64_t)sub * gridDim.x;
         const int64_t n = tile * 16 + l15;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) sum[t] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < NT; ++t) sum[t] = v4f{0.f, 0.f, 0.f, 0.f};
         for (int s = 0; s < nslices; ++s) {
             const int c0 = s * a.slice, c1 = min(a.chunks, c0 + a.slice);
             const int e0 = first_of(c0, c1, ks), e1 = first_of(c0, c1, ks + 1);
@@ -556,27 +571,27 @@ __global__ __launch_bounds__(64 * SCORE_WAVES) void store_scores_kernel(const St
                 j = jn;
             }
         }
-        red_t res[MT];
+        red_t res[NT];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            if constexpr (QBF16) res[t] = sum[t];
+        for (int t = 0; t < NT; ++t) {
+            if constexpr (FULL) res[t] = sum[t];
             else res[t] = (sum[t][2] + sum[t][1]) + sum[t][0];
         }
         if (a.ks > 1) {                                          // the waves that share the tile, in fixed order
 #pragma unroll
-            for (int t = 0; t < MT; ++t) red[(wave * MT + t) * 64 + lane] = res[t];
+            for (int t = 0; t < NT; ++t) red[(wave * NT + t) * 64 + lane] = res[t];
             __syncthreads();
             if (ks == 0) {
                 for (int w = 1; w < a.ks; ++w)
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) res[t] += red[((wave + w) * MT + t) * 64 + lane];
+                    for (int t = 0; t < NT; ++t) res[t] += red[((wave + w) * NT + t) * 64 + lane];
             }
             __syncthreads();
         }
         if (ks == 0 && n < a.rows && tile < tiles) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                if constexpr (QBF16) {
+            for (int t = 0; t < NT; ++t) {
+                if constexpr (FULL) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int qi = t * 16 + 4 * c + r;
@@ -603,9 +618,11 @@ static hipError_t scores_launch_mt(const StoreScoreArgs& a, unsigned grid, size_
 template <bool QBF16, int GROUP>
 static hipError_t scores_launch(const StoreScoreArgs& a, int mt, unsigned grid, size_t lds, hipStream_t st) {
     if (mt == 1) return scores_launch_mt<QBF16, GROUP, 1>(a, grid, lds, st);
-    if (mt == 2) return scores_launch_mt<QBF16, GROUP, 2>(a, grid, lds, st);
-    if (mt == 3) return scores_launch_mt<QBF16, GROUP, 3>(a, grid, lds, st);
-    return scores_launch_mt<QBF16, GROUP, 4>(a, grid, lds, st);
+    if constexpr (QBF16) {
+        if (mt == 2) return scores_launch_mt<QBF16, GROUP, 2>(a, grid, lds, st);
+        if (mt == 4) return scores_launch_mt<QBF16, GROUP, 4>(a, grid, lds, st);
+    }
+    return scores_launch_mt<QBF16, GROUP, 3>(a, grid, lds, st);
 }
 
 extern "C" int abc_store_scores(int q_dtype, const void* q, int64_t ldq, int64_t nq, const void* data, const void* scale, int64_t rows,
@@ -622,7 +639,7 @@ extern "C" int abc_store_scores(int q_dtype, const void* q, int64_t ldq, int64_t
         return abc_fail_invalid("store_scores: data must be 16-byte aligned, scale to the scales of 128 values");
     hipStream_t st = (hipStream_t)stream;
     const bool bf = q_dtype == ABC_DT_BF16;
-    const int chunks = (dim + 127) / 128, parts = bf ? 1 : 3, most = bf ? 64 : 16;
+    const int chunks = (dim + 127) / 128, most = bf ? 64 : 16;
     const int64_t passes = (nq + most - 1) / most;
     for (int64_t p = 0; p < passes; ++p) {
         const int64_t q0 = nq * p / passes, q1 = nq * (p + 1) / passes;
@@ -631,19 +648,20 @@ extern "C" int abc_store_scores(int q_dtype, const void* q, int64_t ldq, int64_t
         a.q = (const char*)q + q0 * ldq * (bf ? 2 : 4); a.ldq = ldq;
         a.data = (const char*)data; a.scale = (const uint16_t*)scale; a.rows = rows;
         a.dim = dim; a.chunks = chunks; a.out = out + q0 * ldo; a.ldo = ldo;
-        const int tiles16 = bf ? (a.nq + 15) / 16 : (a.nq + 3) / 4;
-        const int mt = tiles16;
+        const int mt = bf ? (a.nq + 15) / 16 : a.nq <= 4 ? 1 : 3;
+        const bool full = bf || mt == 3;
+        const int lrows = bf ? a.nq : mt == 3 ? (a.nq + 3) / 4 * 12 : a.nq * 3, nt = bf ? mt : 1;
         // LDS: the waves' strips of scales, the queries (in slices of a row where they are too many), the sums of waves that share a tile
         const int64_t tiles = (rows + 15) / 16;
         int slice = 0, ks = 1;
         size_t red = 0;
         auto fit = [&] {                                          // 1 piece at least: 64 rows of 272 bytes fit beside 84 KB
-            slice = (int)((SCORE_LDS - SCORE_WAVES * SCORE_STRIP - red) / (a.nq * parts) - 16) / 256;
+            slice = (int)((SCORE_LDS - SCORE_WAVES * SCORE_STRIP - red) / lrows - SCORE_PAD(full)) / 256;
             if (slice > chunks) slice = chunks;
         };
         fit();
         if (tiles < 2048 && chunks > 1) {
-            red = (size_t)SCORE_WAVES * mt * 64 * (bf ? 16 : 4);
+            red = (size_t)SCORE_WAVES * nt * 64 * (full ? 16 : 4);
             fit();
             while (ks < 8 && tiles * ks < 4096 && ks * 2 <= slice) ks *= 2;
         }
@@ -651,7 +669,7 @@ extern "C" int abc_store_scores(int q_dtype, const void* q, int64_t ldq, int64_t
         a.ks = ks;
         const int64_t wgs = (tiles + SCORE_WAVES / ks - 1) / (SCORE_WAVES / ks);
         const unsigned grid = (unsigned)(wgs < 256 ? wgs : 256);
-        const size_t lds = (size_t)SCORE_WAVES * SCORE_STRIP + (size_t)a.nq * parts * (slice * 256 + 16) + red;
+        const size_t lds = (size_t)SCORE_WAVES * SCORE_STRIP + (size_t)lrows * (slice * 256 + SCORE_PAD(full)) + red;
         hipError_t e;
         if (group == 32) e = bf ? scores_launch<true, 32>(a, mt, grid, lds, st) : scores_launch<false, 32>(a, mt, grid, lds, st);
         else if (group == 64) e = bf ? scores_launch<true, 64>(a, mt, grid, lds, st) : scores_launch<false, 64>(a, mt, grid, lds, st);
