@@ -839,8 +839,11 @@ __device__ __forceinline__ bool arrive_last(unsigned* cnt, unsigned n, unsigned*
 struct Red { float a, b; int c; };
 // maximum, sum and minimum over the workgroup of 256 threads, in one round; fixed order
 __device__ __forceinline__ Red block_red(float mx, float sum, int mn, Red* red) {
+    mx = max16(mx);
+    sum = sum16(sum);
+    mn = min16(mn);
 #pragma unroll
-    for (int m = 32; m > 0; m >>= 1) {
+    for (int m = 16; m < 64; m <<= 1) {
         mx = fmaxf(mx, __shfl_xor(mx, m, 64));
         sum += __shfl_xor(sum, m, 64);
         mn = min(mn, __shfl_xor(mn, m, 64));
@@ -853,10 +856,26 @@ __device__ __forceinline__ Red block_red(float mx, float sum, int mn, Red* red) 
     for (int w = 1; w < 4; ++w) { r.a = fmaxf(r.a, red[w].a); r.b += red[w].b; r.c = min(r.c, red[w].c); }
     return r;
 }
+// three sums over the workgroup at once
+__device__ __forceinline__ void block_sum(float& x, float& y, int& n, Red* red) {
+    x = sum16(x);
+    y = sum16(y);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        if (m >= 16) { x += __shfl_xor(x, m, 64); y += __shfl_xor(y, m, 64); }
+        n += __shfl_xor(n, m, 64);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = Red{x, y, n};
+    __syncthreads();
+    x = (red[0].a + red[1].a) + (red[2].a + red[3].a);
+    y = (red[0].b + red[1].b) + (red[2].b + red[3].b);
+    n = (red[0].c + red[1].c) + (red[2].c + red[3].c);
+}
 
 __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
     __shared__ Red red[4];
-    __shared__ float le[DISTILL_MAX_K];
+    __shared__ __attribute__((aligned(16))) float le[DISTILL_MAX_K];
     __shared__ __attribute__((aligned(16))) int li[DISTILL_MAX_K];
     __shared__ unsigned last;
     const int64_t b = blockIdx.y;
@@ -867,6 +886,33 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
     float mx, se;
     int am;
     bool nan = false;
+    // the teacher's list: entries at[], scores v[], logits z[]; best: the largest score, bad: an entry that makes the row NaN
+    const int64_t* idx = a.idx + b * a.k;
+    const float* score = a.score + b * a.k;
+    float v[4], z[4], best = -INFINITY, bad = 0.f;
+    int at[4], some = 0;
+    auto take_list = [&] {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = tid + u * 256;
+            at[u] = -1;
+            v[u] = -INFINITY;
+            if (i >= a.k) continue;
+            const int64_t j = idx[i];
+            const float x = score[i];
+            if (j >= 0 && !(x == -INFINITY)) {
+                some = 1;
+                if (j >= a.T || !(x < INFINITY)) bad = 1.f;      // a column that is not there, a score that is no number: the row is NaN
+                else { at[u] = (int)j; v[u] = x; best = fmaxf(best, x); }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            z[u] = 0.f;
+            if (at[u] >= 0)
+                for (int p = 0; p < a.splits; ++p) z[u] += part[p * a.slab + at[u]];
+        }
+    };
     if (!a.ready) {
         const int64_t j0 = (int64_t)blockIdx.x * DISTILL_SEG + tid * 4;
         v4f x[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
@@ -918,13 +964,15 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
     if (a.ready) {
         // ---- the product's waves have left a record for each of their stretches of the row
         const v4f* seg = (const v4f*)a.seg + b * a.segs;
-        mx = -INFINITY;
-        for (int i = tid; i < a.segs; i += 256) mx = fmaxf(mx, seg[i][0]);
+        const v4f first = tid < a.segs ? seg[tid] : v4f{-INFINITY, 0.f, __int_as_float(INT32_MAX), 0.f};
+        take_list();                                             // (its loads run beside the records')
+        mx = first[0];
+        for (int i = tid + 256; i < a.segs; i += 256) mx = fmaxf(mx, seg[i][0]);
         mx = block_red(mx, 0.f, 0, red).a;
         se = 0.f;
         am = INT32_MAX;
         for (int i = tid; i < a.segs; i += 256) {
-            const v4f x = seg[i];
+            const v4f x = i == tid ? first : seg[i];
             if (x[0] == mx) am = min(am, __float_as_int(x[2]));
             se += x[0] > -INFINITY ? x[1] * exp_neg(x[0] - mx) : x[1];   // (nothing but NaN there: x[1] is NaN, else 0)
         }
@@ -961,39 +1009,19 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
     }
     float l = nan ? __uint_as_float(0x7FC00000u) : mx + logf(se);
     // ---- the teacher's list: softmax over its entries, the best of them, the row's loss
-    const int64_t* idx = a.idx + b * a.k;
-    const float* score = a.score + b * a.k;
-    float v[4], best = -INFINITY, bad = 0.f;
-    int at[4], some = 0;
+    if (!a.ready) take_list();
+    const int k8 = (a.k + 7) & ~7;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int i = tid + u * 256;
-        at[u] = -1;
-        v[u] = -INFINITY;
-        if (i >= a.k) continue;
-        const int64_t j = idx[i];
-        const float x = score[i];
-        if (j >= 0 && !(x == -INFINITY)) {
-            some = 1;
-            if (j >= a.T || !(x < INFINITY)) bad = 1.f;          // a column that is not there, a score that is no number: the row is NaN
-            else { at[u] = (int)j; v[u] = x; best = fmaxf(best, x); }
-        }
-        li[i] = at[u];
-    }
+    for (int u = 0; u < 4; ++u)
+        if (tid + u * 256 < k8) li[tid + u * 256] = at[u];       // (-1 past the list)
     {
         const Red r = block_red(best, bad, -some, red);
         best = r.a;
         bad = r.b;
         some = -r.c;
     }
-    float z[4];                                                  // on their way while the shares are summed
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        z[u] = 0.f;
-        if (at[u] >= 0)
-            for (int p = 0; p < a.splits; ++p) z[u] += part[p * a.slab + at[u]];
-        z[u] *= inv;
-    }
+    for (int u = 0; u < 4; ++u) z[u] *= inv;
     float e[4], esum = 0.f;
     int first = INT32_MAX;
 #pragma unroll
@@ -1006,7 +1034,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
             if (v[u] == 0.f) first = min(first, i);
         }
         esum += e[u];
-        if (i < a.k) le[i] = e[u];
+        if (i < k8) le[i] = e[u];
     }
     {
         const Red r = block_red(0.f, esum, first, red);
@@ -1025,8 +1053,19 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
         float all = 0.f;
         bool mine = at[u] >= 0 && bad == 0.f;
         if (mine)
-            for (int o = 0; o < a.k; ++o)
-                if (li[o] == at[u]) { mine = mine && o >= i; all += le[o]; }
+            for (int o = 0; o < k8; o += 8) {                    // eight at a time: their reads are one wait
+                int4 l[2];
+                v4f w[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) { l[h] = *(const int4*)(li + o + 4 * h); w[h] = *(const v4f*)(le + o + 4 * h); }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int lo[4] = {l[h].x, l[h].y, l[h].z, l[h].w};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (lo[c] == at[u]) { mine = mine && o + 4 * h + c >= i; all += w[h][c]; }
+                }
+            }
         a.t[b * a.k + i] = mine ? __fdiv_rn(all, esum) : 0.f;
         a.li[b * a.k + i] = mine ? at[u] : -1;
     }
@@ -1051,9 +1090,8 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
         hs += get(a.row + a.B + i);
         ns += get(a.row + 2 * a.B + i) > 0.f ? 1 : 0;
     }
-    ls = block_red(0.f, ls, 0, red).b;
-    hs = block_red(0.f, hs, 0, red).b;
-    const float n = fmaxf(block_red(0.f, (float)ns, 0, red).b, 1.f);
+    block_sum(ls, hs, ns, red);
+    const float n = fmaxf((float)ns, 1.f);
     if (tid == 0) {
         a.out_loss[0] = __fdiv_rn(ls, n);
         a.out_agree[0] = __fdiv_rn(hs, n);
