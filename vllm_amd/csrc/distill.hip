@@ -681,8 +681,10 @@ __device__ __forceinline__ bool gemm_mix(const GemmArgs& g, int item, char* smem
     return B.outside();
 }
 
-// A stage is on its way into one LDS buffer while the other is multiplied, and no register holds it in between.  A third buffer (two
-// stages on their way) leaves one workgroup a CU less and is slower: 512 x 16384 x 3584, scores 112 us for 86, gradients 159 for 155.
+// A stage is on its way into one LDS buffer while the other is multiplied, and no register holds it in between.  512 x 16384 x 3584 in
+// bf16: scores 68 us, gradients 131 us (0.88 and 1.0 PFLOP/s; a large product of a library 1.38).  Measured and left: a third buffer (one
+// workgroup a CU less: 112 and 159 us), wave tiles of 128 x 64, one wave a SIMD, with the fragments' reads and the loads spread among the
+// MFMAs by hand (4 % of the scores' time; the fragments' LDS reads, which bound it, are a quarter less), and the loads alone spread (slower).
 template <class C>
 __device__ __forceinline__ bool gemm_straight(const GemmArgs& g, int item, char* smem) {
     GEMM_BEGIN(C::KB * 32)
@@ -1290,7 +1292,8 @@ static BwdLayout bwd_layout(int64_t B, int64_t C, int64_t T, int d, bool fast, b
             x.nn = (int)((n + tile - 1) / tile);
             int64_t sp = (tile == 128 ? 512 : 1024) / ((int64_t)x.nm * x.nn);
             const int64_t stages = (k + 63) / 64;
-            if (sp > stages / 2) sp = stages / 2;
+            const int64_t most = tile == 128 ? stages / 8 : stages / 2;   // as plan() has it
+            if (sp > most) sp = most;
             if (sp > 32) sp = 32;
             if (sp < 1) sp = 1;
             const int64_t per = (stages + sp - 1) / sp;
