@@ -298,3 +298,15 @@ def test_in_a_captured_graph():
         with pytest.raises(AbcError, match="captured"):
             s.append(x[:2])
         x[:2].add_(0)                                              # a capture of nothing is an error of its own
+
+
+def test_more_rows_than_a_launch_takes():
+    """2^28 rows of 16 threads are 2^32 threads."""
+    n = (1 << 28) + 37
+    s = empty(n + 3, 1, 128)
+    values = (torch.arange(13) - 6).to(torch.bfloat16)[:, None]
+    at = torch.arange(n, device=DEV) % 13
+    s.append(values.to(DEV)[at])
+    got = s.read()
+    want = store_oracle.store_values(values, 128).float().to(DEV)
+    assert torch.equal(got[:n], want[at]) and not got[n:].any()

@@ -88,6 +88,7 @@ struct StoreWriteArgs {
     void* scale;
     const int32_t* claim;           // claim[slot] = the last row that names it (null: the kernel looks through `slots` itself)
     int tx;                         // threads a row (a power of two, 16..256)
+    int64_t row0;                   // first row of this launch
 };
 
 // Rows that name the same slot: the last one is the one that stays, as when the rows are written one after another.
@@ -112,7 +113,7 @@ template <bool BF16, int GROUP>
 __global__ __launch_bounds__(256) void store_write_kernel(const StoreWriteArgs a) {
     __shared__ uint32_t red[4];
     const int tx = a.tx, t = threadIdx.x & (tx - 1);
-    const int64_t row = (int64_t)blockIdx.x * (256 / tx) + threadIdx.x / tx;
+    const int64_t row = a.row0 + (int64_t)blockIdx.x * (256 / tx) + threadIdx.x / tx;
     const bool live = row < a.n;
     int64_t slot = -1;
     if (live) slot = a.slots ? a.slots[row] : (a.first + row) % a.capacity;
@@ -203,11 +204,10 @@ __global__ __launch_bounds__(256) void store_write_kernel(const StoreWriteArgs a
     }
 }
 
-static int store_check(const char* what, int64_t capacity, int dim, int group) {
+static int store_check(int64_t capacity, int dim, int group) {
     if (capacity < 0 || capacity > 0x7FFFFFFFll) return abc_fail_invalid("store: capacity out of range [0, 2^31)");
     if (dim < 1 || dim > STORE_MAX_DIM) return abc_fail_invalid("store: dim out of range [1, 8192]");
     if (group != 0 && group != 32 && group != 64 && group != 128) return abc_fail_invalid("store: group must be 32, 64 or 128 (0 = the 8-bit form)");
-    (void)what;
     return ABC_OK;
 }
 
@@ -217,6 +217,13 @@ static int row_threads(int pieces) {
     return tx;
 }
 
+// A launch has fewer than 2^32 threads: rows a launch, and its workgroups for n rows from row0 on.
+static int64_t rows_a_launch(int tx) { return (int64_t)(1 << 23) * (256 / tx); }
+static unsigned row_groups(int64_t n, int64_t row0, int tx) {
+    const int64_t m = n - row0 < rows_a_launch(tx) ? n - row0 : rows_a_launch(tx);
+    return (unsigned)((m + 256 / tx - 1) / (256 / tx));
+}
+
 extern "C" size_t abc_store_write_workspace_bytes(int64_t n, int64_t capacity) {
     if (n <= STORE_SCAN_MAX || capacity <= 0) return 0;
     return (size_t)capacity * 4;
@@ -224,7 +231,7 @@ extern "C" size_t abc_store_write_workspace_bytes(int64_t n, int64_t capacity) {
 
 extern "C" int abc_store_write(int x_dtype, const void* x, int64_t ldx, const int64_t* slots, int64_t first, int64_t n, int dim,
                                void* data, void* scale, int64_t capacity, int group, void* ws, size_t ws_bytes, void* stream) {
-    int rc = store_check("write", capacity, dim, group);
+    int rc = store_check(capacity, dim, group);
     if (rc) return rc;
     if (x_dtype != ABC_DT_F32 && x_dtype != ABC_DT_BF16) return abc_fail_invalid("store_write: rows must be f32 or bf16");
     if (n < 0 || n > 0x7FFFFFFFll) return abc_fail_invalid("store_write: row count out of range [0, 2^31)");
@@ -247,14 +254,16 @@ extern "C" int abc_store_write(int x_dtype, const void* x, int64_t ldx, const in
         hipLaunchKernelGGL(store_claim_clear_kernel, dim3(g), dim3(256), 0, st, slots, n, capacity, (int32_t*)ws);
         hipLaunchKernelGGL(store_claim_kernel, dim3(g), dim3(256), 0, st, slots, n, capacity, (int32_t*)ws);
     }
-    const unsigned grid = (unsigned)((n + 256 / a.tx - 1) / (256 / a.tx));
     const bool bf = x_dtype == ABC_DT_BF16;
 #define STORE_WRITE(G) do { if (bf) hipLaunchKernelGGL((store_write_kernel<true, G>), dim3(grid), dim3(256), 0, st, a); \
                             else hipLaunchKernelGGL((store_write_kernel<false, G>), dim3(grid), dim3(256), 0, st, a); } while (0)
-    if (group == 0) STORE_WRITE(0);
-    else if (group == 32) STORE_WRITE(32);
-    else if (group == 64) STORE_WRITE(64);
-    else STORE_WRITE(128);
+    for (a.row0 = 0; a.row0 < n; a.row0 += rows_a_launch(a.tx)) {
+        const unsigned grid = row_groups(n, a.row0, a.tx);
+        if (group == 0) STORE_WRITE(0);
+        else if (group == 32) STORE_WRITE(32);
+        else if (group == 64) STORE_WRITE(64);
+        else STORE_WRITE(128);
+    }
 #undef STORE_WRITE
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? ABC_OK : abc_fail_hip(e, "store_write launch");
@@ -269,6 +278,7 @@ struct StoreReadArgs {
     int dim, width, tx;
     void* out;
     int64_t ldo;
+    int64_t row0;                   // first row of this launch
 };
 
 // the 8 fp32 values of one word of e2m1 codes, times s (exact: 2 significant bits times 8)
@@ -282,7 +292,7 @@ __device__ __forceinline__ void fp4_values(uint32_t w, float s, float (&v)[8]) {
 template <bool BF16, int GROUP>
 __global__ __launch_bounds__(256) void store_read_kernel(const StoreReadArgs a) {
     const int tx = a.tx, t = threadIdx.x & (tx - 1);
-    const int64_t i = (int64_t)blockIdx.x * (256 / tx) + threadIdx.x / tx;
+    const int64_t i = a.row0 + (int64_t)blockIdx.x * (256 / tx) + threadIdx.x / tx;
     if (i >= a.n) return;
     const int64_t row = a.index ? a.index[i] : a.first + i;
     char* out = (char*)a.out + i * a.ldo * (BF16 ? 2 : 4);
@@ -320,7 +330,7 @@ __global__ __launch_bounds__(256) void store_read_kernel(const StoreReadArgs a) 
 
 extern "C" int abc_store_read(const int64_t* index, int64_t first, int64_t n, const void* data, const void* scale, int64_t capacity,
                               int dim, int group, int out_dtype, void* out, int64_t ldo, void* stream) {
-    int rc = store_check("read", capacity, dim, group);
+    int rc = store_check(capacity, dim, group);
     if (rc) return rc;
     if (out_dtype != ABC_DT_F32 && out_dtype != ABC_DT_BF16) return abc_fail_invalid("store_read: rows are read as f32 or bf16");
     if (n < 0 || n > 0x7FFFFFFFll) return abc_fail_invalid("store_read: row count out of range [0, 2^31)");
@@ -333,15 +343,17 @@ extern "C" int abc_store_read(const int64_t* index, int64_t first, int64_t n, co
     a.index = index; a.first = first; a.n = n; a.capacity = capacity; a.data = data; a.scale = scale;
     a.dim = dim; a.width = (dim + 127) / 128 * 128; a.out = out; a.ldo = ldo;
     a.tx = row_threads(group ? (dim + 7) / 8 : (dim + 15) / 16);
-    const unsigned grid = (unsigned)((n + 256 / a.tx - 1) / (256 / a.tx));
     hipStream_t st = (hipStream_t)stream;
     const bool bf = out_dtype == ABC_DT_BF16;
 #define STORE_READ(G) do { if (bf) hipLaunchKernelGGL((store_read_kernel<true, G>), dim3(grid), dim3(256), 0, st, a); \
                            else hipLaunchKernelGGL((store_read_kernel<false, G>), dim3(grid), dim3(256), 0, st, a); } while (0)
-    if (group == 0) STORE_READ(0);
-    else if (group == 32) STORE_READ(32);
-    else if (group == 64) STORE_READ(64);
-    else STORE_READ(128);
+    for (a.row0 = 0; a.row0 < n; a.row0 += rows_a_launch(a.tx)) {
+        const unsigned grid = row_groups(n, a.row0, a.tx);
+        if (group == 0) STORE_READ(0);
+        else if (group == 32) STORE_READ(32);
+        else if (group == 64) STORE_READ(64);
+        else STORE_READ(128);
+    }
 #undef STORE_READ
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? ABC_OK : abc_fail_hip(e, "store_read launch");
@@ -627,7 +639,7 @@ static hipError_t scores_launch(const StoreScoreArgs& a, int mt, unsigned grid, 
 
 extern "C" int abc_store_scores(int q_dtype, const void* q, int64_t ldq, int64_t nq, const void* data, const void* scale, int64_t rows,
                                 int dim, int group, float* out, int64_t ldo, void* stream) {
-    int rc = store_check("scores", rows, dim, group);
+    int rc = store_check(rows, dim, group);
     if (rc) return rc;
     if (group == 0) return abc_fail_invalid("store_scores: the 4-bit form only (the 8-bit form is searched by abc_topk_i8)");
     if (q_dtype != ABC_DT_F32 && q_dtype != ABC_DT_BF16) return abc_fail_invalid("store_scores: queries must be f32 or bf16");
