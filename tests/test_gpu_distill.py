@@ -340,6 +340,31 @@ def test_on_another_stream_and_in_captured_graphs():
             assert all(torch.equal(a, b) for a, b in zip(o, want))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_in_a_captured_graph(dtype):
+    """The large products' kernels ask for more LDS than a launch has by itself, also while a graph is captured."""
+    q, p, m, index, score = (x.to(DEV) for x in problem(256, 1000, 15_400, 1024, 40, 3, dtype))
+    leaves = (q.requires_grad_(True), p.requires_grad_(True), torch.tensor(0.07, device=DEV, requires_grad=True))
+
+    def step():
+        loss, agree = call(leaves[0], leaves[1], m, leaves[2], index, score, 0.05)
+        return (loss.detach(), agree) + torch.autograd.grad(loss, leaves)
+
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for i in range(3):
+        with torch.no_grad():
+            leaves[0].mul_(-1)
+            leaves[2].fill_(0.05 + 0.01 * i)
+            if dtype is torch.float32 and i == 1:
+                leaves[1][5] *= 1e6                              # past what the fp16 parts hold: the other kernels run in this replay
+        g.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_a_training_step_over_a_store():
     """As a program uses them together: a teacher's store answers with its best rows, the student's memory of older candidates is read
     back, the loss draws the student towards the teacher's list, the step's candidates enter the memory."""

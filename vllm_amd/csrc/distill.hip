@@ -1312,10 +1312,15 @@ static BwdLayout bwd_layout(int64_t B, int64_t C, int64_t T, int d, bool fast, b
     return L;
 }
 
+#define MAX_TILES ((1 << 24) - 8)     // a launch has fewer than 2^32 threads
+static int64_t tiles_of(int64_t rows, int tile) { return (rows + tile - 1) / tile; }
+
 static int distill_check(int dtype, int64_t B, int64_t C, int64_t M, int d, int k) {
     if (dtype != ABC_DT_F32 && dtype != ABC_DT_BF16) return abc_fail_invalid("distill: embeddings must be f32 or bf16");
     if (B < 1 || C < 1 || M < 0) return abc_fail_invalid("distill: need at least one query and one candidate");
     if (B > 65535 || C > 0x7FFFFFF0ll || M > 0x7FFFFFF0ll || C + M > 0x7FFFFFF0ll) return abc_fail_invalid("distill: at most 65535 queries and 2^31 - 16 candidates");
+    if (tiles_of(C + M, 64) * tiles_of(B, 64) > MAX_TILES || tiles_of(C, 64) * tiles_of(d, 64) > MAX_TILES)
+        return abc_fail_invalid("distill: too many query-candidate pairs for one launch (2^24 tiles of 64 x 64)");
     if (d < 8 || d % 8 || d > 65536) return abc_fail_invalid("distill: d must be a multiple of 8 in [8, 65536]");
     if (k < 1 || k > DISTILL_MAX_K) return abc_fail_invalid("distill: a list has 1 to 1024 entries");
     return ABC_OK;
@@ -1379,7 +1384,6 @@ typedef CfgDma<DmaKS<2, 256, 512>, DmaKS<2, 128, 512>, 2, 2, 256, 128, 512, true
 
 // 256 rows of a side in one tile, by eight waves, instead of two tiles of 128: fp32 values of the other side are read and split half
 // as often (256 x 32768 x 4096: scores 221 us for 249, gradients 294 for 311).  Taken where at most a fifth more rows are computed for it.
-static int64_t tiles_of(int64_t rows, int tile) { return (rows + tile - 1) / tile; }
 static GemmArgs tall(GemmArgs g) {
     g.nm = (int)tiles_of(g.a.rows, 256);
     return g;
