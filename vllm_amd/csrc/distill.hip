@@ -514,7 +514,7 @@ __device__ __forceinline__ void finish(const GemmArgs& g, int tm, int tn, int sp
     constexpr int WM = Waves<C>::WM, WN = Waves<C>::WN, STAGE = STAGE_VALUES; \
     constexpr bool TWO = C::KEEP > 1; \
     typedef typename std::conditional<C::F16, v8h, v8bf>::type frag_t; \
-    const int per = g.nm * g.splits, tn = item / per, inner = item % per, tm = inner % g.nm, sp = inner / g.nm; \
+    const int per = g.nm * g.nn, sp = item / per, inner = item % per, tn = inner / g.nm, tm = inner % g.nm; \
     const int64_t k0 = sp * g.kstep, k1 = min(g.k, k0 + g.kstep); \
     const int ns = (int)((k1 - k0 + STAGE - 1) / STAGE); \
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = Waves<C>::m(wave), wn = Waves<C>::n(wave); \
@@ -739,8 +739,9 @@ __device__ __forceinline__ bool gemm_any(const GemmArgs& g, int item, char* smem
     else return gemm_straight<C>(g, item, smem);
 }
 
-// an XCD (every eighth id) takes a run of neighbouring tiles, those of one n tile and split next to each other, so that the larger
-// operand's values are fetched once into its L2
+// an XCD (every eighth id) takes a run of neighbouring tiles: of one part of k, one n tile's next to each other, so that both operands'
+// values of that part are fetched into one L2 or two (512 x 16384 x 3584 in bf16, a step: 251 us; with an n tile's parts of k next to each
+// other every L2 fetched all of g for each of its n tiles, 0.7 GB in all: 261 us)
 __device__ __forceinline__ int item_of(int id, int n) { return (id & 7) * ((n + 7) >> 3) + (id >> 3); }
 
 // flag: null, or the word that says whether the fp16 parts hold the values; the launch runs where it equals run_if
