@@ -277,7 +277,7 @@ int abc_mean_pool_bwd_f32(const float* dx, const int64_t* ids, int64_t pad_id, c
  *
  * abc_store_write: row i of x goes to slot slots[i], or to (first + i) % capacity where slots is null (n <= capacity then).  A slot
  *   outside [0, capacity) drops its row; of rows that name one slot the last is kept.
- *   workspace >= abc_store_write_workspace_bytes(n, capacity) where slots is given (0 up to 1024 rows).
+ *   workspace >= abc_store_write_workspace_bytes(n, capacity) where slots is given (0 up to 2048 rows).
  * abc_store_read: out[i, :] = the values held by row index[i] (first + i where index is null); index < 0 gives zeros, index >=
  *   capacity NaN.  fp32 products code * scale, rounded once to bf16 where out is bf16.
  * abc_store_scores (fp4): out[i, n] = q[i, :] . (values of row n), n < rows; fp32 sums, fp32 queries at full precision.

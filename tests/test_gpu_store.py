@@ -107,7 +107,7 @@ def test_groups_that_are_not_finite_read_as_nan():
         assert bool(((got.double() - want)[ok].abs() <= 2.0 ** -24 * want[ok].abs()).all())
 
 
-@pytest.mark.parametrize("n", [2, 300, 1024, 1025, 5000])
+@pytest.mark.parametrize("n", [2, 300, 1025, 2048, 2049, 5000])
 @pytest.mark.parametrize("group,dim", [(0, 96), (64, 96), (128, 2048), (0, 2048)])
 def test_the_last_of_rows_that_name_one_slot_stays(n, group, dim):
     cap = 37
@@ -270,7 +270,7 @@ def test_a_store_beyond_32_bit_offsets():
 def test_in_a_captured_graph():
     """Write, read and scores in one graph, replayed on new rows, eager work between the replays."""
     s = empty(64, 384, 32)
-    x, slots, q = rows(1500, 384, 0).to(DEV), torch.zeros(1500, dtype=torch.int64, device=DEV), rows(2, 384, 3).to(DEV)
+    x, slots, q = rows(2500, 384, 0).to(DEV), torch.zeros(2500, dtype=torch.int64, device=DEV), rows(2, 384, 3).to(DEV)
     other = empty(64, 384, 32)
     st = torch.cuda.Stream(DEV)
 
@@ -286,8 +286,8 @@ def test_in_a_captured_graph():
     with torch.cuda.graph(graph):
         got = step(s)
     for i in range(3):
-        x.copy_(rows(1500, 384, 20 + i))
-        slots.copy_(torch.randint(0, 64, (1500,), generator=torch.Generator().manual_seed(i)))
+        x.copy_(rows(2500, 384, 20 + i))
+        slots.copy_(torch.randint(0, 64, (2500,), generator=torch.Generator().manual_seed(i)))
         graph.replay()
         want = step(other)
         torch.cuda.synchronize()

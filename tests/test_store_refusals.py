@@ -32,9 +32,9 @@ def test_write_refuses(bad):
 
 
 def test_write_workspace():
-    assert lib().abc_store_write_workspace_bytes(1024, 10) == 0 and lib().abc_store_write_workspace_bytes(1025, 10) == 40
-    assert write(n=1025) == -2 and b"workspace too small" in lib().abc_last_error()
-    assert write(n=1025, ws=OK, ws_bytes=39) == -2
+    assert lib().abc_store_write_workspace_bytes(2048, 10) == 0 and lib().abc_store_write_workspace_bytes(2049, 10) == 40
+    assert write(n=2049) == -2 and b"workspace too small" in lib().abc_last_error()
+    assert write(n=2049, ws=OK, ws_bytes=39) == -2
     assert write(n=0) == 0 and read(n=0) == 0 and scores(nq=0) == 0 and scores(rows=0) == 0
 
 

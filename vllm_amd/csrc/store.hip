@@ -23,7 +23,9 @@ int abc_fail_ws(size_t need, size_t have);
 
 #define STORE_MAX_DIM 8192
 #define SCORE_LDS 163840              // a workgroup's LDS in the scoring kernel: a CU's
-#define STORE_SCAN_MAX 1024          // writes of up to this many rows look for repeated slots inside the writing kernel
+// writes of up to this many rows look for repeated slots inside the writing kernel (fp4/128, us, with the claims' two launches: 1024 x 4096 6.4 /
+// 9.7, 2048 x 4096 10.8 / 13.7, 4096 x 4096 22 / 21)
+#define STORE_SCAN_MAX 2048
 
 typedef __attribute__((ext_vector_type(8))) __bf16 v8bf;
 typedef __attribute__((ext_vector_type(2))) __bf16 v2bf;
@@ -667,11 +669,13 @@ extern "C" int abc_store_scores(int q_dtype, const void* q, int64_t ldq, int64_t
         const int64_t tiles = (rows + 15) / 16;
         int slice = 0, ks = 1;
         size_t red = 0;
-        auto fit = [&] {                                          // 1 piece at least: 64 rows of 272 bytes fit beside 84 KB
+        auto fit = [&] {                                          // 1 piece at least: 64 rows of 320 bytes fit beside 84 KB
             slice = (int)((SCORE_LDS - SCORE_WAVES * SCORE_STRIP - red) / lrows - SCORE_PAD(full)) / 256;
             if (slice > chunks) slice = chunks;
         };
         fit();
+        // several waves a tile where there are fewer than 2048 (1 x 5000 x 3584: 6.6 us, one wave a tile 16.5; 1 x 30 000: 15.0 and 17.2; beyond, 1 x
+        // 40 000: 17.2, two waves a tile 18.3)
         if (tiles < 2048 && chunks > 1) {
             red = (size_t)SCORE_WAVES * nt * 64 * (full ? 16 : 4);
             fit();
