@@ -1223,18 +1223,29 @@ __global__ __launch_bounds__(256) void distill_sum_kernel(const SumArgs a) {
 // ---- plans ---------------------------------------------------------------------------------------------------------------
 struct Plan { int tile, splits; int64_t kstep; int nm, nn; };
 
-// Tiles of 128 x 128 where two workgroups of them a CU (512) come together, 64 x 64 otherwise (four a CU); k is split until that many
-// workgroups run, as long as a split keeps four stages of 64.
-static Plan plan(int64_t m, int64_t n, int64_t k) {
+// Tiles of 128 x 128 (two workgroups a CU) or 64 x 64 (four), and k in so many parts that the CUs have work.  A tile of 128
+// needs half the operands' reads; tiles of 64 give more workgroups.  The choice goes by the tiles of 128 times the parts of 8 stages that k has
+// (`least`).  Measured, us, 64 / 128:
+//   fp32 scores, from 288      128 x 1024 x 4096 (72) 36 / 45, 256 x 4096 x 1024 (192) 38 / 48, 128 x 4096 x 4096 (288) 50 / 50, 256 x 8192 x 1024 (384) 52 / 50
+//   fp32 gradients, from 128   by the product with the longer k: 128 x 1024 x 4096 (96) 41 / 47, 1000 x 1000 x 1024 (128) 60 / 53,
+//                              256 x 4096 x 1024 (144) 59 / 51, 128 x 4096 x 4096 (288) 100 / 69
+//   bf16, from 64              scores of 128 x 1024 x 4096 (72) 30 / 22, 128 x 8192 x 1024 (192) 28 / 24
+// Tiles of 64: parts until `wgs` workgroups run, 256 for the scores, whose rows' launch adds the slabs up (128 x 1024 x 4096, forward: 27 us, with
+// 1024 35; 64 x 8192 x 1024 in bf16 18 and 27), 1024 for the gradients.
+#define LEAST_SCORES 288
+#define LEAST_GRADS 128
+#define LEAST_BF16 64
+static Plan plan(int64_t m, int64_t n, int64_t k, int least, int wgs) {
     Plan p;
     auto tiles = [&](int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
     const int64_t stages = (k + 63) / 64;
-    p.tile = m > 64 && n > 64 && tiles(128) * (stages / 8 + 1) >= 512 ? 128 : 64;
+    p.tile = m > 64 && n > 64 && tiles(128) * (stages / 8 + 1) >= least ? 128 : 64;
     p.nm = (int)((m + p.tile - 1) / p.tile);
     p.nn = (int)((n + p.tile - 1) / p.tile);
-    int64_t sp = (p.tile == 128 ? 512 : 1024) / ((int64_t)p.nm * p.nn);
+    int64_t sp = (p.tile == 128 ? 512 : wgs) / ((int64_t)p.nm * p.nn);
     const int64_t most = p.tile == 128 ? stages / 8 : stages / 2;
     if (sp > most) sp = most;
+    if (sp > wgs / 16) sp = wgs / 16;
     if (sp > 32) sp = 32;
     if (sp < 1) sp = 1;
     const int64_t per = (stages + sp - 1) / sp;
@@ -1255,10 +1266,11 @@ struct FwdLayout {
 
 static FwdLayout fwd_layout(int dtype, int64_t B, int64_t T, int d, int k) {
     FwdLayout L;
-    L.s = plan(B, T, d);
+    L.s = plan(B, T, d, dtype == ABC_DT_BF16 ? LEAST_BF16 : LEAST_SCORES, 256);
     L.lds = (T + 31) / 32 * 32;
     L.segs = L.s.splits == 1 ? L.s.nn * 2 : (int)((T + DISTILL_SEG - 1) / DISTILL_SEG);
-    // from about 8 GFLOP a product on, half the matrix work is worth the launches that find out and then return
+    // From about 8 GFLOP a product on, half the matrix work is worth the launches that find out and then return (256 x 16 384 x 1024, forward and
+    // backward: 121 us, without 150).
     L.fast = dtype == ABC_DT_F32 && L.s.tile == 128 && 2.0 * (double)B * (double)T * d >= 8e9;
     size_t o = up((size_t)L.s.splits * B * L.lds * 4);
     L.off_s = 0;
@@ -1278,14 +1290,15 @@ static FwdLayout fwd_layout(int dtype, int64_t B, int64_t T, int d, int k) {
 }
 
 struct BwdLayout { Plan q, p; int64_t ldg; int segs; size_t off_g, off_dt, off_pq, off_pp, total; };
-static BwdLayout bwd_layout(int64_t B, int64_t C, int64_t T, int d, bool fast, bool dq, bool dp) {
+static BwdLayout bwd_layout(int dtype, int64_t B, int64_t C, int64_t T, int d, bool fast, bool dq, bool dp) {
+    const int least = dtype == ABC_DT_BF16 ? LEAST_BF16 : LEAST_GRADS;
     BwdLayout L;
     L.ldg = (T + 31) / 32 * 32;                                // as the logits' rows
     L.segs = (int)((L.ldg + DISTILL_SEG - 1) / DISTILL_SEG);
-    L.q = plan(B, d, T);
-    L.p = plan(C, d, B);
+    L.q = plan(B, d, T, least, 1024);
+    L.p = plan(C, d, B, least, 1024);
     if (fast || (L.q.tile == 128) != (L.p.tile == 128)) {         // one launch, one kind of tile: that of the larger product
-        const int tile = fast || (T > C && B > 64 ? L.q.tile : L.p.tile) == 128 ? 128 : 64;
+        const int tile = fast || (T >= B ? L.q.tile : L.p.tile) == 128 ? 128 : 64;
         auto with = [&](Plan& x, int64_t m, int64_t n, int64_t k) {
             if (x.tile == tile) return;
             x.tile = tile;
@@ -1333,7 +1346,7 @@ extern "C" size_t abc_distill_workspace_bytes(int dtype, int64_t B, int64_t C, i
 }
 extern "C" size_t abc_distill_bwd_workspace_bytes(int dtype, int64_t B, int64_t C, int64_t M, int d, int k) {
     if (distill_check(dtype, B, C, M, d, k)) return 0;
-    return bwd_layout(B, C, C + M, d, fwd_layout(dtype, B, C + M, d, k).fast, true, true).total;
+    return bwd_layout(dtype, B, C, C + M, d, fwd_layout(dtype, B, C + M, d, k).fast, true, true).total;
 }
 
 static GemmArgs gemm_args(const Side& a, const Side& b, int64_t k, const Plan& p, void* out, int64_t ldo, int64_t slab) {
@@ -1445,7 +1458,7 @@ extern "C" int abc_distill_bwd(int dtype, const void* q, const void* p, const vo
     const int64_t T = C + M;
     const FwdLayout F = fwd_layout(dtype, B, T, d, k);
     if (fwd_ws_bytes < F.total) return abc_fail_ws(F.total, fwd_ws_bytes);
-    const BwdLayout L = bwd_layout(B, C, T, d, F.fast, dq, dp);
+    const BwdLayout L = bwd_layout(dtype, B, C, T, d, F.fast, dq, dp);
     if (!ws || ws_bytes < L.total) return abc_fail_ws(L.total, ws_bytes);
     if (((uintptr_t)ws | (uintptr_t)fwd_ws) & 15) return abc_fail_invalid("distill_bwd: workspaces must be 16-byte aligned");
     if (!dq && !dp && !d_temp) return ABC_OK;
