@@ -199,7 +199,7 @@ int abc_infonce_bwd(const float* q, const float* p, const float* lse, const floa
  *   t_b = softmax over row b's entries of score / teacher_temp;  row_b = sum_i t_bi (log t_bi - z_b,idx) + logsumexp_j z_bj
  *   out_loss [1] f32: mean of row_b over the rows that have an entry (0 where none has)
  *   out_agree [1] f32: share of those rows whose best candidate (argmax z) is the best entry of the list
- *   B in [1, 65535], d % 8 == 0, d <= 65536, k in [1, 1024].
+ *   B in [1, 65535], d % 8 == 0, d <= 65536, k in [1, 1024]; B x T and C x d at most 2^23 tiles of 64 x 64.
  * abc_distill_bwd: `fwd_ws` is the workspace abc_distill_fwd was given for the same arguments, unchanged since (it is only read:
  *   the backward may run more than once).  dq [B,d], dp [C,d] in dtype, d_temp [1] f32, each nullable (not computed), overwritten;
  *   grad_out is a device scalar.  Rows without an entry receive no gradient.

@@ -22,7 +22,7 @@ def bwd(dtype=F32, q=OK, p=OK, memory=None, temp=OK, go=OK, B=4, C=8, M=0, d=16,
 
 
 SIZES = [dict(dtype=I8), dict(dtype=7), dict(B=0), dict(B=65536), dict(C=0), dict(M=-1), dict(M=1 << 31), dict(d=0), dict(d=12), dict(d=65544),
-         dict(k=0), dict(k=1025), dict(C=1 << 30), dict(B=1, C=1, M=(1 << 30) - 1), dict(B=65, C=1 << 29), dict(C=1 << 25, d=65536)]
+         dict(k=0), dict(k=1025), dict(C=1 << 30), dict(B=1, C=1, M=1 << 29), dict(B=65, C=1 << 29), dict(C=1 << 25, d=65536)]
 
 
 @pytest.mark.parametrize("bad", SIZES)
@@ -38,6 +38,10 @@ def test_sizes_are_refused(bad):
                                  dict(agree=None), dict(q=OK + 8), dict(p=OK + 4), dict(tt=0.0), dict(tt=-1.0), dict(tt=float("nan"))])
 def test_forward_refuses(bad):
     assert fwd(**bad, ws_bytes=1 << 30) == -1 and lib().abc_last_error()
+
+
+def test_the_largest_sizes_that_are_taken():
+    assert lib().abc_distill_workspace_bytes(F32, 1, 1, (1 << 29) - 1, 8, 3) > 1 << 31 and lib().abc_distill_workspace_bytes(F32, 65535, 8, 0, 65536, 1024) > 0
 
 
 def test_workspaces():
