@@ -1231,24 +1231,26 @@ struct Plan { int tile, splits; int64_t kstep; int nm, nn; };
 //   fp32 gradients, from 128   by the product with the longer k: 128 x 1024 x 4096 (96) 41 / 47, 1000 x 1000 x 1024 (128) 60 / 53,
 //                              256 x 4096 x 1024 (144) 59 / 51, 128 x 4096 x 4096 (288) 100 / 69
 //   bf16, from 64              scores of 128 x 1024 x 4096 (72) 30 / 22, 128 x 8192 x 1024 (192) 28 / 24
-// Tiles of 64: parts until `wgs` workgroups run, 256 for the scores, whose rows' launch adds the slabs up (128 x 1024 x 4096, forward: 27 us, with
-// 1024 35; 64 x 8192 x 1024 in bf16 18 and 27), 1024 for the gradients.
+// Parts of k: until two workgroups a CU (tiles of 64: four) run, as long as a part keeps 8 stages of 64; tiles of 64 until every CU has one, as
+// long as it keeps two.  More parts are more slabs to write and add up: 128 x 1024 x 4096, forward 27 us, with parts until four a CU run 35,
+// backward 32 and 38; 32 x 21 000 x 4096 221 and, one workgroup a CU, 256; 17 x 300 x 4096, forward 19.2 us with 16 parts, 20.8 with 32 (cap).
 #define LEAST_SCORES 288
 #define LEAST_GRADS 128
 #define LEAST_BF16 64
-static Plan plan(int64_t m, int64_t n, int64_t k, int least, int wgs) {
+static int64_t parts_of(const Plan& p, int64_t stages, int cap) {
+    const int64_t tiles = (int64_t)p.nm * p.nn;
+    int64_t sp = min((p.tile == 128 ? 512 : 1024) / tiles, stages / 8);
+    if (p.tile == 64) sp = max(sp, min(256 / tiles, stages / 2));
+    return max((int64_t)1, min(sp, (int64_t)cap));
+}
+static Plan plan(int64_t m, int64_t n, int64_t k, int least, int cap) {
     Plan p;
     auto tiles = [&](int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
     const int64_t stages = (k + 63) / 64;
     p.tile = m > 64 && n > 64 && tiles(128) * (stages / 8 + 1) >= least ? 128 : 64;
     p.nm = (int)((m + p.tile - 1) / p.tile);
     p.nn = (int)((n + p.tile - 1) / p.tile);
-    int64_t sp = (p.tile == 128 ? 512 : wgs) / ((int64_t)p.nm * p.nn);
-    const int64_t most = p.tile == 128 ? stages / 8 : stages / 2;
-    if (sp > most) sp = most;
-    if (sp > wgs / 16) sp = wgs / 16;
-    if (sp > 32) sp = 32;
-    if (sp < 1) sp = 1;
+    const int64_t sp = parts_of(p, stages, cap);
     const int64_t per = (stages + sp - 1) / sp;
     p.kstep = per * 64;
     p.splits = (int)((stages + per - 1) / per);
@@ -1267,7 +1269,7 @@ struct FwdLayout {
 
 static FwdLayout fwd_layout(int dtype, int64_t B, int64_t T, int d, int k) {
     FwdLayout L;
-    L.s = plan(B, T, d, dtype == ABC_DT_BF16 ? LEAST_BF16 : LEAST_SCORES, 256);
+    L.s = plan(B, T, d, dtype == ABC_DT_BF16 ? LEAST_BF16 : LEAST_SCORES, 16);
     L.lds = (T + 31) / 32 * 32;
     L.segs = L.s.splits == 1 ? L.s.nn * 2 : (int)((T + DISTILL_SEG - 1) / DISTILL_SEG);
     // From about 8 GFLOP a product on, half the matrix work is worth the launches that find out and then return (256 x 16 384 x 1024, forward and
@@ -1296,8 +1298,8 @@ static BwdLayout bwd_layout(int dtype, int64_t B, int64_t C, int64_t T, int d, b
     BwdLayout L;
     L.ldg = (T + 31) / 32 * 32;                                // as the logits' rows
     L.segs = (int)((L.ldg + DISTILL_SEG - 1) / DISTILL_SEG);
-    L.q = plan(B, d, T, least, 1024);
-    L.p = plan(C, d, B, least, 1024);
+    L.q = plan(B, d, T, least, 32);
+    L.p = plan(C, d, B, least, 32);
     if (fast || (L.q.tile == 128) != (L.p.tile == 128)) {         // one launch, one kind of tile: that of the larger product
         const int tile = fast || (T >= B ? L.q.tile : L.p.tile) == 128 ? 128 : 64;
         auto with = [&](Plan& x, int64_t m, int64_t n, int64_t k) {
@@ -1305,12 +1307,7 @@ static BwdLayout bwd_layout(int dtype, int64_t B, int64_t C, int64_t T, int d, b
             x.tile = tile;
             x.nm = (int)((m + tile - 1) / tile);
             x.nn = (int)((n + tile - 1) / tile);
-            int64_t sp = (tile == 128 ? 512 : 1024) / ((int64_t)x.nm * x.nn);
-            const int64_t stages = (k + 63) / 64;
-            const int64_t most = tile == 128 ? stages / 8 : stages / 2;   // as plan() has it
-            if (sp > most) sp = most;
-            if (sp > 32) sp = 32;
-            if (sp < 1) sp = 1;
+            const int64_t stages = (k + 63) / 64, sp = parts_of(x, stages, 32);
             const int64_t per = (stages + sp - 1) / sp;
             x.kstep = per * 64;
             x.splits = (int)((stages + per - 1) / per);
@@ -1390,8 +1387,8 @@ typedef CfgDma<DmaKC<2, 64>, DmaKS<1, 64>, 2, 1, 64, 64, 256, false, true> GradQ
 typedef CfgDma<DmaKS<2, 64>, DmaKS<1, 64>, 2, 1, 64, 64, 256, false, true> GradPB64;
 typedef Cfg<LoadKC<3, 128, 1>, LoadKS<3, 128, 1>, 3, 128, 1, 1, 0> GradQF128;
 typedef Cfg<LoadKS<3, 128, 1>, LoadKS<3, 128, 1>, 3, 128, 1, 1, 0> GradPF128;
-typedef Cfg<LoadKC<3, 64, 2>, LoadKS<3, 64, 2>, 3, 64, 2, 2, 1> GradQF64;
-typedef Cfg<LoadKS<3, 64, 2>, LoadKS<3, 64, 2>, 3, 64, 2, 2, 1> GradPF64;
+typedef Cfg<LoadKC<3, 64, 2>, LoadKS<3, 64, 2>, 3, 64, 2, 1, 0> GradQF64;
+typedef Cfg<LoadKS<3, 64, 2>, LoadKS<3, 64, 2>, 3, 64, 2, 1, 0> GradPF64;
 typedef CfgMix<DmaKC<2, 128>, LoadKS<2, 128, 1>, 128, 128, 256, 1> GradQH128;
 typedef CfgDma<DmaKS<2, 128>, DmaKS<2, 128>, 2, 2, 128, 128, 256, true, false> GradPH128;
 typedef CfgMix<DmaKC<2, 256, 512>, LoadKS<2, 128, 1, 512>, 256, 128, 512, 0> GradQH256;
