@@ -398,3 +398,29 @@ def test_a_training_step_over_a_store():
     # the memory is a corpus: the 8-bit form is searched by the exact top-k, and holds the step's candidates now
     idx = search.topk(search.Embeddings(p[:5].to(DEV), "i8"), memory.embeddings(), 1)[1][:, 0].cpu()
     assert torch.equal(idx, torch.arange(5))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_memory_past_4_gib(dtype):
+    """Rows behind 2^32 bytes are the ones the lists name.  Reference in fp64 by a matrix product of this card.
+
+    A score of unit rows is off by at most 2^-21 (what the parts leave out) + D / 32 * 2^-24 (the sums): 8.2e-6, z by 1.2e-4 at a
+    temperature of 0.07, a row's loss by twice that and a probability by 2.4e-4 of itself.  dq is a sum of unit rows, by g / temp / rows: its
+    norm is off by at most that share of (|p|_1 + |t|_1) / temp / rows = 2 / 0.07 / 8, and by its own rounding."""
+    d, M, B, C, temp = 4096, (1 << 32) // (4096 * (4 if dtype is torch.float32 else 2)) + 3001, 8, 4, 0.07
+    g = torch.Generator(DEV).manual_seed(5)
+    unit_rows = lambda n: torch.nn.functional.normalize(torch.randn(n, d, generator=g, device=DEV), dim=1).to(dtype)
+    q, p, m = unit_rows(B).requires_grad_(True), unit_rows(C), unit_rows(M)
+    index = C + M - 1 - torch.arange(B * 3, device=DEV).view(B, 3) * 100
+    score = torch.randn(B, 3, generator=g, device=DEV)
+    loss, _ = call(q, p, m, torch.tensor(temp, device=DEV), index, score, 0.5)
+    dq, = torch.autograd.grad(loss, q)
+    cand = torch.cat((p, m)).double()
+    z = q.detach().double() @ cand.T / float(torch.tensor(temp))
+    logt = torch.log_softmax(score.double() / 0.5, dim=1)
+    want = (logt.exp() * (logt - z.gather(1, index))).sum(1) + torch.logsumexp(z, 1)
+    assert abs(float(loss.detach()) - float(want.mean())) <= 2.4e-4
+    gm = torch.softmax(z, 1).scatter_add(1, index, -logt.exp()) / B / float(torch.tensor(temp))
+    ref = gm @ cand
+    lim = 2.4e-4 * 2 / 0.07 / B + (2.0 ** -8 if dtype is torch.bfloat16 else 2.0 ** -20) * ref.norm(dim=1)
+    assert bool(((dq.double() - ref).norm(dim=1) <= lim).all())

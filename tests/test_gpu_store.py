@@ -310,3 +310,23 @@ def test_more_rows_than_a_launch_takes():
     got = s.read()
     want = store_oracle.store_values(values, 128).float().to(DEV)
     assert torch.equal(got[:n], want[at]) and not got[n:].any()
+
+
+def test_rows_past_4_gib():
+    """4-bit rows of 2 KB from slot 2^21 on, 8-bit rows of 4 KB from 2^20 on: written, read and scored there."""
+    x, q = rows(5, 4096, 1), rows(3, 4096, 2)
+    for group, slots in ((128, torch.tensor([3, (1 << 21) - 1, 1 << 21, (1 << 21) + 9, 2_200_000])),
+                         (0, torch.tensor([0, (1 << 20) - 1, 1 << 20, (1 << 20) + 1, 1_200_001]))):
+        big, small = empty(int(slots[-1]) + 1, 4096, group), empty(5, 4096, group)
+        big.write(x.to(DEV), slots.to(DEV))
+        small.write(x.to(DEV), torch.arange(5, device=DEV))
+        same_bits((big.read(slots.to(DEV)),), (small.read(),))
+        if group:
+            got = big.scores(q.to(DEV))
+            want = torch.zeros_like(got)
+            want[:, slots.to(DEV)] = small.scores(q.to(DEV))
+            # the waves that share a small store's rows add up in another order: 32 pieces' sums, a rounding each
+            size = q.abs() @ small.read().cpu().abs().T
+            assert bool(((got - want)[:, slots.to(DEV)].cpu().abs() <= 64 * 2.0 ** -24 * size).all())
+            want[:, slots.to(DEV)] = got[:, slots.to(DEV)]
+            assert torch.equal(got, want)

@@ -370,7 +370,7 @@ def _store_out(out: torch.Tensor, shape: tuple, n: int, data: torch.Tensor) -> T
 
 def store_scores(q: torch.Tensor, data: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     """f32 [nq, rows]: inner products of the queries q [nq, dim] (f32 / bf16) with every row of a 4-bit store.  For a few queries,
-    where the stream over the store is the cost; a large set of them belongs in topk."""
+    where the stream over the store is the cost; a large set of them belongs in topk.  Carries no gradient."""
     group, width, rows = _store_form(data, scale)
     if group == 0:
         raise _lib.AbcError("store_scores: the 4-bit form only (an int8 store is searched by topk)")
