@@ -18,8 +18,9 @@
 //   bf16          one product for s; the gradients take two (g in hi + mid, 2^-16 relative, below the 2^-8 of the result's own
 //                 rounding).
 //
-// An MFMA rounds its accumulator once (to nearest), so the products of the lower parts have an accumulator of their own: the sum of
-// the leading ones is rounded K / 32 times, not 6 K / 32.
+// An MFMA rounds its accumulator once (to nearest), so the products of the lower parts have an accumulator of their own where the result
+// is fp32: the sum of the leading ones is rounded K / 32 times, not 6 K / 32.  bf16 gradients have one (2 K / 32 roundings of 2^-24 beside the
+// result's own 2^-9) and fit three workgroups a CU (1000 x 5000 x 3584 backward: 185 -> 174 us).
 #include "common.h"
 #include <type_traits>
 #include "../../include/abcsearch.h"
@@ -400,7 +401,7 @@ struct Cfg {
     typedef LA_ LA;
     typedef LB_ LB;
     static constexpr int NT = 256, PA = PARTS_, PB = PARTS_, KEEP = PARTS_, TM = TILE_, TN = TILE_, DEPTH = DEPTH_, LBUF = LBUF_, FROM = FROM_, KIND = 0;
-    static constexpr bool F16 = false, OUT_BF16 = false, SCORES = LA::KC && LB::KC;
+    static constexpr bool F16 = false, OUT_BF16 = false, LOW = true, SCORES = LA::KC && LB::KC;
     static constexpr int LDS = LBUF * (PA * TM + PB * TN) * 64;
 };
 template <class DA_, class LB_, int TM_, int TN_, int NT_, int FROM_>
@@ -408,7 +409,7 @@ struct CfgMix {
     typedef DA_ DA;
     typedef LB_ LB;
     static constexpr int NT = NT_, PA = 2, PB = 2, KEEP = 2, TM = TM_, TN = TN_, FROM = FROM_, KIND = 1;
-    static constexpr bool F16 = true, OUT_BF16 = false, SCORES = LB::KC;
+    static constexpr bool F16 = true, OUT_BF16 = false, LOW = true, SCORES = LB::KC;
     static constexpr int BUF = DA::BYTES + PB * TN * 64, LDS = 2 * BUF;
     static_assert(DA::KC && DA::KB == 1, "");
 };
@@ -418,7 +419,7 @@ struct CfgDma {
     typedef DB_ DB;
     static constexpr int NT = NT_, PA = PA_, PB = PB_, KEEP = PA_, TM = TM_, TN = TN_, BUF = DA::BYTES + DB::BYTES, LDS = 2 * BUF;
     static constexpr int KB = DA::KB, KIND = 2;
-    static constexpr bool F16 = F16_, OUT_BF16 = OUT_BF16_, SCORES = DA::KC && DB::KC;
+    static constexpr bool F16 = F16_, OUT_BF16 = OUT_BF16_, LOW = F16, SCORES = DA::KC && DB::KC;   // bf16 results: one accumulator will do
     static_assert(DA::KB == DB::KB, "");
 };
 struct Straight { static __host__ __device__ constexpr int tile_index(int r) { return r; } };
@@ -438,7 +439,7 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 template <class C, class LA, class LB, class ACC, class LOW>
 __device__ __forceinline__ void finish(const GemmArgs& g, int tm, int tn, int sp, const ACC& acc, const LOW& low) {
     constexpr int WM = Waves<C>::WM, WN = Waves<C>::WN;
-    constexpr bool TWO = C::KEEP > 1;
+    constexpr bool TWO = C::LOW;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, h = lane >> 4, wm = Waves<C>::m(wave), wn = Waves<C>::n(wave);
     const float f = g.scale * (g.splits == 1 && g.f0 ? factor_of(g.f0, g.f1, g.f2) : 1.f);
     constexpr bool PAIR = LB::tile_index(16) == 1;               // a lane's blocks j and j + 1 hold neighbouring columns
@@ -509,7 +510,7 @@ __device__ __forceinline__ void finish(const GemmArgs& g, int tm, int tn, int sp
 // what every form of the product starts with: its tile, its part of k, its accumulators
 #define GEMM_BEGIN(STAGE_VALUES) \
     constexpr int WM = Waves<C>::WM, WN = Waves<C>::WN, STAGE = STAGE_VALUES; \
-    constexpr bool TWO = C::KEEP > 1; \
+    constexpr bool TWO = C::LOW; \
     typedef typename std::conditional<C::F16, v8h, v8bf>::type frag_t; \
     const int per = g.nm * g.nn, sp = item / per, inner = item % per, tn = inner / g.nm, tm = inner % g.nm; \
     const int64_t k0 = sp * g.kstep, k1 = min(g.k, k0 + g.kstep); \
@@ -722,7 +723,7 @@ __device__ __forceinline__ bool gemm_straight(const GemmArgs& g, int item, char*
                     for (int pb = 0; pb < C::PB; ++pb)
                         if (pa + pb < C::KEEP)
 #pragma unroll
-                            for (int j = 0; j < WN; ++j) mfma<C>(pa + pb == 0 ? acc[i][j] : low[TWO ? i : 0][TWO ? j : 0], fa[pa][i], fb[pb][j]);
+                            for (int j = 0; j < WN; ++j) mfma<C>(!TWO || pa + pb == 0 ? acc[i][j] : low[TWO ? i : 0][TWO ? j : 0], fa[pa][i], fb[pb][j]);
             }
         }
     }
