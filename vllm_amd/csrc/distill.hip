@@ -20,7 +20,7 @@
 //
 // An MFMA rounds its accumulator once (to nearest), so the products of the lower parts have an accumulator of their own where the result
 // is fp32: the sum of the leading ones is rounded K / 32 times, not 6 K / 32.  bf16 gradients have one (2 K / 32 roundings of 2^-24 beside the
-// result's own 2^-9) and fit three workgroups a CU (1000 x 5000 x 3584 backward: 185 -> 174 us).
+// result's own 2^-8) and fit three workgroups a CU (1000 x 5000 x 3584 backward: 185 -> 174 us).
 #include "common.h"
 #include <type_traits>
 #include "../../include/abcsearch.h"
