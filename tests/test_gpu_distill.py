@@ -78,9 +78,9 @@ SHAPES = [(1, 1, 0, 8, 1), (1, 3, 0, 16, 2), (2, 5, 7, 24, 3), (33, 100, 0, 72, 
 
 # fp32 products of 8 GFLOP and more go by fp16 parts
 # tiles of 128 and, fp32, of 256 rows of queries; the second: of 128 alone, with odd ends on every side; then fp32 gradients, and all three
-# products, in tiles of 128 without the fp16 parts; narrow rows
+# products, in tiles of 128 without the fp16 parts; narrow rows, the second of them in tiles of 128 x 96 (bf16)
 LARGE = [(256, 1000, 15_400, 1024, 40), (300, 901, 12_000, 1192, 17), (520, 2100, 0, 4096, 9), (400, 1501, 0, 1024, 7), (130, 3900, 201, 3000, 9),
-         (1000, 2000, 29_001, 136, 5), (700, 1500, 7, 8, 3), (513, 900, 0, 24, 5)]
+         (1000, 2000, 29_001, 136, 5), (1000, 2601, 600, 264, 9), (700, 1500, 7, 8, 3), (513, 900, 0, 24, 5)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])

@@ -1263,6 +1263,7 @@ static inline size_t up(size_t x) { return (x + 255) & ~(size_t)255; }
 struct FwdLayout {
     Plan s;
     bool fast;                       // fp32 by fp16 parts
+    bool narrow;                     // bf16: tiles of 128 x 96
     int64_t lds;
     int segs;
     size_t off_s, off_seg, off_lse, off_t, off_li, off_row, off_stat, off_cnt, off_q, off_qout, off_flag, total;
@@ -1271,6 +1272,12 @@ struct FwdLayout {
 static FwdLayout fwd_layout(int dtype, int64_t B, int64_t T, int d, int k) {
     FwdLayout L;
     L.s = plan(B, T, d, dtype == ABC_DT_BF16 ? LEAST_BF16 : LEAST_SCORES, 16);
+    // bf16, two workgroups a CU: where one round holds tiles of 128 x 96 they fill it better than those of 128 x 128 (1000 x 5000 x 3584, forward: 67 us
+    // and 76; 1000 x 6100 x 4096 75 and 85; 256 x 20 000 x 3584 60 and 66; 500 x 7000 x 768 31 and 30), and better than two parts of a short k (1000 x 3200 x
+    // 1024 36 and 41, 128 x 30 000 x 1024 32 and 39; but 1000 x 3500 x 3584 59 and 56).
+    const int64_t n96 = (T + 95) / 96;
+    L.narrow = dtype == ABC_DT_BF16 && L.s.tile == 128 && (L.s.splits == 1 || d < 2048) && L.s.nm * n96 > 256 && L.s.nm * n96 <= 512;
+    if (L.narrow) { L.s.nn = (int)n96; L.s.splits = 1; L.s.kstep = (d + 63) / 64 * 64; }
     L.lds = (T + 31) / 32 * 32;
     L.segs = L.s.splits == 1 ? L.s.nn * 2 : (int)((T + DISTILL_SEG - 1) / DISTILL_SEG);
     // From about 8 GFLOP a product on, half the matrix work is worth the launches that find out and then return (256 x 16 384 x 1024, forward and
@@ -1376,6 +1383,7 @@ static void launch_grads(const GemmArgs& gq, const GemmArgs& gp, bool dq, bool d
 
 // s: bf16; fp32 by three bf16 parts (128 / 64 wide tiles); fp32 by two fp16 parts (the queries' are ready)
 typedef CfgDma<DmaKC<1, 128>, DmaKC<1, 128>, 1, 1, 128, 128, 256, false, false> ScoresB128;
+typedef CfgDma<DmaKC<1, 128>, DmaKC<1, 96>, 1, 1, 128, 96, 256, false, false> ScoresB96;
 typedef CfgDma<DmaKC<1, 64>, DmaKC<1, 64>, 1, 1, 64, 64, 256, false, false> ScoresB64;
 typedef Cfg<LoadKC<3, 128, 1>, LoadKC<3, 128, 1>, 3, 128, 1, 1, 0> ScoresF128;
 typedef Cfg<LoadKC<3, 64, 3>, LoadKC<3, 64, 3>, 3, 64, 3, 2, 1> ScoresF64;
@@ -1424,7 +1432,8 @@ extern "C" int abc_distill_fwd(int dtype, const void* q, const void* p, const vo
     const bool ready = L.s.splits == 1;
     if (ready) { g.seg = (float*)(w + L.off_seg); g.segs = L.segs; g.f2 = temp; }
     if (dtype == ABC_DT_BF16) {
-        if (L.s.tile == 128) launch_scores<ScoresB128>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
+        if (L.narrow) launch_scores<ScoresB96>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
+        else if (L.s.tile == 128) launch_scores<ScoresB128>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
         else launch_scores<ScoresB64>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
     } else if (L.fast) {
         unsigned* qout = (unsigned*)(w + L.off_qout);
