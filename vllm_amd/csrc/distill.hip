@@ -682,7 +682,8 @@ __device__ __forceinline__ bool gemm_mix(const GemmArgs& g, int item, char* smem
 // A stage is on its way into one LDS buffer while the other is multiplied, and no register holds it in between.  512 x 16384 x 3584 in
 // bf16: scores 68 us, gradients 131 us (0.88 and 1.0 PFLOP/s; a large product of a library 1.38).  Measured and left: a third buffer (one
 // workgroup a CU less: 112 and 159 us), wave tiles of 128 x 64, one wave a SIMD, with the fragments' reads and the loads spread among the
-// MFMAs by hand (4 % of the scores' time; the fragments' LDS reads, which bound it, are a quarter less), and the loads alone spread (slower).
+// MFMAs by hand (4 % of the scores' time), and the loads alone spread (slower).  What bounds it: MFMAs are busy 46 to 51 % of the clocks, at
+// 1.95 GHz (the power limit); waves wait 28 % of theirs for a stage.
 template <class C>
 __device__ __forceinline__ bool gemm_straight(const GemmArgs& g, int item, char* smem) {
     GEMM_BEGIN(C::KB * 32)
