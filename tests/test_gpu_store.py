@@ -330,3 +330,36 @@ def test_rows_past_4_gib():
             assert bool(((got - want)[:, slots.to(DEV)].cpu().abs() <= 64 * 2.0 ** -24 * size).all())
             want[:, slots.to(DEV)] = got[:, slots.to(DEV)]
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("group", [0, 128])
+def test_what_is_written_is_known_to_have_changed(group):
+    """A graph that saved a buffer or a store's scale refuses its backward after the kernel wrote there; a corpus kept by version is new."""
+    from vllm_amd import search
+    s = empty(40, 128, group)
+    s.write(rows(40, 128, 0).to(DEV), torch.arange(40, device=DEV))
+    buf, w = torch.empty(40, 128, device=DEV), torch.ones(40, 128, device=DEV, requires_grad=True)
+    s.read(out=buf)
+    loss = (w * buf).sum()
+    s.read(out=buf[:7], index=torch.arange(7, device=DEV))
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+    loss = (torch.ones_like(s.scale, dtype=torch.float32, requires_grad=True) * s.scale).sum()
+    s.write(rows(1, 128, 1).to(DEV), torch.zeros(1, dtype=torch.int64, device=DEV))
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+    q = rows(3, 128, 5).to(DEV)
+
+    def negatives(c):
+        found = {}
+        for i in range(3):
+            search.negatives_for_sample(i, found, q, c, top=5)
+        return found
+
+    s.read(out=buf)
+    a = negatives(buf)
+    s.write(rows(40, 128, 9).to(DEV), torch.arange(40, device=DEV))
+    s.read(out=buf)
+    b, want = negatives(buf), negatives(buf.clone())
+    search.release_resident()
+    assert b == want and a != b

@@ -321,6 +321,13 @@ def store_write(x: torch.Tensor, slots: Optional[torch.Tensor], data: torch.Tens
     if n:
         _launch(lib.abc_store_write, "abc_store_write", data.device, dt, x.data_ptr(), ld, at, int(first), n, dim, data.data_ptr(),
                 scale.data_ptr(), capacity, group, None if ws is None else ws.data_ptr(), need)
+        _changed((data, scale))
+
+
+def _changed(tensors) -> None:
+    """Tell torch that a kernel wrote into these tensors: a graph that saved one of them refuses its backward, and what is kept by a
+    tensor's version (search.negatives_for_sample's resident corpus) is made anew."""
+    torch.autograd.graph.increment_version(tensors)
 
 
 def store_read(index: Optional[torch.Tensor], data: torch.Tensor, scale: torch.Tensor, dim: int, dtype: torch.dtype = torch.float32,
@@ -336,7 +343,8 @@ def store_read(index: Optional[torch.Tensor], data: torch.Tensor, scale: torch.T
     else:
         index = _index64(index, data, "index")
         shape, n, at = (*index.shape, dim), index.numel(), index.data_ptr()
-    if out is None:
+    given = out is not None
+    if not given:
         dt = _ROW_DT.get(dtype)
         if dt is None:
             raise _lib.AbcError(f"store_read: rows are read as f32 or bf16, not {dtype}")
@@ -347,6 +355,8 @@ def store_read(index: Optional[torch.Tensor], data: torch.Tensor, scale: torch.T
     if n:
         _launch(_lib.load().abc_store_read, "abc_store_read", data.device, at, 0, n, data.data_ptr(), scale.data_ptr(), capacity, dim, group,
                 dt, to, ld)
+        if given:
+            _changed(out)
     return out
 
 
