@@ -202,7 +202,8 @@ int abc_infonce_bwd(const float* q, const float* p, const float* lse, const floa
  *   B in [1, 65535], d % 8 == 0, d <= 65536, k in [1, 1024]; B x T and C x d at most 2^23 tiles of 64 x 64.
  * abc_distill_bwd: `fwd_ws` is the workspace abc_distill_fwd was given for the same arguments, unchanged since (it is only read:
  *   the backward may run more than once).  dq [B,d], dp [C,d] in dtype, d_temp [1] f32, each nullable (not computed), overwritten;
- *   grad_out is a device scalar.  Rows without an entry receive no gradient.
+ *   grad_out is a device scalar.  Rows without an entry receive no gradient (dq is zero there whatever the candidates hold) and send
+ *   none (an infinity or a NaN in such a row's query reaches no candidate).
  * Both workspaces may hold anything before; nothing is kept in the library between calls; results do not vary from run to run.
  */
 size_t abc_distill_workspace_bytes(int dtype, int64_t B, int64_t C, int64_t M, int d, int k);

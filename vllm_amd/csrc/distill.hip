@@ -6,6 +6,9 @@
 //   loss = mean of row_b over the rows that have an entry; a row without one counts nowhere and receives no gradient
 //   g_bj = (softmax(z)_bj - sum_{i: idx(b,i) = j} t_bi) grad_out / rows;  dq = g/temp c, dc = (g/temp)^T q, dtemp = -sum g z / temp
 //
+// A row without an entry has g = 0, and 0 times an infinity or a NaN is not 0: the candidates' product reads such a row's query as zeros
+// (a copy that the kernel of g makes beside it, or the split kernel its parts), and its dq is written as zeros.
+//
 // Three products (s, dq, dc) over B x T x d are the work, on the 16-bit matrix cores (v_mfma_f32_16x16x32):
 //
 //   fp32, small   x = hi + mid + lo, three bf16 values that carry 24 bits (hi cut, the rest rounded), and the six products of the
@@ -358,6 +361,7 @@ struct GemmArgs {
     const float *f0, *f1, *f2;       // splits == 1, f0 given: times f0[0] f1[0] / f2[0]
     float* seg;                      // splits == 1, given: every wave's part of a row's statistics, [rows][segs][4] (RowArgs), z = value / f2[0]
     int segs;
+    const float* live;               // given: a row of A's side where it is not above 0 gives zeros
 };
 
 // reductions over the 16 lanes that hold a row of an accumulator; every lane gets the result
@@ -451,6 +455,7 @@ __device__ __forceinline__ void finish(const GemmArgs& g, int tm, int tn, int sp
     // columns n, n + 1 of row m: g.b.rows is even, or the row goes on
     auto put_pair = [&](int64_t m, int64_t n, float a, float b) {
         if (m >= g.a.rows || n >= g.b.rows) return;
+        if (!C::SCORES && g.live && !(g.live[m] > 0.f)) a = b = 0.f;
         if (C::OUT_BF16 && g.splits == 1) *(uint32_t*)((uint16_t*)g.out + m * g.ldo + n) = f32_to_bf16_bits(a) | f32_to_bf16_bits(b) << 16;
         else *(v2f*)((float*)g.out + sp * g.slab + m * g.ldo + n) = v2f{a, b};
     };
@@ -774,15 +779,23 @@ __global__ __launch_bounds__(CQ::NT, 2) void distill_grads_kernel(const GemmArgs
     }
 }
 
-// the queries' fp16 parts, once for all tiles of the two products that read them; rows_out[b]: row b does not fit them.  dpad: d up to 32s
-__global__ __launch_bounds__(256) void distill_split_kernel(const float* __restrict__ q, int d, int dpad, char* __restrict__ out,
+// whether entry (index, score) of a list is one
+__device__ __forceinline__ bool is_entry(int64_t j, float x) { return j >= 0 && !(x == -INFINITY); }
+
+// the queries' fp16 parts, once for all tiles of the two products that read them, zeros for a row without an entry; rows_out[b]: row b does
+// not fit them.  dpad: d up to 32s
+__global__ __launch_bounds__(256) void distill_split_kernel(const float* __restrict__ q, int d, int dpad, const int64_t* __restrict__ idx,
+                                                            const float* __restrict__ score, int list, char* __restrict__ out,
                                                             unsigned* __restrict__ rows_out, unsigned* __restrict__ flag) {
     __shared__ float red[4];
     const int64_t b = blockIdx.x;
     if (b == 0 && threadIdx.x == 0) *flag = 0u;
+    bool some = false;
+    for (int i = threadIdx.x; i < list; i += 256) some |= is_entry(idx[b * list + i], score[b * list + i]);
+    some = __syncthreads_or(some);
     float top = 0.f;
     for (int k = threadIdx.x * 4; k < dpad; k += 1024) {
-        const v4f x = k < d ? *(const v4f*)(q + b * d + k) : v4f{0.f, 0.f, 0.f, 0.f};
+        const v4f x = k < d && some ? *(const v4f*)(q + b * d + k) : v4f{0.f, 0.f, 0.f, 0.f};
         uint32_t lo[2], hi[2];
         split_pair(x[0], x[1], lo);
         split_pair(x[2], x[3], hi);
@@ -905,7 +918,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
             if (i >= a.k) continue;
             const int64_t j = idx[i];
             const float x = score[i];
-            if (j >= 0 && !(x == -INFINITY)) {
+            if (is_entry(j, x)) {
                 some = 1;
                 if (j >= a.T || !(x < INFINITY)) bad = 1.f;      // a column that is not there, a score that is no number: the row is NaN
                 else { at[u] = (int)j; v[u] = x; best = fmaxf(best, x); }
@@ -1105,7 +1118,8 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
 }
 
 // ---- softmax - target ----------------------------------------------------------------------------------------------------
-// HBM-bound: the logits once, g once, in the form that the products take (512 x 16 384: 67 MB in 15.5 us, 4.3 TB/s).
+// HBM-bound: the logits once, g once, in the form that the products take (512 x 16 384: 67 MB in 15.5 us, 4.3 TB/s).  One workgroup more a row
+// copies its query for the candidates' product.
 enum { G_F32, G_F16, G_BF16 };
 struct GradArgs {
     const float* s;                  // [B][lds]
@@ -1120,7 +1134,11 @@ struct GradArgs {
     int form;                        // G_F32, G_F16 (G_F32 where flag is set) or G_BF16
     const unsigned* flag;
     void* g;                         // [B][ldg] fp32 or two parts of 16 bits; zeros from T on
-    float* dt;                       // [B][segments]: sums of (softmax - target) z
+    int segs;
+    float* dt;                       // [B][segs]: sums of (softmax - target) z
+    const char* q;
+    char* qlive;                     // given (segs + 1 workgroups a row): the queries, zeros for rows without an entry.  G_F16: where flag is set
+    int qbytes;                      // a query's
 };
 
 __global__ __launch_bounds__(256) void distill_grad_kernel(const GradArgs a) {
@@ -1129,8 +1147,14 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(const GradArgs a) {
     const int64_t b = blockIdx.y, j0 = (int64_t)blockIdx.x * DISTILL_SEG;
     const int tid = threadIdx.x;
     const bool has = a.has[b] > 0.f;
-    const float inv = __fdiv_rn(1.f, a.temp[0]), l = a.lse[b];
     const int form = a.form == G_F16 && *a.flag ? G_F32 : a.form;
+    if ((int)blockIdx.x == a.segs) {
+        if (form == G_F16) return;                               // (the split kernel has seen to their parts)
+        for (int i = tid * 16; i < a.qbytes; i += 4096)
+            *(v4u*)(a.qlive + b * a.qbytes + i) = has ? *(const v4u*)(a.q + b * a.qbytes + i) : v4u{0, 0, 0, 0};
+        return;
+    }
+    const float inv = __fdiv_rn(1.f, a.temp[0]), l = a.lse[b];
     v4f x[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -1175,7 +1199,7 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(const GradArgs a) {
         }
     }
     dt = block_red(0.f, dt, 0, red).b;
-    if (tid == 0) a.dt[b * gridDim.x + blockIdx.x] = dt;
+    if (tid == 0) a.dt[b * a.segs + blockIdx.x] = dt;
 }
 
 // ---- sums of the split products' slabs, and of the temperature's gradient ------------------------------------------------
@@ -1185,6 +1209,8 @@ struct SumArgs {
     int64_t n[2];                    // values, a multiple of 4 (0: nothing to do)
     int splits[2];
     int blocks0;                     // workgroups of the first
+    const float* live;               // of the first's rows of d values: one that is not above 0 gives zeros
+    int d;
     const float* dt;
     int64_t ndt;
     const float *f0, *f1, *f2;       // grad_out, 1 / rows, temp
@@ -1217,6 +1243,7 @@ __global__ __launch_bounds__(256) void distill_sum_kernel(const SumArgs a) {
             if (p + o < a.splits[which]) x += y[o];
     }
     x *= f;
+    if (which == 0 && !(a.live[(uint32_t)i / (uint32_t)a.d] > 0.f)) x = v4f{0.f, 0.f, 0.f, 0.f};   // (at most 65 535 x 65 536 values)
     if constexpr (BF16) {
         uint32_t lo = f32_to_bf16_bits(x[0]) | f32_to_bf16_bits(x[1]) << 16, hi = f32_to_bf16_bits(x[2]) | f32_to_bf16_bits(x[3]) << 16;
         *(uint2*)((uint16_t*)a.out[which] + i) = uint2{lo, hi};
@@ -1301,7 +1328,7 @@ static FwdLayout fwd_layout(int dtype, int64_t B, int64_t T, int d, int k) {
     return L;
 }
 
-struct BwdLayout { Plan q, p; int64_t ldg; int segs; size_t off_g, off_dt, off_pq, off_pp, total; };
+struct BwdLayout { Plan q, p; int64_t ldg; int segs; size_t off_g, off_dt, off_pq, off_pp, off_ql, total; };
 static BwdLayout bwd_layout(int dtype, int64_t B, int64_t C, int64_t T, int d, bool fast, bool dq, bool dp) {
     const int least = dtype == ABC_DT_BF16 ? LEAST_BF16 : LEAST_GRADS;
     BwdLayout L;
@@ -1329,6 +1356,7 @@ static BwdLayout bwd_layout(int dtype, int64_t B, int64_t C, int64_t T, int d, b
     L.off_dt = o; o += up((size_t)B * L.segs * 4);
     L.off_pq = o; o += dq && L.q.splits > 1 ? up((size_t)L.q.splits * B * d * 4) : 0;
     L.off_pp = o; o += dp && L.p.splits > 1 ? up((size_t)L.p.splits * C * d * 4) : 0;
+    L.off_ql = o; o += dp ? up((size_t)B * d * (dtype == ABC_DT_BF16 ? 2 : 4)) : 0;
     L.total = o;
     return L;
 }
@@ -1438,7 +1466,8 @@ extern "C" int abc_distill_fwd(int dtype, const void* q, const void* p, const vo
         else launch_scores<ScoresB64>(g, nullptr, 0, nullptr, nullptr, 0, cnt, nc, st);
     } else if (L.fast) {
         unsigned* qout = (unsigned*)(w + L.off_qout);
-        hipLaunchKernelGGL(distill_split_kernel, dim3((unsigned)B), dim3(256), 0, st, (const float*)q, d, (d + 31) / 32 * 32, w + L.off_q, qout, flag);
+        hipLaunchKernelGGL(distill_split_kernel, dim3((unsigned)B), dim3(256), 0, st, (const float*)q, d, (d + 31) / 32 * 32, teacher_idx, teacher_score, k,
+                           w + L.off_q, qout, flag);
         GemmArgs h = g;
         h.a = Side{w + L.off_q, w + L.off_q, B, (d + 31) / 32 * 64, B, (d + 31) / 32 * 32};
         if (tiles_of(B, 256) * 2 * 5 <= tiles_of(B, 128) * 6) launch_scores<ScoresH256>(tall(h), nullptr, 0, flag, qout, B, cnt, nc, st);
@@ -1481,16 +1510,18 @@ extern "C" int abc_distill_bwd(int dtype, const void* q, const void* p, const vo
     a.s = (const float*)(f + F.off_s); a.lds = F.lds; a.lse = (const float*)(f + F.off_lse); a.t = (const float*)(f + F.off_t);
     a.li = (const int*)(f + F.off_li); a.has = (const float*)(f + F.off_row) + 2 * B; a.temp = temp;
     a.T = T; a.ldg = L.ldg; a.k = k; a.form = bf ? G_BF16 : F.fast ? G_F16 : G_F32; a.flag = flag;
-    a.g = w + L.off_g; a.dt = (float*)(w + L.off_dt);
-    hipLaunchKernelGGL(distill_grad_kernel, dim3((unsigned)L.segs, (unsigned)B), dim3(256), 0, st, a);
+    a.g = w + L.off_g; a.segs = L.segs; a.dt = (float*)(w + L.off_dt);
+    a.q = (const char*)q; a.qlive = w + L.off_ql; a.qbytes = d * (bf ? 2 : 4);
+    hipLaunchKernelGGL(distill_grad_kernel, dim3((unsigned)(L.segs + (dp ? 1 : 0)), (unsigned)B), dim3(256), 0, st, a);
     SumArgs sa = {};
     if (dq || dp) {
         const Side gq{a.g, a.g, B, L.ldg, B, L.ldg}, gp{a.g, a.g, B, L.ldg, C, L.ldg};                       // fp32
         const Side hq{a.g, a.g, B, L.ldg * 2, B, L.ldg}, hp{a.g, a.g, B, L.ldg * 2, C, L.ldg};               // two parts
-        const Side cand{p, memory, C, d, d, d}, query{q, q, B, d, d, d};
+        const Side cand{p, memory, C, d, d, d}, query{a.qlive, a.qlive, B, d, d, d};
         GemmArgs xq = gemm_args(gq, cand, T, L.q, L.q.splits > 1 ? (void*)(w + L.off_pq) : dq, d, B * d);
         GemmArgs xp = gemm_args(gp, query, B, L.p, L.p.splits > 1 ? (void*)(w + L.off_pp) : dp, d, C * d);
         for (GemmArgs* x : {&xq, &xp}) { x->f0 = grad_out; x->f1 = stat; x->f2 = temp; }
+        if (L.q.splits == 1) xq.live = a.has;
         if (bf) {
             xq.a = hq;
             xp.a = hp;
@@ -1515,7 +1546,7 @@ extern "C" int abc_distill_bwd(int dtype, const void* q, const void* p, const vo
     if (sa.n[0] || sa.n[1] || d_temp) {
         sa.blocks0 = (int)((sa.n[0] + 1023) / 1024);
         const int blocks1 = (int)((sa.n[1] + 1023) / 1024);
-        sa.dt = a.dt; sa.ndt = B * L.segs; sa.f0 = grad_out; sa.f1 = stat; sa.f2 = temp; sa.d_temp = d_temp;
+        sa.dt = a.dt; sa.ndt = B * L.segs; sa.f0 = grad_out; sa.f1 = stat; sa.f2 = temp; sa.d_temp = d_temp; sa.live = a.has; sa.d = d;
         if (bf) hipLaunchKernelGGL(distill_sum_kernel<true>, dim3(sa.blocks0 + blocks1 + 1), dim3(256), 0, st, sa);
         else hipLaunchKernelGGL(distill_sum_kernel<false>, dim3(sa.blocks0 + blocks1 + 1), dim3(256), 0, st, sa);
     }
