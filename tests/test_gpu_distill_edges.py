@@ -70,3 +70,49 @@ def test_a_row_without_an_entry_receives_nothing(shape, dtype):
     index[:] = -1
     out = step(q, p, m, 0.07, index, score)
     assert not any(bool(x.any()) for x in out)                      # (a NaN is not zero)
+
+
+def certain(sharp, far, T, D, dtype, temp):
+    """Two rows that are nearly certain of columns 3 and T - 2, and candidates 8 I (their first D), so that dq = 8 g / temp / 2 for the first D
+    columns, with no sum over others: queries with z = sharp at the column and z = far at the D - 1 others, zero (z = 0) beyond D."""
+    q = torch.full((2, D), far * temp / 8)
+    p = torch.zeros(T, D)
+    p[:D] = 8 * torch.eye(D)
+    q[0, 3] = q[1, D - 2] = sharp * temp / 8
+    return q.to(dtype), p.to(dtype), torch.tensor([[3], [D - 2]]), torch.zeros(2, 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [64, 5000])
+@pytest.mark.parametrize("sharp,far,temp", [(1000.0, 988.0, 0.125), (14.0, 2.0, 0.07), (1000.0, 988.0, -0.125), (1000.0, 988.0, 0.07),
+                                            (4000.0, 3990.0, 1.0 / 3)])
+def test_what_a_nearly_certain_row_still_has_to_learn(sharp, far, temp, T, dtype):
+    """One entry, at the row's maximum m: the loss is log(sum), sum = 1 + (D - 1) exp(far - m), and g there is 1 / sum - 1.
+
+    u = 2^-24.  A logit is rounded where it is made: its sum (one product), 1 / temp, theirs: 3 u |z| each for the maximum and for the others,
+    whose difference is then off by 6 u |z| at most, and so is every share of the others, relative to itself; exp adds 8 u.  The sum of exp rounds
+    at its size, 1 (each partial sum that holds the maximum: 2 + log2 of the waves' records, under 12 u), 1 / sum and the product 2 u: 14 u
+    in all for the share at the maximum and, beside its others' 6 u |z| (1 - share), for the loss, whose logarithm adds 8 u.  In bf16 a result is
+    rounded by 2^-8 of itself and g is held to 2^-15; fp32 products of parts lose 2^-21.  The row's g adds up to nothing but those."""
+    D = 64
+    q, p, index, score = certain(sharp, far, T, D, dtype, temp)
+    t32 = float(torch.tensor(temp))
+    z = q.double() @ p.double().t() / t32
+    m, at = z.max(1)
+    assert at.tolist() == index[:, 0].tolist()
+    rest = torch.exp(z - m[:, None]).sum(1) - 1
+    loss, agree, dq, _, _ = step(q, p, None, temp, index, score, 1.0)
+    assert float(agree) == 1.0
+    drift = 6 * U * abs(sharp) + 8 * U
+    want = float(torch.log1p(rest).mean())
+    assert abs(float(loss) - want) <= float(rest.max()) * drift + 22 * U, (float(loss), want)
+    g = dq.double() * (2 * t32 / 8)                                 # 1 / temp and 1 / 2 were applied to g, 8 is the candidate's
+    share = 2.0 ** -15 + 2.0 ** -8 if dtype is torch.bfloat16 else 2.0 ** -21 + 4 * U
+    ref = torch.exp(z - m[:, None])[:, :D] / (1 + rest)[:, None]
+    ref[0, 3] -= 1
+    ref[1, D - 2] -= 1
+    lim = ref.abs() * (share + drift) + 14 * U * (ref < 0)
+    assert bool(((g - ref).abs() <= lim).all()), float(((g - ref).abs() / lim).max())
+    beyond = 1 - torch.exp(z - m[:, None])[:, :D].sum(1) / (1 + rest)           # the columns past D, whose share reaches no query
+    total = (g.sum(1) + beyond).abs()
+    assert bool((total <= ref.abs().sum(1) * share + 14 * U + beyond * drift).all()), total

@@ -6,6 +6,9 @@
 //   loss = mean of row_b over the rows that have an entry; a row without one counts nowhere and receives no gradient
 //   g_bj = (softmax(z)_bj - sum_{i: idx(b,i) = j} t_bi) grad_out / rows;  dq = g/temp c, dc = (g/temp)^T q, dtemp = -sum g z / temp
 //
+// A row's logsumexp stays in two parts, its maximum m and the sum of exp(z - m): in one fp32 number a sum just above 1 would be lost beside a
+// large maximum, and with it what a nearly certain row still has to learn (m = 1000: steps of 6e-5).  softmax(z) = exp(z - m) / sum.
+//
 // A row without an entry has g = 0, and 0 times an infinity or a NaN is not 0: the candidates' product reads such a row's query as zeros
 // (a copy that the kernel of g makes beside it, or the split kernel its parts), and its dq is written as zeros.
 //
@@ -51,6 +54,12 @@ __device__ __forceinline__ float exp_neg(float x) {
     const float n = rintf(x * 1.44269504f);
     const float f = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269502f, -n));      // log2 e in two parts
     return x < -150.f ? 0.f : ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
+}
+
+// z of a sum s.  Rounded wherever it is used: fused into a subtraction it would be another number than the one that the row's maximum is.
+__device__ __forceinline__ float logit(float s, float inv_temp) {
+#pragma clang fp contract(off)
+    return s * inv_temp;
 }
 
 // ---- operands -----------------------------------------------------------------------------------------------------------
@@ -497,7 +506,7 @@ __device__ __forceinline__ void finish(const GemmArgs& g, int tm, int tn, int sp
 #pragma unroll
                     for (int j = 0; j < WN; ++j) {
                         const int64_t n = (int64_t)tn * C::TN + (wn * WN + j) * 16 + l15;
-                        z[j] = n < g.b.rows ? value(i, j, r) * inv : -INFINITY;
+                        z[j] = n < g.b.rows ? logit(value(i, j, r), inv) : -INFINITY;
                         if (z[j] > mx) { mx = z[j]; am = (int)n; }
                         if (z[j] != z[j]) se = z[j];             // a NaN stays one whatever the maximum is
                     }
@@ -831,7 +840,7 @@ struct RowArgs {
     int64_t B, T;
     int k;
     float* seg;                      // [B][segs][4]: maximum, sum of exp(z - maximum), its first column, 1 where a z is NaN
-    float* lse;                      // [B]
+    float* norm;                     // [B] the row's maximum, then [B] 1 / its sum of exp(z - maximum)
     float* t;                        // [B][k]: the teacher's share of column li (all of a column's entries at the first of them), or 0
     int* li;                         // [B][k]: the column, -1 = nothing
     float* row;                      // [B] row losses, then [B] agreement, then [B] 1 where the row has an entry
@@ -959,7 +968,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 if (j0 + u * 1024 + c >= a.T) { x[u][c] = -INFINITY; continue; }
-                x[u][c] *= inv;
+                x[u][c] = logit(x[u][c], inv);
                 if (x[u][c] > mx) { mx = x[u][c]; am = (int)(j0 + u * 1024 + c); }
                 nan |= x[u][c] != x[u][c];
             }
@@ -1025,7 +1034,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
         se = r2.b;
         am = r2.c;
     }
-    float l = nan ? __uint_as_float(0x7FC00000u) : mx + logf(se);
+    if (nan) se = __uint_as_float(0x7FC00000u);
     // ---- the teacher's list: softmax over its entries, the best of them, the row's loss
     if (!a.ready) take_list();
     const int k8 = (a.k + 7) & ~7;
@@ -1039,7 +1048,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
         some = -r.c;
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) z[u] *= inv;
+    for (int u = 0; u < 4; ++u) z[u] = logit(z[u], inv) - mx;
     float e[4], esum = 0.f;
     int first = INT32_MAX;
 #pragma unroll
@@ -1088,10 +1097,11 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
         a.li[b * a.k + i] = mine ? at[u] : -1;
     }
     sum = block_red(0.f, sum, 0, red).b;
-    if (bad > 0.f) l = __uint_as_float(0x7FC00000u);
+    if (bad > 0.f) se = __uint_as_float(0x7FC00000u);
     if (tid == 0) {
-        a.lse[b] = l;
-        put(a.row + b, some ? sum + l : 0.f);
+        a.norm[b] = mx;
+        a.norm[a.B + b] = __fdiv_rn(1.f, se);
+        put(a.row + b, some ? sum + logf(se) : 0.f);
         put(a.row + a.B + b, some && bad == 0.f && am == li[first] ? 1.f : 0.f);
         put(a.row + 2 * a.B + b, some ? 1.f : 0.f);
     }
@@ -1124,7 +1134,7 @@ enum { G_F32, G_F16, G_BF16 };
 struct GradArgs {
     const float* s;                  // [B][lds]
     int64_t lds;
-    const float* lse;
+    const float* norm;               // [2][rows]
     const float* t;
     const int* li;
     const float* has;                // [B]: 1 where the row has an entry
@@ -1154,7 +1164,7 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(const GradArgs a) {
             *(v4u*)(a.qlive + b * a.qbytes + i) = has ? *(const v4u*)(a.q + b * a.qbytes + i) : v4u{0, 0, 0, 0};
         return;
     }
-    const float inv = __fdiv_rn(1.f, a.temp[0]), l = a.lse[b];
+    const float inv = __fdiv_rn(1.f, a.temp[0]), mx = a.norm[b], one = a.norm[gridDim.y + b];
     v4f x[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -1177,8 +1187,8 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(const GradArgs a) {
         v4f y;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const float z = x[u][c] * inv;
-            y[c] = j + c < a.T && has ? exp_neg(z - l) - tg[c] : 0.f;
+            const float z = logit(x[u][c], inv);
+            y[c] = j + c < a.T && has ? fmaf(exp_neg(z - mx), one, -tg[c]) : 0.f;
             if (j + c < a.T && has) dt += y[c] * z;
         }
         if (form == G_F32) *(v4f*)((float*)a.g + b * a.ldg + j) = y;
@@ -1294,7 +1304,7 @@ struct FwdLayout {
     bool narrow;                     // bf16: tiles of 128 x 96
     int64_t lds;
     int segs;
-    size_t off_s, off_seg, off_lse, off_t, off_li, off_row, off_stat, off_cnt, off_q, off_qout, off_flag, total;
+    size_t off_s, off_seg, off_norm, off_t, off_li, off_row, off_stat, off_cnt, off_q, off_qout, off_flag, total;
 };
 
 static FwdLayout fwd_layout(int dtype, int64_t B, int64_t T, int d, int k) {
@@ -1315,7 +1325,7 @@ static FwdLayout fwd_layout(int dtype, int64_t B, int64_t T, int d, int k) {
     L.off_s = 0;
     if (L.s.splits > 1) { L.off_s = o; o += up((size_t)B * L.lds * 4); }
     L.off_seg = o; o += up((size_t)B * L.segs * 16);
-    L.off_lse = o; o += up((size_t)B * 4);
+    L.off_norm = o; o += up((size_t)B * 8);
     L.off_t = o; o += up((size_t)B * k * 4);
     L.off_li = o; o += up((size_t)B * k * 4);
     L.off_row = o; o += up((size_t)B * 12);
@@ -1478,7 +1488,7 @@ extern "C" int abc_distill_fwd(int dtype, const void* q, const void* p, const vo
     RowArgs r;
     r.part = (const float*)w; r.s = (float*)(w + L.off_s); r.splits = L.s.splits; r.segs = L.segs; r.ready = ready; r.slab = B * L.lds; r.lds = L.lds;
     r.temp = temp; r.idx = teacher_idx; r.score = teacher_score; r.teacher_temp = teacher_temp; r.B = B; r.T = T; r.k = k;
-    r.seg = (float*)(w + L.off_seg); r.lse = (float*)(w + L.off_lse); r.t = (float*)(w + L.off_t); r.li = (int*)(w + L.off_li);
+    r.seg = (float*)(w + L.off_seg); r.norm = (float*)(w + L.off_norm); r.t = (float*)(w + L.off_t); r.li = (int*)(w + L.off_li);
     r.row = (float*)(w + L.off_row); r.stat = (float*)(w + L.off_stat); r.cnt = cnt; r.out_loss = out_loss; r.out_agree = out_agree;
     hipLaunchKernelGGL(distill_row_kernel, dim3(ready ? 1u : (unsigned)L.segs, (unsigned)B), dim3(256), 0, st, r);
     hipError_t e = hipGetLastError();
@@ -1507,7 +1517,7 @@ extern "C" int abc_distill_bwd(int dtype, const void* q, const void* p, const vo
     const unsigned* flag = F.fast ? (const unsigned*)(f + F.off_flag) : nullptr;
     const float* stat = (const float*)(f + F.off_stat);
     GradArgs a;
-    a.s = (const float*)(f + F.off_s); a.lds = F.lds; a.lse = (const float*)(f + F.off_lse); a.t = (const float*)(f + F.off_t);
+    a.s = (const float*)(f + F.off_s); a.lds = F.lds; a.norm = (const float*)(f + F.off_norm); a.t = (const float*)(f + F.off_t);
     a.li = (const int*)(f + F.off_li); a.has = (const float*)(f + F.off_row) + 2 * B; a.temp = temp;
     a.T = T; a.ldg = L.ldg; a.k = k; a.form = bf ? G_BF16 : F.fast ? G_F16 : G_F32; a.flag = flag;
     a.g = w + L.off_g; a.segs = L.segs; a.dt = (float*)(w + L.off_dt);
