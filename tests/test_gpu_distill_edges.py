@@ -116,3 +116,24 @@ def test_what_a_nearly_certain_row_still_has_to_learn(sharp, far, temp, T, dtype
     beyond = 1 - torch.exp(z - m[:, None])[:, :D].sum(1) / (1 + rest)           # the columns past D, whose share reaches no query
     total = (g.sum(1) + beyond).abs()
     assert bool((total <= ref.abs().sum(1) * share + 14 * U + beyond * drift).all()), total
+
+
+@pytest.mark.parametrize("B,D", [(64, 64), (1500, 64), (1500, 1024)])
+def test_bf16_gradients_hold_g_to_17_bits(B, D):
+    """Candidates e_0 and -e_0 with nearly the same share, which no list names: dq_0 = (p_0 - p_1) / temp / B shows what g is off by.
+
+    g is held in two rounded bf16 parts, to 2^-17 of itself, twice that in a difference; p itself is off by less than 16 u relative to a share of
+    the row (|z| < 1: products and 1 / temp 3 u, exp 8 u, the sum and its reciprocal 5 u), 32 u in the difference; sums of two products and the
+    factor 4 u; the result is rounded by 2^-8 of itself."""
+    g = torch.Generator().manual_seed(B + D)
+    temp = 1.0
+    q, p = torch.zeros(B, D), torch.zeros(3, D)
+    p[0, 0], p[1, 0], p[2, 1] = 1.0, -1.0, 1.0
+    q[:, 0] = 2.0 ** -11
+    q[:, 1] = torch.rand(B, generator=g) * 2 - 1
+    q, p = q.bfloat16(), p.bfloat16()
+    dq = step(q, p, None, temp, torch.full((B, 1), 2), torch.zeros(B, 1))[2].double()
+    share = torch.softmax(q.double() @ p.double().t(), 1)
+    want = (share[:, 0] - share[:, 1]) / B
+    room = (share[:, 0] + share[:, 1]) / B * (2.0 ** -17 + 20 * U) + 2.0 ** -8 * want.abs()
+    assert bool(((dq[:, 0] - want).abs() <= room).all()), float(((dq[:, 0] - want).abs() / room).max())

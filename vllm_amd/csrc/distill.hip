@@ -21,8 +21,8 @@
 //                 2^-23 of a product.  Holds for rows whose largest magnitude is in [2^-10, 65000] (a value is carried to 2^-36, 2^-26 of
 //                 that, at worst) or zero; unit rows are.  Whether all are is found out while they are read for s; where not, flag is set, and
 //                 the same launches once more, which return at once otherwise, take the six products.
-//   bf16          one product for s; the gradients take two (g in hi + mid, 2^-16 relative, below the 2^-8 of the result's own
-//                 rounding).
+//   bf16          one product for s; the gradients take two (g = hi + mid, both rounded: 2^-17 of g at most, below the 2^-8 of the
+//                 result's own rounding; with hi cut it would be 2^-16, and twice as many results a place off the nearest).
 //
 // An MFMA rounds its accumulator once (to nearest), so the products of the lower parts have an accumulator of their own where the result
 // is fp32: the sum of the leading ones is rounded K / 32 times, not 6 K / 32.  bf16 gradients have one (2 K / 32 roundings of 2^-24 beside the
@@ -98,6 +98,12 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[2]) {
     w[0] = __builtin_bit_cast(uint32_t, h);
     const float ra = fmaf((float)h[0], -2048.f, a * 2048.f), rb = fmaf((float)h[1], -2048.f, b * 2048.f);
     w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{ra, rb}, v2h));
+}
+// two fp32 values as two bf16 parts each, packed, to 2^-17 of the value
+__device__ __forceinline__ void split_round(float a, float b, uint32_t (&w)[2]) {
+    w[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2bf));
+    const float ra = a - __uint_as_float(w[0] << 16), rb = b - __uint_as_float(w[0] & 0xFFFF0000u);
+    w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{ra, rb}, v2bf));
 }
 
 // A converted tile side in LDS: [part][row][32 k], 64 bytes a row, four 16-byte chunks permuted with the row.  A 16-byte access of
@@ -1198,10 +1204,8 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(const GradArgs a) {
                 split_pair(y[0] * G_SCALE, y[1] * G_SCALE, lo);
                 split_pair(y[2] * G_SCALE, y[3] * G_SCALE, hi);
             } else {
-                uint32_t l3[3], h3[3];
-                split_pair(y[0], y[1], l3);
-                split_pair(y[2], y[3], h3);
-                lo[0] = l3[0]; lo[1] = l3[1]; hi[0] = h3[0]; hi[1] = h3[1];
+                split_round(y[0], y[1], lo);
+                split_round(y[2], y[3], hi);
             }
             char* out = (char*)a.g + b * a.ldg * 4 + split_at(j);
             *(uint2*)out = uint2{lo[0], hi[0]};
