@@ -137,3 +137,20 @@ def test_bf16_gradients_hold_g_to_17_bits(B, D):
     want = (share[:, 0] - share[:, 1]) / B
     room = (share[:, 0] + share[:, 1]) / B * (2.0 ** -17 + 20 * U) + 2.0 ** -8 * want.abs()
     assert bool(((dq[:, 0] - want).abs() <= room).all()), float(((dq[:, 0] - want).abs() / room).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_best_entry_at_any_teacher_temperature(dtype):
+    """An infinite temperature makes all shares alike; the best entry is still the one with the largest score."""
+    g = torch.Generator().manual_seed(3)
+    q = p = torch.eye(16, 64).to(dtype)
+    index = torch.stack([torch.randperm(16, generator=g)[:6] for _ in range(16)])
+    score = torch.rand(16, 6, generator=g)
+    index[:8, 4], score[:8, 4] = torch.arange(8), 2.0               # half of the rows: the student's best is the teacher's, in the fifth place
+    index[8:, 0], score[8:, 3] = torch.arange(8, 16), 2.0           # the others: it is in the first place, and not the teacher's best
+    index[8:, 3] = (torch.arange(8, 16) + 1) % 16
+    for tt in (INF, 3e38, 1e30, 1.0, 1e-3):
+        loss, agree, *_ = step(q, p, None, 0.5, index, score, tt)
+        r = distill_ref(q, p, 0.5, index, score, float(torch.tensor(tt)), 16)
+        # 6 shares and logits of at most 2, each within a few u; at 1e-3 the scores' differences of 2000 are divided once: 2000 u
+        assert float(agree) == 0.5 and r["agree"] == 0.5 and abs(float(loss) - float(r["loss"])) <= 2100 * U, tt

@@ -1061,10 +1061,11 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
     for (int u = 0; u < 4; ++u) {
         const int i = tid + u * 256;
         e[u] = 0.f;
+        const bool top = v[u] == best;                           // (of the scores: a quotient by a large temperature may be 0 for others too)
         v[u] = __fdiv_rn(v[u] - best, a.teacher_temp);
         if (at[u] >= 0) {
             e[u] = exp_neg(v[u]);
-            if (v[u] == 0.f) first = min(first, i);
+            if (top) first = min(first, i);
         }
         esum += e[u];
         if (i < k8) le[i] = e[u];
