@@ -154,3 +154,23 @@ def test_the_best_entry_at_any_teacher_temperature(dtype):
         r = distill_ref(q, p, 0.5, index, score, float(torch.tensor(tt)), 16)
         # 6 shares and logits of at most 2, each within a few u; at 1e-3 the scores' differences of 2000 are divided once: 2000 u
         assert float(agree) == 0.5 and r["agree"] == 0.5 and abs(float(loss) - float(r["loss"])) <= 2100 * U, tt
+
+
+def test_a_loss_that_is_kept_holds_no_workspace():
+    """After its backward a loss kept for a log is four bytes (an allocator's block); before it, or with retain_graph, the logits stay."""
+    B, C, D = 256, 4096, 64
+    g = torch.Generator().manual_seed(4)
+    leaves = [x.to(DEV).requires_grad_(True) for x in (unit(B, D, g), unit(C, D, g))]
+    index, score = torch.randint(C, (B, 4), generator=g).to(DEV), torch.rand(B, 4, generator=g).to(DEV)
+    kept = []
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated(DEV)
+    for _ in range(3):
+        loss, agree = call(leaves[0], leaves[1], None, 0.07, index, score, 1.0)
+        torch.autograd.grad(loss, leaves, retain_graph=True)
+        assert torch.cuda.memory_allocated(DEV) - before >= B * C * 4
+        torch.autograd.grad(loss, leaves)
+        kept.append((loss, agree))
+        assert torch.cuda.memory_allocated(DEV) - before < 1 << 20
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(loss, leaves)

@@ -1326,6 +1326,7 @@ static FwdLayout fwd_layout(int dtype, int64_t B, int64_t T, int d, int k) {
     // From about 8 GFLOP a product on, half the matrix work is worth the launches that find out and then return (256 x 16 384 x 1024, forward and
     // backward: 121 us, without 150).
     L.fast = dtype == ABC_DT_F32 && L.s.tile == 128 && 2.0 * (double)B * (double)T * d >= 8e9;
+    // (slabs, which the backward keeps without reading them: 512 tiles of 64 KB, 1024 of 16 KB, 32 MB at most)
     size_t o = up((size_t)L.s.splits * B * L.lds * 4);
     L.off_s = 0;
     if (L.s.splits > 1) { L.off_s = o; o += up((size_t)B * L.lds * 4); }

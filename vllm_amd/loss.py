@@ -205,8 +205,7 @@ class _Distill(torch.autograd.Function):
         _launch(lib.abc_distill_fwd, "abc_distill_fwd", dev, dtype, q.data_ptr(), p.data_ptr(), mem, t.data_ptr(), index.data_ptr(),
                 score.data_ptr(), teacher_temp, B, C, M, d, k, loss.data_ptr(), agree.data_ptr(), ws.data_ptr(), need)
         if any(ctx.needs_input_grad):
-            ctx.save_for_backward(q, p, t, memory)
-            ctx.ws = ws
+            ctx.save_for_backward(q, p, t, memory, ws)                      # (freed with the graph, not with the last loss that is kept)
             ctx.meta = (dtype, B, C, M, d, k, need, temp.dtype, temp.shape)
         ctx.mark_non_differentiable(agree)
         return loss, agree
@@ -218,7 +217,7 @@ class _Distill(torch.autograd.Function):
 
 
 def _distill_bwd(ctx, grad_loss, _grad_agree):
-    q, p, t, memory = ctx.saved_tensors
+    q, p, t, memory, fwd_ws = ctx.saved_tensors
     dtype, B, C, M, d, k, fwd_need, tdtype, tshape = ctx.meta
     lib = _lib.load()
     need_q, need_p, need_t = ctx.needs_input_grad[:3]
@@ -231,7 +230,7 @@ def _distill_bwd(ctx, grad_loss, _grad_agree):
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _launch(lib.abc_distill_bwd, "abc_distill_bwd", dev, dtype, q.data_ptr(), p.data_ptr(), None if memory is None else memory.data_ptr(),
             t.data_ptr(), go.data_ptr(), B, C, M, d, k, None if dq is None else dq.data_ptr(),
-            None if dp is None else dp.data_ptr(), None if dt is None else dt.data_ptr(), ctx.ws.data_ptr(), fwd_need, ws.data_ptr(), need)
+            None if dp is None else dp.data_ptr(), None if dt is None else dt.data_ptr(), fwd_ws.data_ptr(), fwd_need, ws.data_ptr(), need)
     if dt is not None and tdtype is not torch.float32:
         dt = dt.to(tdtype)
     return dq, dp, dt, None, None, None, None
