@@ -174,3 +174,40 @@ def test_a_loss_that_is_kept_holds_no_workspace():
         assert torch.cuda.memory_allocated(DEV) - before < 1 << 20
         with pytest.raises(RuntimeError, match="second time"):
             torch.autograd.grad(loss, leaves)
+
+
+def test_temperatures_under_capture():
+    """A number and a tensor on the card are captured; a parameter on the host, whose copy could not be, is refused and the capture goes on."""
+    from vllm_amd._lib import AbcError
+    from vllm_amd.loss import Temperature, compute_contrastive_loss
+    g = torch.Generator().manual_seed(6)
+    leaves = [x.to(DEV).requires_grad_(True) for x in (unit(32, 64, g), unit(80, 64, g))]
+    index, score = torch.randint(80, (32, 4), generator=g).to(DEV), torch.rand(32, 4, generator=g).to(DEV)
+    temps = (0.07, torch.tensor([0.07], device=DEV), Temperature().to(DEV))
+
+    def passes():
+        out = []
+        for t in temps:
+            loss, agree = call(leaves[0], leaves[1], None, t, index, score, 0.5)
+            out += [loss.detach(), agree, *torch.autograd.grad(loss, leaves)]
+        loss, acc = compute_contrastive_loss(leaves[0], leaves[1], 0.07)
+        return out + [loss.detach(), acc, *torch.autograd.grad(loss, leaves)]
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for host in (Temperature(), torch.tensor(0.07)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(AbcError, match="capture: the temperature is on cpu"):
+                    call(leaves[0], leaves[1], None, host, index, score, 0.5)
+        got = passes()
+    for i in range(3):
+        with torch.no_grad():
+            leaves[0].copy_(unit(32, 64, g))
+        graph.replay()
+        want = passes()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    host = Temperature()                                            # outside a capture it is brought over, and gets its gradient
+    loss, _ = call(leaves[0], leaves[1], None, host, index, score, 0.5)
+    loss.backward()
+    assert host.temp.grad.device.type == "cpu" and torch.equal(loss.detach(), got[0])

@@ -126,17 +126,17 @@ class _InfoNCE(torch.autograd.Function):
         return dq, None, dp, dt, None
 
 
-def _temp_param(temperature) -> torch.Tensor:
+def _temp_param(temperature, device: torch.device) -> torch.Tensor:
     t = getattr(temperature, "temp", temperature)
     if not torch.is_tensor(t):
-        t = torch.tensor(float(t), dtype=torch.float32)
+        t = torch.full((), float(t), dtype=torch.float32, device=device)    # (a fill: a copy from the host could not be captured)
     return t
 
 
 def _loss_and_acc(q_embeds, p_embeds, temperature, label_smoothing, local_rows, p_local=None):
     """p_embeds: the full candidate matrix; its first `local_rows` rows are `p_local` (default: p_embeds[:local_rows]),
     the only rows that receive a gradient."""
-    temp = _temp_param(temperature)
+    temp = _temp_param(temperature, q_embeds.device)
     if temp.device != q_embeds.device:
         temp = temp.to(q_embeds.device)
     if p_local is None:
@@ -161,6 +161,8 @@ def _captured_leaves(leaves, refuse: bool) -> list:
     there before.  A leaf has one gradient node while any autograd graph of it lives, bound to the stream that graph was built on; a
     captured backward that reaches a node of an eager graph makes the eager stream wait inside the capture, which ends the process when the
     capture ends.  Whether a node was there before: one that only this function holds is gone when it lets go, with its mark.
+    Only the tensors handed over are looked at.  Of leaves further up (an encoder's parameters) a node that the capture itself has made and one
+    from before look alike; there it is for the caller, as for every captured backward, to let go of earlier graphs.
     Returns the marked nodes: hold them until the call's own graph does."""
     held = []
     for x in leaves:
@@ -177,7 +179,7 @@ def _captured_leaves(leaves, refuse: bool) -> list:
                 raise _lib.AbcError(
                     "capture: an autograd graph of a leaf (queries, candidates or temperature) is alive from before; its gradient belongs to "
                     "another stream and capturing this backward would end the process.  Drop earlier losses and outputs of these leaves "
-                    "before the capture (inside one capture: call this loss first, or hand it x * 1)")
+                    "before the capture (inside one capture: call this loss before other uses of them)")
             continue
         node.metadata["abc_capture"] = stream
         held.append(node)
@@ -252,9 +254,13 @@ def compute_distillation_loss(q_embeds, p_embeds, temperature, teacher_index, te
 
     q_embeds [B, D], p_embeds and memory all bf16 run on bf16 products with fp32 sums and return bf16 gradients; any other mix is
     computed in fp32.  Returns (loss, agreement): agreement is the share of the rows with an entry whose best candidate is the
-    list's best entry.  Differentiable (once) w.r.t. q_embeds, p_embeds and temperature.temp.  Under graph capture take gradients
-    with torch.autograd.grad, as for every captured backward.  No counterpart in the reference."""
-    temp = _temp_param(temperature)
+    list's best entry.  Differentiable (once) w.r.t. q_embeds, p_embeds and temperature.temp.  
+
+    Under graph capture take gradients with torch.autograd.grad and have the temperature on the embeddings' device.  No autograd graph from
+    before the capture may hold a leaf that the backward reaches (torch would end the process): of q_embeds, p_embeds and the temperature
+    that are leaves themselves this is checked and refused; of an encoder's parameters behind them, or of embeddings computed before the
+    capture, it is not.  No counterpart in the reference."""
+    temp = _temp_param(temperature, q_embeds.device)
     dev, width = q_embeds.device, q_embeds.shape[-1]
     embeds = (q_embeds, p_embeds) if memory is None else (q_embeds, p_embeds, memory)
     same = True                                                             # all bf16 or all fp32, as they come
@@ -276,8 +282,11 @@ def compute_distillation_loss(q_embeds, p_embeds, temperature, teacher_index, te
     if not teacher_temperature > 0.0:
         raise _lib.AbcError("distillation: teacher_temperature must be positive")
     held = None
-    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
-        held = _captured_leaves((q_embeds, p_embeds, temp), refuse=True)
+    if torch.cuda.is_current_stream_capturing():
+        if temp.device != dev:
+            raise _lib.AbcError(f"capture: the temperature is on {temp.device}, and a copy of it to {dev} cannot be captured; move it there first")
+        if torch.is_grad_enabled():
+            held = _captured_leaves((q_embeds, p_embeds, temp), refuse=True)
     if temp.device != dev:
         temp = temp.to(dev)
     if not (same and (q_embeds.dtype is torch.bfloat16 or q_embeds.dtype is torch.float32)):
