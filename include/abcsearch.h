@@ -197,6 +197,8 @@ int abc_infonce_bwd(const float* q, const float* p, const float* lse, const floa
  *   z = (q @ cand^T) / temp;  teacher_idx [B,k] i64 / teacher_score [B,k] f32: the teacher's list of each query, as abc_topk_*
  *   returns it (an index < 0 or a score of -inf is no entry; an index >= T makes the row NaN; an index may come twice)
  *   t_b = softmax over row b's entries of score / teacher_temp;  row_b = sum_i t_bi (log t_bi - z_b,idx) + logsumexp_j z_bj
+ *   (the divergence where no column comes twice; else below that of the added shares by the entropy within a column, a constant)
+ *   f32 values are multiplied in 16-bit parts: an infinity makes its products NaN (bf16: +-inf as in any product)
  *   out_loss [1] f32: mean of row_b over the rows that have an entry (0 where none has)
  *   out_agree [1] f32: share of those rows whose best candidate (argmax z) is the best entry of the list
  *   B in [1, 65535], d % 8 == 0, d <= 65536, k in [1, 1024]; B x T and C x d at most 2^23 tiles of 64 x 64.
@@ -281,7 +283,8 @@ int abc_mean_pool_bwd_f32(const float* dx, const int64_t* ids, int64_t pad_id, c
  *   workspace >= abc_store_write_workspace_bytes(n, capacity) where slots is given (0 up to 2048 rows).
  * abc_store_read: out[i, :] = the values held by row index[i] (first + i where index is null); index < 0 gives zeros, index >=
  *   capacity NaN.  fp32 products code * scale, rounded once to bf16 where out is bf16.
- * abc_store_scores (fp4): out[i, n] = q[i, :] . (values of row n), n < rows; fp32 sums, fp32 queries at full precision.
+ * abc_store_scores (fp4): out[i, n] = q[i, :] . (values of row n), n < rows; fp32 sums, fp32 queries at full precision (from 2^-100 on;
+ *   the products of a group are added up before its scale is applied: values up to 2^118).
  */
 size_t abc_store_write_workspace_bytes(int64_t n, int64_t capacity);
 int abc_store_write(int x_dtype, const void* x, int64_t ldx, const int64_t* slots, int64_t first, int64_t n, int dim, void* data,

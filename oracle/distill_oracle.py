@@ -45,7 +45,7 @@ def distill_ref(q, cand, temp, index, score, teacher_temp, n_local, grad_out=1.0
 def distill_bounds(r, q, cand, temp, score, teacher_temp, n_local, k, bf16, grad_out=1.0):
     """How far fp32 arithmetic can be from `r`: u = 2^-24 is half a step of fp32; a sum of n terms in any order is off by at most n u times the
     sum of the terms' magnitudes; what the products of bf16 parts leave out is below 2^-21 of a product (mid lo + lo mid + lo lo with
-    |mid| <= 2^-7, |lo| <= 2^-15 of the value), what the products of fp16 parts leave out below 2^-22 (each value is off by 2^-24 of it and
+    |mid| <= 2^-7, |lo| <= 2^-15 of the value), what the products of fp16 parts leave out is at most 2^-21 (each value is off by 2^-23 of it and
     by 2^-36, lo lo is 2^-22 of a product); exp and log are off by at most 4 steps (8 u).  `cand` rows of magnitude 2^-10 and more carry
     the 2^-36 as 2^-26 of the row's largest value: `floor` below."""
     u, lost = 2.0 ** -24, 0.0 if bf16 else 2.0 ** -21

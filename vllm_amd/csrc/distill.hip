@@ -16,9 +16,9 @@
 //
 //   fp32, small   x = hi + mid + lo, three bf16 values that carry 24 bits (hi cut, the rest rounded), and the six products of the
 //                 parts down to 2^-16 relative (hi hi, hi mid, mid hi, hi lo, lo hi, mid mid): what is left out is below 2^-21 of a
-//                 product, random in sign.  Any fp32 value.
-//   fp32, large   x = hi + 2^-11 lo, two fp16 values of 11 bits each, and three products: half the matrix work for an error of
-//                 2^-23 of a product.  Holds for rows whose largest magnitude is in [2^-10, 65000] (a value is carried to 2^-36, 2^-26 of
+//                 product, random in sign.  Any finite fp32 value (an infinity leaves NaN in the lower parts).
+//   fp32, large   x = hi + 2^-11 lo, two fp16 values of 11 bits each (2^-23 of the value), and three products (lo lo, 2^-22, is left
+//                 out): half the matrix work for an error of at most 2^-21 of a product, 2^-23 in the root mean square.  Holds for rows whose largest magnitude is in [2^-10, 65000] (a value is carried to 2^-36, 2^-26 of
 //                 that, at worst) or zero; unit rows are.  Whether all are is found out while they are read for s; where not, flag is set, and
 //                 the same launches once more, which return at once otherwise, take the six products.
 //   bf16          one product for s; the gradients take two (g = hi + mid, both rounded: 2^-17 of g at most, below the 2^-8 of the
@@ -830,7 +830,7 @@ __global__ __launch_bounds__(256) void distill_split_kernel(const float* __restr
 }
 
 // ---- the rows: logsumexp, the teacher's list, the loss -------------------------------------------------------------------
-// A workgroup a row where the product left its waves' statistics (40 to 80 records of 64 columns), else one for 2048 columns, which adds up the
+// A workgroup a row where the product left its waves' statistics (two records a tile: 106 for 5000 columns, 256 for 16 384), else one for 2048 columns, which adds up the
 // slabs, and the last of a row's goes on.  Bound by latency: records, list, the list's logits, five reductions, two arrivals, one after
 // another.  1000 rows of 5000, list of 10: 14 us; 512 of 16 384, list of 100: 16.5; 128 of 1024 in 8 slabs, list of 64: 11.
 struct RowArgs {

@@ -395,7 +395,7 @@ __device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uin
 // hold the parts' sums of one query.  Up to sixteen: a part an A tile, all three into one accumulator, the smallest part first (13
 // queries, 100 003 x 1000: 21 us; four queries a tile, four tiles, reads a third more LDS and spills: 30 us).  Products and sums are
 // fp32.  A group's sum is scaled once.  The loads of the next four pieces (the next tile's, at a tile's end) are on their way while
-// four are multiplied: 8 KB a wave, 128 KB a CU.  Scales come 16 bytes a lane, 32 of a row at a time, and go through a strip of LDS
+// four are multiplied: 4 KB a wave, 64 KB a CU.  Scales come 16 bytes a lane, 32 of a row at a time, and go through a strip of LDS
 // of the wave's own (read where they are needed, 2 bytes a lane, they cost a third of the time: every access touches 16 lines).
 // 1 x 412 500 x 4096: 149 us, 5.8 TB/s.  With more queries MFMAs, sums and the fragments' LDS reads come to bound it: 103 000 x 4096, 1 / 6 / 13 fp32 queries 41 /
 // 69 / 88 us, 16 / 32 / 64 bf16 46 / 75 / 130 us.

@@ -301,7 +301,7 @@ def _store_rows(x: torch.Tensor, like: torch.Tensor, width: int, what: str) -> T
 def store_write(x: torch.Tensor, slots: Optional[torch.Tensor], data: torch.Tensor, scale: torch.Tensor, first: int = 0) -> None:
     """Quantise the rows of x [n, dim] (f32 / bf16) into the given slots of a store, in place; slots None: the n slots from
     `first` on, past the last one on from 0.  A slot outside the store drops its row (-1 = padding), and of rows that name the same slot
-    the last one stays."""
+    the last one stays.  More than 2048 rows with slots take 4 bytes of scratch for every slot of the store while the call runs."""
     group, width, capacity = _store_form(data, scale)
     x, n, dim, ld, dt = _store_rows(x, data, width, "store_write")
     lib = _lib.load()
@@ -380,7 +380,8 @@ def _store_out(out: torch.Tensor, shape: tuple, n: int, data: torch.Tensor) -> T
 
 def store_scores(q: torch.Tensor, data: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     """f32 [nq, rows]: inner products of the queries q [nq, dim] (f32 / bf16) with every row of a 4-bit store.  For a few queries,
-    where the stream over the store is the cost; a large set of them belongs in topk.  Carries no gradient."""
+    where the stream over the store is the cost; a large set of them belongs in topk.  Carries no gradient.  A group's products are added up before
+    its scale is applied: queries of up to 2^118."""
     group, width, rows = _store_form(data, scale)
     if group == 0:
         raise _lib.AbcError("store_scores: the 4-bit form only (an int8 store is searched by topk)")

@@ -248,12 +248,15 @@ def compute_distillation_loss(q_embeds, p_embeds, temperature, teacher_index, te
     The candidates are the rows of p_embeds [C, D] and after them the rows of `memory` [M, D], constants that receive no
     gradient (read back from a search.EmbeddingStore, or the other ranks' rows c_global[n:] of gathered_candidates).
     teacher_index [B, k] numbers them (0 .. C + M - 1), teacher_scores [B, k] are the teacher's scores of them, as topk returns them:
-    an index below 0 or a score of -inf is no entry, a column may come twice (its shares add up).  The teacher's shares are
-    softmax(teacher_scores / teacher_temperature) over a row's entries, which carry no gradient.  A row without an entry counts
-    nowhere and gets a gradient of zero; an index past the candidates makes the loss NaN.
+    an index below 0 or a score of -inf is no entry.  The teacher's shares are softmax(teacher_scores / teacher_temperature) over a row's
+    entries, which carry no gradient.  A row's value is sum_i share_i (log share_i - log softmax_column(i)) over the entries: the divergence
+    where no column comes twice, as in topk's lists.  A column may come twice: the gradients are those of its added shares, and the value
+    lies below the divergence of the added shares by the entropy within the column, a constant (so that it may be negative).  A row
+    without an entry counts nowhere and gets a gradient of zero; an index past the candidates makes the loss NaN.
 
     q_embeds [B, D], p_embeds and memory all bf16 run on bf16 products with fp32 sums and return bf16 gradients; any other mix is
-    computed in fp32.  Returns (loss, agreement): agreement is the share of the rows with an entry whose best candidate is the
+    computed in fp32, on the 16-bit parts of its values: an infinity in an embedding makes its logits NaN there (in bf16 +-inf where the
+    products are).  A width that is no multiple of 8 costs padded copies of queries, candidates and memory in every call.  Returns (loss, agreement): agreement is the share of the rows with an entry whose best candidate is the
     list's best entry.  Differentiable (once) w.r.t. q_embeds, p_embeds and temperature.temp.  
 
     Under graph capture take gradients with torch.autograd.grad and have the temperature on the embeddings' device.  No autograd graph from
