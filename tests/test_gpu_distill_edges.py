@@ -211,3 +211,30 @@ def test_temperatures_under_capture():
     loss, _ = call(leaves[0], leaves[1], None, host, index, score, 0.5)
     loss.backward()
     assert host.temp.grad.device.type == "cpu" and torch.equal(loss.detach(), got[0])
+
+
+def test_more_pairs_than_a_launch_has_threads_for():
+    """65 535 rows of 2^19 candidates: 256 stretches of 2048 logits a row and the row's query are 257 x 65 535 workgroups of 256 threads."""
+    B, T, d = 65535, 1 << 19, 8
+    torch.cuda.empty_cache()
+    need = 2 * B * T * 4 + (4 << 30)
+    free = torch.cuda.mem_get_info(DEV)[0]
+    if need > 0.95 * free:
+        pytest.skip(f"{need >> 30} GiB of {free >> 30} GiB that are free")
+    g = torch.Generator(DEV).manual_seed(1)
+    q, p = torch.randn(B, d, device=DEV, generator=g).bfloat16(), torch.randn(T, d, device=DEV, generator=g).bfloat16()
+    index, score = torch.randint(T, (B, 3), device=DEV, generator=g), torch.rand(B, 3, device=DEV, generator=g)
+    q[5], index[5] = NAN, -1
+    q.requires_grad_(True)
+    p.requires_grad_(True)
+    loss, _ = call(q, p, None, 1.0, index, score, 1.0)
+    dq, dp = torch.autograd.grad(loss, (q, p))
+    assert bool(torch.isfinite(loss.detach())) and bool(torch.isfinite(dp).all()) and not dq[5].any()
+    rows = [0, 1, B // 2, B - 1]
+    shares = torch.softmax(q.detach()[rows].double() @ p.detach().double().t(), 1)
+    want = shares.scatter_add(1, index[rows], -torch.softmax(score[rows].double(), 1)) @ p.detach().double() / (B - 1)
+    # a result is rounded by 2^-8 of itself at most; g by 2^-17 of the shares and of the list's, whose sums of candidates (|c| up to 5) are not small
+    size = (shares @ p.detach().double().abs() + 5) / (B - 1)
+    assert bool(((dq[rows].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -15 * size).all())
+    del loss, dq, dp
+    torch.cuda.empty_cache()

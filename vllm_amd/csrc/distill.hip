@@ -1151,7 +1151,7 @@ struct GradArgs {
     int form;                        // G_F32, G_F16 (G_F32 where flag is set) or G_BF16
     const unsigned* flag;
     void* g;                         // [B][ldg] fp32 or two parts of 16 bits; zeros from T on
-    int segs;
+    int segs, seg0;                  // seg0: this launch's first
     float* dt;                       // [B][segs]: sums of (softmax - target) z
     const char* q;
     char* qlive;                     // given (segs + 1 workgroups a row): the queries, zeros for rows without an entry.  G_F16: where flag is set
@@ -1161,11 +1161,12 @@ struct GradArgs {
 __global__ __launch_bounds__(256) void distill_grad_kernel(const GradArgs a) {
     __shared__ __attribute__((aligned(16))) float target[DISTILL_SEG];
     __shared__ Red red[4];
-    const int64_t b = blockIdx.y, j0 = (int64_t)blockIdx.x * DISTILL_SEG;
+    const int seg = a.seg0 + (int)blockIdx.x;
+    const int64_t b = blockIdx.y, j0 = (int64_t)seg * DISTILL_SEG;
     const int tid = threadIdx.x;
     const bool has = a.has[b] > 0.f;
     const int form = a.form == G_F16 && *a.flag ? G_F32 : a.form;
-    if ((int)blockIdx.x == a.segs) {
+    if (seg == a.segs) {
         if (form == G_F16) return;                               // (the split kernel has seen to their parts)
         for (int i = tid * 16; i < a.qbytes; i += 4096)
             *(v4u*)(a.qlive + b * a.qbytes + i) = has ? *(const v4u*)(a.q + b * a.qbytes + i) : v4u{0, 0, 0, 0};
@@ -1214,7 +1215,7 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(const GradArgs a) {
         }
     }
     dt = block_red(0.f, dt, 0, red).b;
-    if (tid == 0) a.dt[b * a.segs + blockIdx.x] = dt;
+    if (tid == 0) a.dt[b * a.segs + seg] = dt;
 }
 
 // ---- sums of the split products' slabs, and of the temperature's gradient ------------------------------------------------
@@ -1528,7 +1529,9 @@ extern "C" int abc_distill_bwd(int dtype, const void* q, const void* p, const vo
     a.T = T; a.ldg = L.ldg; a.k = k; a.form = bf ? G_BF16 : F.fast ? G_F16 : G_F32; a.flag = flag;
     a.g = w + L.off_g; a.segs = L.segs; a.dt = (float*)(w + L.off_dt);
     a.q = (const char*)q; a.qlive = w + L.off_ql; a.qbytes = d * (bf ? 2 : 4);
-    hipLaunchKernelGGL(distill_grad_kernel, dim3((unsigned)(L.segs + (dp ? 1 : 0)), (unsigned)B), dim3(256), 0, st, a);
+    const int all = L.segs + (dp ? 1 : 0), most = (int)(((1 << 24) - 1) / B);   // a launch has fewer than 2^32 threads
+    for (a.seg0 = 0; a.seg0 < all; a.seg0 += most)
+        hipLaunchKernelGGL(distill_grad_kernel, dim3((unsigned)min(most, all - a.seg0), (unsigned)B), dim3(256), 0, st, a);
     SumArgs sa = {};
     if (dq || dp) {
         const Side gq{a.g, a.g, B, L.ldg, B, L.ldg}, gp{a.g, a.g, B, L.ldg, C, L.ldg};                       // fp32
