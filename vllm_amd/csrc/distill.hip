@@ -700,10 +700,10 @@ __device__ __forceinline__ bool gemm_mix(const GemmArgs& g, int item, char* smem
 }
 
 // A stage is on its way into one LDS buffer while the other is multiplied, and no register holds it in between.  512 x 16384 x 3584 in
-// bf16: scores 68 us, gradients 131 us (0.88 and 1.0 PFLOP/s; a large product of a library 1.38).  Measured and left: a third buffer (one
+// bf16: scores 69 to 72 us, gradients 127 to 132 us (0.86 and 1.0 PFLOP/s; a large product of a library 1.38).  Measured and left: a third buffer (one
 // workgroup a CU less: 112 and 159 us), wave tiles of 128 x 64, one wave a SIMD, with the fragments' reads and the loads spread among the
-// MFMAs by hand (4 % of the scores' time), and the loads alone spread (slower).  What bounds it: MFMAs are busy 46 to 51 % of the clocks, at
-// 1.95 GHz (the power limit); waves wait 28 % of theirs for a stage.
+// MFMAs by hand (4 % of the scores' time), and the loads alone spread (slower).  What bounds it: MFMAs are busy 46 to 51 % of the clocks; the
+// waves wait 28 % of theirs for a stage, whose loads have the one before to arrive in, and 38 % for their turn to issue.
 template <class C>
 __device__ __forceinline__ bool gemm_straight(const GemmArgs& g, int item, char* smem) {
     GEMM_BEGIN(C::KB * 32)
@@ -1135,8 +1135,8 @@ __global__ __launch_bounds__(256) void distill_row_kernel(const RowArgs a) {
 }
 
 // ---- softmax - target ----------------------------------------------------------------------------------------------------
-// HBM-bound: the logits once, g once, in the form that the products take (512 x 16 384: 67 MB in 15.5 us, 4.3 TB/s).  One workgroup more a row
-// copies its query for the candidates' product.
+// HBM-bound: the logits once, g once, in the form that the products take (512 x 16 384: 67 MB in 16.5 us).  One workgroup more a row copies its
+// query for the candidates' product (1.2 us of them, 7 MB).
 enum { G_F32, G_F16, G_BF16 };
 struct GradArgs {
     const float* s;                  // [B][lds]
@@ -1450,7 +1450,7 @@ typedef CfgMix<DmaKC<2, 256, 512>, LoadKS<2, 128, 1, 512>, 256, 128, 512, 0> Gra
 typedef CfgDma<DmaKS<2, 256, 512>, DmaKS<2, 128, 512>, 2, 2, 256, 128, 512, true, false> GradPH256;
 
 // 256 rows of a side in one tile, by eight waves, instead of two tiles of 128: fp32 values of the other side are read and split half
-// as often (256 x 32768 x 4096: scores 221 us for 249, gradients 294 for 311).  Taken where at most a fifth more rows are computed for it.
+// as often (256 x 32768 x 4096, with the kernels around them: scores 221 us for 249, gradients 294 for 311).  Taken where at most a fifth more rows are computed for it.
 static GemmArgs tall(GemmArgs g) {
     g.nm = (int)tiles_of(g.a.rows, 256);
     return g;

@@ -397,8 +397,10 @@ __device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uin
 // fp32.  A group's sum is scaled once.  The loads of the next four pieces (the next tile's, at a tile's end) are on their way while
 // four are multiplied: 4 KB a wave, 64 KB a CU.  Scales come 16 bytes a lane, 32 of a row at a time, and go through a strip of LDS
 // of the wave's own (read where they are needed, 2 bytes a lane, they cost a third of the time: every access touches 16 lines).
-// 1 x 412 500 x 4096: 149 us, 5.8 TB/s.  With more queries MFMAs, sums and the fragments' LDS reads come to bound it: 103 000 x 4096, 1 / 6 / 13 fp32 queries 41 /
-// 69 / 88 us, 16 / 32 / 64 bf16 46 / 75 / 130 us.
+// 1 x 412 500 x 4096: 149 us, 5.8 TB/s.  More queries than LDS holds whole (fp32: more than 4 of 4096 values, 16 of 1000; bf16: more than 16 of
+// 4096) go in slices of the row: for every round of tiles each slice is read, split and put into LDS again between two barriers, and the
+// loads of codes do not go on across them.  That is the step in 103 000 x 4096, 1 / 4 / 6 / 13 fp32 queries 36 / 39 / 61 / 76 us, 16 / 32 / 64 bf16 42 / 63 /
+// 121 us (412 500 rows: 150 / 165 / 246 / 304 and 186 / 266 / 441).
 #define SCORE_WAVES 16               // a workgroup: all that a CU holds of this kernel, so that the queries stand in its LDS once
 #define SCORE_STRIP 1280             // bytes of scales a wave: 16 rows of 32, 80 bytes apart
 // between a query part's rows in LDS.  64, with the four 16-byte chunks of a fragment's 64 bytes permuted with the row: a fragment's 16 lanes
@@ -674,7 +676,7 @@ extern "C" int abc_store_scores(int q_dtype, const void* q, int64_t ldq, int64_t
             if (slice > chunks) slice = chunks;
         };
         fit();
-        // several waves a tile where there are fewer than 2048 (1 x 5000 x 3584: 6.6 us, one wave a tile 16.5; 1 x 30 000: 15.0 and 17.2; beyond, 1 x
+        // several waves a tile where there are fewer than 2048 (1 x 5000 x 3584: 6.9 us, one wave a tile 16.5; 1 x 30 000: 15.0 and 17.2; beyond, 1 x
         // 40 000: 17.2, two waves a tile 18.3)
         if (tiles < 2048 && chunks > 1) {
             red = (size_t)SCORE_WAVES * nt * 64 * (full ? 16 : 4);
